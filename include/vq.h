@@ -229,6 +229,59 @@ int vq_attention_seg_tiled(const float *q, const void *kc, const void *vc, float
                            int nseg, int heads, int kv_heads, int hd, const int32_t *page_table, int page_size,
                            int pages_per_seq, void *stream);
 
+/* ---- the KV cache in 4 bits ------------------------------------------------------------------------------
+ * 18 bytes for 32 values instead of 64 (fp16). The head dims of a (token, kv head) are quantized in groups of 32: a scale d, an
+ * f16 of at most 7 significant bits (a multiple of 2^-20 below 2^-14), a zero point z and codes c, both in 0 .. 15; a code
+ * stands for d (c - z), which is exactly an f16. d is the smallest such value with 15 d >= max(x, 0) - min(x, 0), at most 4352
+ * (values past 15 d read back as 15 d's end of the range); z = rint(-min(x, 0) / d), c = rint(x / d) + z cut to 0 .. 15, ties to
+ * even. A value is off by d / 2 at most. A row of k or v that holds a value that is not finite becomes a K row of NaN and a V
+ * row of zeros: every query that sees the position gets NaN, the others are not touched.
+ *
+ * A block is the P positions of one kv head in one page (P = page_size) or in a contiguous cache (P = max_seq rounded up to a
+ * multiple of 8): code words (u32; element 2 i of the word's eight at bits 4 i, element 2 i + 1 at bits 16 + 4 i), then headers
+ * (u16: the bits of d, whose low four are zero, with z in them).
+ *   K  words [P][4][hd / 32]: word (g, u) holds dims 32 u + 8 g .. + 7;  headers [P][hd / 32]
+ *   V  words [P / 8][hd]: a word holds positions 8 s .. 8 s + 7 of one dim, dim d at ((d / 16w) * 16 + d % 16) * w + (d / 16) % w
+ *      with w = 4 where hd is a multiple of 64, else 2;  headers [P / 8][hd / 32][8]
+ * A pool is [page][kv_head] blocks, a contiguous cache [kv_head] blocks. hd is a multiple of 32 up to 256, page_size a multiple of
+ * 8; zeroed memory reads as zeros. Caches are 16-byte aligned. `pages` is the pool's page count: a table entry outside [0, pages)
+ * is not followed: nothing is written through it, and its positions read as NaN. */
+
+/* Bytes of a cache of `blocks` blocks of `positions` positions (rounded up to a multiple of 8) of hd dims; 0 for an invalid
+ * shape. */
+size_t vq_kv4_bytes(long long blocks, int positions, int hd);
+
+/* vq_kv_append / vq_kv_append_seg into 4-bit caches. Segments of one slot may meet inside a word of V (their positions must not
+ * overlap). No counterpart in the reference, whose caches are fp32 or fp16 (qwen_runtime.cu:115-128, 2419-2447). */
+int vq_kv4_append(const float *k, const float *v, void *kc, void *vc, int ntok, int kv_heads, int max_seq, int hd, int pos0,
+                  void *stream);
+int vq_kv4_append_seg(const float *k, const float *v, void *kc, void *vc, const int32_t *segs, int nseg, int kv_heads, int hd,
+                      const int32_t *page_table, int page_size, int pages_per_seq, int pages, void *stream);
+
+/* The inverse: the values that the caches hold at the rows' positions into k, v [rows][kv_heads][hd] fp32 (a prefix saved to host
+ * memory, a cache looked into). No counterpart in the reference. */
+int vq_kv4_read(const void *kc, const void *vc, float *k, float *v, int ntok, int kv_heads, int max_seq, int hd, int pos0,
+                void *stream);
+int vq_kv4_read_seg(const void *kc, const void *vc, float *k, float *v, const int32_t *segs, int nseg, int kv_heads, int hd,
+                    const int32_t *page_table, int page_size, int pages_per_seq, int pages, void *stream);
+
+/* Workspace bytes of vq_attention4_ws / vq_attention4_seg_ws for these shapes; 0 for passes that take none, and for invalid
+ * arguments. */
+size_t vq_attention4_workspace_bytes(int heads, int kv_heads, int hd, int seq_len, int ntok, int window);
+size_t vq_attention4_seg_workspace_bytes(const int32_t *segs, int nseg, int heads, int kv_heads, int hd);
+
+/* vq_attention / vq_attention_seg over 4-bit caches: the products are exact f16 products of the cache's values with the query
+ * and the softmax weights as f16 pairs (22 significant bits), sums in fp32. With a workspace (16-byte aligned, >= the matching
+ * query, else VQ_ERR_WORKSPACE) a context may be cut into chunks that are merged in chunk order (deterministic); with NULL each
+ * row's keys are walked in one order, which does not depend on the other rows of the pass (the batch-invariant mode). No
+ * counterpart in the reference (its attention reads fp32 and fp16 caches, qwen_runtime.cu:128-162, 2449-2478). */
+int vq_attention4_ws(const float *q, const void *kc, const void *vc, float *out, int heads, int kv_heads, int hd, int max_seq,
+                     int seq_len, int ntok, int bidirectional, int window, void *workspace, size_t workspace_bytes,
+                     void *stream);
+int vq_attention4_seg_ws(const float *q, const void *kc, const void *vc, float *out, const int32_t *segs, int nseg, int heads,
+                         int kv_heads, int hd, const int32_t *page_table, int page_size, int pages_per_seq, int pages,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
 /* Causal depthwise conv + SiLU over ntok tokens: per channel the state [channels][K] (K <= VQ_CONV_MAX_K) holds
  * the last K inputs; per token it shifts, appends x[t][c], and out[t][c] = silu(state . w[c]). snap (may be
  * NULL): [ntok - 1][channels][K] states after each token but the last. write_state = 0 leaves the state

@@ -284,3 +284,53 @@ def gather_paged(pool: np.ndarray, pt_row, page_size: int, kv_heads: int, length
     hd = pool.shape[-1]
     flat = pool.reshape(-1, hd)
     return np.stack([flat[paged_rows(pt_row, page_size, kv_heads, h, np.arange(length))] for h in range(kv_heads)])
+
+
+# ---- the KV cache in 4 bits (layout and rounding rule: include/vq.h; no counterpart in the reference) ---------------
+
+
+def kv4_quantize(x):
+    """Codes uint8 [..., hd], scales float64 and zero points uint8 [..., hd / 32] of finite x [..., hd]: the scale is looked up
+    among all f16 values of at most 7 significant bits whose multiples by 15 are finite."""
+    a = np.asarray(x, np.float64)
+    g = a.reshape(*a.shape[:-1], -1, 32)
+    grid = np.arange(0, 0x7C00, 16, dtype=np.uint16).view(np.float16).astype(np.float64)
+    grid = grid[15 * grid <= 65504]
+    lo, hi = np.minimum(g.min(-1), 0.0), np.maximum(g.max(-1), 0.0)
+    d = grid[np.minimum(np.searchsorted(15 * grid, hi - lo), grid.size - 1)]
+    by = np.where(d > 0, d, 1.0)
+    z = np.minimum(np.rint(-lo / by), 15)
+    c = np.clip(np.rint(g / by[..., None]) + z[..., None], 0, 15)
+    return c.reshape(a.shape).astype(np.uint8), d, z.astype(np.uint8)
+
+
+def kv4_values(k, v):
+    """float64 values that the caches hold of rows k, v [..., hd]; a row with a value that is not finite: NaN and zeros."""
+    out = []
+    ok = np.isfinite(k).all(-1) & np.isfinite(v).all(-1)
+    for x, broken in ((k, np.nan), (v, 0.0)):
+        c, d, z = kv4_quantize(np.where(ok[..., None], x, 0))
+        w = (np.repeat(d, 32, -1) * (c.astype(np.float64) - np.repeat(z, 32, -1)))
+        out.append(np.where(ok[..., None], w, broken))
+    return out
+
+
+def _kv4_words(c):
+    """uint32 words of codes [..., 8]."""
+    e = np.arange(8)
+    return (c.astype(np.uint64) << (4 * (e // 2) + 16 * (e % 2)).astype(np.uint64)).sum(-1).astype(np.uint32)
+
+
+def kv4_block(x, values: bool) -> np.ndarray:
+    """Bytes of a K block (values: of a V block) of finite x [P][hd], P a multiple of 8."""
+    p, hd = x.shape
+    c, d, z = kv4_quantize(x)
+    h = d.astype(np.float16).view(np.uint16) | z
+    if not values:
+        return np.concatenate([_kv4_words(c.reshape(p, hd // 32, 4, 8)).transpose(0, 2, 1).copy().view(np.uint8).reshape(-1),
+                               h.view(np.uint8).reshape(-1)])
+    w, dim = 4 if hd % 64 == 0 else 2, np.arange(hd)
+    words = np.zeros((p // 8, hd), np.uint32)
+    words[:, ((dim // (16 * w)) * 16 + dim % 16) * w + dim // 16 % w] = _kv4_words(c.reshape(p // 8, 8, hd).transpose(0, 2, 1))
+    h = h.reshape(p // 8, 8, hd // 32).transpose(0, 2, 1).copy()
+    return np.concatenate([words.view(np.uint8).reshape(-1), h.view(np.uint8).reshape(-1)])

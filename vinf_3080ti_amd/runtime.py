@@ -73,11 +73,13 @@ WEIGHT_GRANULE = 2 << 20
 
 @dataclass
 class _Buffer:
-    data: torch.Tensor  # float32 or float16
+    data: torch.Tensor  # float32, float16 or, for a 4-bit cache, uint8
     elem: int
     # data was handed out (buffer_tensor): its storage may be exchanged or resized, so every use asks for the address
     # (0.1 us), and for the size where that has changed. A storage that is this entry's alone keeps both.
     lent: bool = False
+    # A 4-bit KV cache (alloc_kv4): its blocks, positions of a block and head dims. elem is 1 then: sizes are in bytes.
+    kv4: tuple[int, int, int] | None = None
 
     def __post_init__(self) -> None:
         self.address = self.data.data_ptr
@@ -222,7 +224,7 @@ class Runtime:
         if b.lent and b.address() != b.ptr:
             b.look_again()
         if b.elem != 4:
-            raise TypeError(f"device buffer {name} is fp16 (KV cache), not fp32")
+            raise TypeError(f"device buffer {name} is {'fp16' if b.elem == 2 else '4-bit'} (KV cache), not fp32")
         if b.n < min_n:
             raise ValueError(f"device buffer {name} has {b.n} floats, need {min_n}")
         return b
@@ -422,6 +424,19 @@ class Runtime:
         dtype = torch.float32 if elem == 4 else torch.float16
         self.buffers[name] = _Buffer(torch.zeros(int(n), dtype=dtype, device=self.device), elem)
 
+    def alloc_kv4(self, name: str, blocks: int, positions: int, hd: int) -> None:
+        """Zeroed K or V cache in 4 bits (layout: include/vq.h), 4.5 bits a value with its scales: `blocks` blocks of
+        `positions` positions of hd dims (a multiple of 32 up to 256). A contiguous cache has kv_heads blocks of max_seq
+        positions (rounded up to a multiple of 8), a page pool pages * kv_heads blocks of page_size positions (a multiple of 8).
+        kv_append, attention and their _seg forms take it as they take fp32 and fp16 caches, K and V both in 4 bits; to write,
+        read, copy and zero it is a buffer of bytes. No counterpart in the reference, whose caches are fp32 or fp16."""
+        fits = 0 < blocks < 1 << 48 and 0 < positions < 1 << 31 and 0 < hd < 1 << 31
+        n = self._lib.vq_kv4_bytes(blocks, positions, hd) if fits else 0
+        if not n:
+            raise ValueError(f"4-bit cache {name}: invalid shape ({blocks} blocks, {positions} positions, {hd} dims)")
+        data = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        self.buffers[name] = _Buffer(data, 1, kv4=(int(blocks), -(-int(positions) // 8) * 8, int(hd)))
+
     def zero(self, name: str) -> None:
         buf = self._any_buffer(name)
         _lib.check(self._lib.vq_zero(buf.data.data_ptr(), buf.data.numel() * buf.elem, self._stream()), "zero")
@@ -607,6 +622,11 @@ class Runtime:
         n, cache = kv_heads * hd * ntok, kv_heads * hd * max_seq
         kb, vb = self._f32_buffer(k, n), self._f32_buffer(v, n)
         kcb, vcb = self._any_buffer(kc), self._any_buffer(vc)
+        if kcb.kv4 or vcb.kv4:
+            self._kv4_pair(kc, kcb, vc, vcb, kv_heads, max_seq, hd)
+            _lib.check(self._lib.vq_kv4_append(kb.ptr, vb.ptr, kcb.ptr, vcb.ptr, ntok, kv_heads, max_seq, hd, pos,
+                                               self._stream()), "kv_append")
+            return
         for name, b in ((kc, kcb), (vc, vcb)):
             if b.n < cache:
                 raise ValueError(f"device buffer {name} has {b.n} values, need {cache}")
@@ -627,6 +647,16 @@ class Runtime:
         n, cache = heads * hd * ntok, kv_heads * hd * max_seq
         qb = self._f32_buffer(q, n)
         kcb, vcb = self._any_buffer(kc), self._any_buffer(vc)
+        if kcb.kv4 or vcb.kv4:
+            self._kv4_pair(kc, kcb, vc, vcb, kv_heads, max_seq, hd)
+            ob = self._f32_buffer(out, n)
+            nws = 0
+            if not self.batch_invariant:
+                nws = self._lib.vq_attention4_workspace_bytes(heads, kv_heads, hd, seq_len, ntok, int(window))
+            st = self._launch(nws, self._lib.vq_attention4_ws, qb.ptr, kcb.ptr, vcb.ptr, ob.ptr, heads, kv_heads, hd, max_seq,
+                              seq_len, ntok, int(bidirectional), int(window))
+            _lib.check(st, "attention")
+            return
         for name, b in ((kc, kcb), (vc, vcb)):
             if b.n < cache:
                 raise ValueError(f"device buffer {name} has {b.n} values, need {cache}")
@@ -770,6 +800,46 @@ class Runtime:
             raise TypeError("K and V caches differ in precision")
         return kcb, vcb
 
+    def _kv4_pair(self, kc: str, kcb: _Buffer, vc: str, vcb: _Buffer, kv_heads: int, positions: int, hd: int) -> int:
+        """Check a 4-bit cache pair against a call's shape (positions of a block: max_seq, or page_size); returns the pages that
+        both hold."""
+        if not (kcb.kv4 and vcb.kv4):
+            raise TypeError("K and V caches differ in precision")
+        blocks = min(kcb.kv4[0], vcb.kv4[0])
+        for name, b in ((kc, kcb), (vc, vcb)):
+            if b.kv4[1] != -(-positions // 8) * 8 or b.kv4[2] != hd:
+                raise ValueError(f"4-bit cache {name} has blocks of {b.kv4[1]} positions of {b.kv4[2]} dims, not {positions} of {hd}")
+            if b.lent and b.n < self._lib.vq_kv4_bytes(*b.kv4):
+                raise ValueError(f"device buffer {name} has {b.n} bytes, need {self._lib.vq_kv4_bytes(*b.kv4)}")
+        if kv_heads < 1 or blocks < kv_heads:
+            raise ValueError(f"4-bit caches {kc}, {vc} hold {blocks} blocks, need {kv_heads}")
+        return blocks // kv_heads
+
+    def kv4_read(self, kc: str, vc: str, k: str, v: str, kv_heads: int, max_seq: int, hd: int, pos: int, ntok: int = 1) -> None:
+        """The values that contiguous 4-bit caches hold at positions pos .. pos + ntok - 1 into k, v [ntok][kv_heads][hd] fp32:
+        kv_append the other way. No counterpart in the reference."""
+        if ntok < 1 or pos < 0 or pos + ntok > max_seq:
+            raise ValueError(f"positions [{pos}, {pos + ntok}) outside KV cache of {max_seq}")
+        n = kv_heads * hd * ntok
+        kb, vb = self._f32_buffer(k, n), self._f32_buffer(v, n)
+        kcb, vcb = self._any_buffer(kc), self._any_buffer(vc)
+        self._kv4_pair(kc, kcb, vc, vcb, kv_heads, max_seq, hd)
+        _lib.check(self._lib.vq_kv4_read(kcb.ptr, vcb.ptr, kb.ptr, vb.ptr, ntok, kv_heads, max_seq, hd, pos, self._stream()),
+                   "kv4_read")
+
+    def kv4_read_seg(self, kc: str, vc: str, k: str, v: str, kv_heads: int, hd: int) -> None:
+        """The values that paged 4-bit caches hold at each segment's positions into the segment's rows of k, v: kv_append_seg the
+        other way. No counterpart in the reference."""
+        self._seg_ready()
+        n = kv_heads * hd * self._seg_rows()
+        kb, vb = self._f32_buffer(k, n), self._f32_buffer(v, n)
+        kcb, vcb = self._any_buffer(kc), self._any_buffer(vc)
+        pt, page, pps = self._page_table()
+        pages = self._kv4_pair(kc, kcb, vc, vcb, kv_heads, page, hd)
+        for arr, count in self._seg_tables:
+            _lib.check(self._lib.vq_kv4_read_seg(kcb.ptr, vcb.ptr, kb.ptr, vb.ptr, arr, count, kv_heads, hd, pt, page, pps, pages,
+                                                 self._stream()), "kv4_read_seg")
+
     def rope_seg(self, x: str, heads: int, hd: int, rot: int, base: float) -> None:
         """NeoX RoPE with each segment's positions (Runtime_rope_seg, qwen_runtime.cu:2400-2417)."""
         self._seg_ready()
@@ -788,6 +858,12 @@ class Runtime:
         kb, vb = self._f32_buffer(k, rowsz * self._seg_rows()), self._f32_buffer(v, rowsz * self._seg_rows())
         kcb, vcb = self._kv_pair(kc, vc, rowsz)
         pt, page, pps = self._page_table()
+        if kcb.kv4:
+            pages = self._kv4_pair(kc, kcb, vc, vcb, kv_heads, page, hd)
+            for arr, n in self._seg_tables:
+                _lib.check(self._lib.vq_kv4_append_seg(kb.ptr, vb.ptr, kcb.ptr, vcb.ptr, arr, n, kv_heads, hd, pt, page, pps,
+                                                       pages, self._stream()), "kv_append_seg")
+            return
         for arr, n in self._seg_tables:
             _lib.check(self._lib.vq_kv_append_seg(kb.ptr, vb.ptr, kcb.ptr, vcb.ptr,
                                                   kcb.elem, arr, n, kv_heads, hd, pt, page, pps,
@@ -804,6 +880,14 @@ class Runtime:
         kcb, vcb = self._kv_pair(kc, vc, 1)
         ob = self._f32_buffer(out, rowsz * self._seg_rows())
         pt, page, pps = self._page_table()
+        if kcb.kv4:
+            pages = self._kv4_pair(kc, kcb, vc, vcb, kv_heads, page, hd)
+            for arr, n in self._seg_tables:
+                nws = 0 if self.batch_invariant else self._lib.vq_attention4_seg_workspace_bytes(arr, n, heads, kv_heads, hd)
+                st = self._launch(nws, self._lib.vq_attention4_seg_ws, qb.ptr, kcb.ptr, vcb.ptr, ob.ptr, arr, n, heads, kv_heads,
+                                  hd, pt, page, pps, pages)
+                _lib.check(st, "attention_seg")
+            return
         tiled = self._tiled_attention(self._seg_longest)
         for arr, n in self._seg_tables:
             if tiled:  # prompt rows in the pass, or batch-invariant mode
@@ -1076,10 +1160,15 @@ class HipWeightRuntime:
 
     def read_floats(self, name: str, n: int = -1, offset: int = 0) -> list[float]:
         """A buffer's elements as Python floats; fp16 buffers (KV caches) are widened exactly."""
-        width = "<f2" if self._rt.buffer_elem(name) == 2 else "<f4"
+        elem = self._rt.buffer_elem(name)
+        if elem == 1:
+            raise TypeError(f"device buffer {name} is a 4-bit KV cache: kv4_read gives its values")
+        width = "<f2" if elem == 2 else "<f4"
         return np.frombuffer(self._rt.read(name, n, offset), dtype=width).tolist()
 
     def write_floats(self, name: str, values, offset: int = 0) -> None:
+        if name in self._rt.buffers and self._rt.buffer_elem(name) == 1:
+            raise TypeError(f"device buffer {name} is a 4-bit KV cache: kv_append writes its values")
         self._rt.write(name, np.ascontiguousarray(values, dtype="<f4").tobytes(), offset)
 
     def __getattr__(self, name: str):
