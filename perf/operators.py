@@ -412,7 +412,7 @@ def _plain_verify(s):
     # In 64 bits: of 248320 tokens many have less than 1e-8 of the mass, and a random number falls between their borders.
     top, best = logits.max(1)
     t = s["temp"][seq, None]
-    p = torch.exp((logits - top[:, None]).double() / torch.where(t > 0, t, torch.ones_like(t)))
+    p = torch.exp((logits.double() - top[:, None]) / torch.where(t > 0, t, torch.ones_like(t)))
     p /= p.sum(1, keepdim=True)
     one = torch.zeros_like(p).scatter_(1, best[:, None], 1.0)
     p = torch.where(t > 0, p, one)
