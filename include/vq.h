@@ -282,6 +282,15 @@ int vq_attention4_seg_ws(const float *q, const void *kc, const void *vc, float *
                          int kv_heads, int hd, const int32_t *page_table, int page_size, int pages_per_seq, int pages,
                          void *workspace, size_t workspace_bytes, void *stream);
 
+/* Page work of paged caches, in one launch where it fits (32 pools, 192 copies, 192 entries): for every copies[i] = (from, to) the
+ * page `to` of each of the npools pools gets page `from`'s bytes (pool p: `pages` pages of page_bytes[p] bytes from pools[p]), and
+ * for every entries[i] = (index, page) page_table[index] = page. pools, page_bytes, copies ([ncopies][2]) and entries
+ * ([nentries][2]) are host arrays, read before the call returns; either list may be empty. No page may be written twice or both
+ * read and written (VQ_ERR_ARG); pages and indices outside their ranges: VQ_ERR_SHAPE; nothing is launched then. No counterpart
+ * in the reference, whose page table is written by its caller (set_paging, qwen_runtime.cu:2333-2350). */
+int vq_move_pages(void *const *pools, const size_t *page_bytes, int npools, int pages, const int32_t *copies, int ncopies,
+                  int32_t *page_table, int table_entries, const int32_t *entries, int nentries, void *stream);
+
 /* Causal depthwise conv + SiLU over ntok tokens: per channel the state [channels][K] (K <= VQ_CONV_MAX_K) holds
  * the last K inputs; per token it shifts, appends x[t][c], and out[t][c] = silu(state . w[c]). snap (may be
  * NULL): [ntok - 1][channels][K] states after each token but the last. write_state = 0 leaves the state

@@ -58,6 +58,7 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "vq_attention4_seg_workspace_bytes": (SZ, [P, I, I, I, I]),
     "vq_attention4_ws": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, SZ, P]),
     "vq_attention4_seg_ws": (I, [P, P, P, P, P, I, I, I, I, P, I, I, I, P, SZ, P]),
+    "vq_move_pages": (I, [P, P, I, I, P, I, P, I, P, I, P]),
     "vq_conv_update": (I, [P, P, P, P, I, I, I, P, I, P]),
     "vq_conv_update_seg": (I, [P, P, P, P, I, I, P, I, P, I, P]),
     "vq_gated_delta": (I, [P, P, P, P, P, P, I, P, I, I, I, I, F, I, I, P, I, P]),

@@ -28,7 +28,8 @@ HIPCC_FLAGS = [
 
 
 def sources() -> list[Path]:
-    return [CSRC / "vq_api.hip", CSRC / "vq_ops.hip", CSRC / "vq_kv4.hip"] + sorted(CSRC.glob("vq_t_*.hip"))
+    units = ("vq_api", "vq_ops", "vq_kv4", "vq_pages")
+    return [CSRC / f"{u}.hip" for u in units] + sorted(CSRC.glob("vq_t_*.hip"))
 
 
 def headers() -> list[Path]:

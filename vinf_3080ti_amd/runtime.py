@@ -27,6 +27,7 @@ import torch
 
 from . import _lib
 from .gguf_types import HIP_MATVEC_TYPES, GGUFTensorType, traits
+from .pages import PageBook, as_pairs
 
 MAX_TOKENS = 8  # tokens per matvec launch (kMaxTokens, qwen_runtime.cu:572)
 MAX_ARGMAX_ROWS = 256  # kMaxArgmaxRows (qwen_runtime.cu:573)
@@ -175,6 +176,8 @@ class Runtime:
         self._segments: list[tuple[int, int, int, int]] = []
         self._seg_tables: list[tuple[ctypes.Array, int]] = []  # as int32 tables of one launch each
         self._seg_span = self._seg_longest = 0
+        self._pages: tuple[PageBook, dict[str, int]] | None = None  # the book, and bytes of a page of each pool
+        self._pages_lock = threading.Lock()
         # Resident-weight memory: an optional arena and the executor's per-layer weight groups. Nothing streams
         # over PCIe here, so the stream order only records which uploads were requested as streamed.
         self._arena: _Region | None = None
@@ -743,7 +746,94 @@ class Runtime:
         if page_size < 1 or pages_per_seq < 1 or max_slots < 1:
             raise ValueError("invalid paging shape")
         pt = self._f32_buffer(page_table, pages_per_seq * max_slots)
-        self._paging = (pt, int(page_size), int(pages_per_seq), int(max_slots))
+        paging = (pt, int(page_size), int(pages_per_seq), int(max_slots))
+        if self._paging is not None and (self._paging[0] is not pt or self._paging[1:] != paging[1:]):
+            self._pages = None  # another table: set_page_pools again
+        self._paging = paging
+
+    # Pages of the caches as the runtime deals them: the pages_* calls keep the book of who holds which (pages.py) and write
+    # the page table, in stream order with the passes on the current stream. They are a scheduler's calls between passes, not for
+    # a captured graph (what they decided would be replayed).
+    def set_page_pools(self, pools: Sequence[str], pages: int) -> None:
+        """The runtime deals the pages from now on: `pools` are the caches (buffers of `pages` pages each, of any precision) that
+        share set_paging's page table, page i of one belonging to page i of every other. Every slot is empty then. set_paging with
+        another table or shape ends it. No counterpart in the reference, whose callers write the table."""
+        if self._paging is None:
+            raise RuntimeError("set_paging first")
+        names = list(pools)
+        if isinstance(pools, (str, bytes)) or len(set(names)) < len(names):
+            raise ValueError("pools are distinct buffer names")
+        if not 1 <= pages < 1 << 31:
+            raise ValueError("pages must be positive")
+        sizes = []
+        for name in names:
+            b = self._any_buffer(name)
+            n = self._lib.vq_kv4_bytes(*b.kv4) if b.kv4 else b.n * b.elem
+            if n % pages:
+                raise ValueError(f"device buffer {name} is not {pages} pages of one size")
+            sizes.append(n // pages)
+        _, page, per_slot, slots = self._paging
+        self._pages = (PageBook(int(pages), page, per_slot, slots), dict(zip(names, sizes)))
+
+    def _page_work(self, plan, what: str) -> int:
+        """plan(book) -> (copies, entries), then both on the device; returns the pages copied."""
+        if self._pages is None or self._paging is None:
+            raise RuntimeError("set_page_pools first")
+        with self._pages_lock:
+            book, pools = self._pages
+            ptrs = []
+            for name, size in pools.items():
+                b = self._any_buffer(name)
+                if b.n * b.elem < size * book.pages:
+                    raise ValueError(f"device buffer {name} has {b.n * b.elem} bytes, need {size * book.pages}")
+                ptrs.append(b.ptr)
+            table, _, _ = self._page_table()
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{what}: page work cannot be captured")
+            copies, entries = plan(book)
+            if copies or entries:
+                n, ca, ea = len(ptrs), as_pairs(copies), as_pairs(entries)
+                st = self._lib.vq_move_pages((ctypes.c_void_p * n)(*ptrs), (ctypes.c_size_t * n)(*pools.values()), n, book.pages,
+                                             ca.ctypes.data, len(copies), table, book.per_slot * book.slots, ea.ctypes.data,
+                                             len(entries), self._stream())
+                _lib.check(st, what)
+            return len(copies)
+
+    def pages_reserve(self, segments) -> None:
+        """Make the rows that a pass is about to write ((slot, pos0, rows, ...) as in set_segments) the slot's own: pages that it
+        lacks are taken, pages that it shares replaced by copies. ValueError when the pool has too few, and nothing changes."""
+        self._page_work(lambda book: book.reserve(segments), "pages_reserve")
+
+    def pages_fork(self, src: int, dst: Sequence[int], length: int) -> None:
+        """Empty slots dst begin as src's first `length` positions, in the same pages (pages_reserve parts them where one is
+        written)."""
+        self._page_work(lambda book: ([], book.fork(src, dst, length)), "pages_fork")
+
+    def pages_copy(self, pairs) -> None:
+        """(src, dst, length) each: empty slot dst gets a copy of src's first `length` positions in pages of its own."""
+        self._page_work(lambda book: book.copy(pairs), "pages_copy")
+
+    def pages_free(self, slots: Sequence[int], length: int = 0) -> None:
+        """The slots give back the pages behind their first `length` positions (all of them by default; after a verification that
+        refused drafts, those behind what was accepted). Table entries are left as they are."""
+        self._page_work(lambda book: (book.free(slots, length), ([], []))[1], "pages_free")
+
+    def pages_compact(self) -> int:
+        """Move pages so that those in use are the lowest ids; returns how many moved."""
+        return self._page_work(lambda book: book.compact(), "pages_compact")
+
+    def pages_of(self, slot: int) -> list[int]:
+        """The pages that a slot holds, in the order of its positions."""
+        if self._pages is None:
+            raise RuntimeError("set_page_pools first")
+        book = self._pages[0]
+        return list(book.rows[book._slot(slot)])
+
+    def pages_available(self) -> int:
+        """Pages that no slot holds."""
+        if self._pages is None:
+            raise RuntimeError("set_page_pools first")
+        return self._pages[0].available()
 
     def set_segments(self, segments) -> int:
         """Row layout of the next *_seg ops: [(slot, pos0, rows[, row0]), ...], rows of a segment being
