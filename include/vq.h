@@ -472,6 +472,26 @@ int vq_dequant_rows(int type, const uint8_t *w, int rows, int cols, float *out, 
  * Replaces: argmax_kernel + Runtime_argmax / Runtime_argmax_rows (qwen_runtime.cu:850-876, 2167-2197). */
 int vq_argmax_rows(const float *x, int n, int ntok, int32_t *out, void *stream);
 
+/* Verification of drafted tokens against the target's logits, and the token that follows. Sequence i < nseq has drafted[i] drafts
+ * (0 .. VQ_MAX_DRAFT) and drafted[i] + 1 rows of logits, the sequences' rows one after the other: logits [rows][vocab], draft [sum
+ * of drafted] token ids, probs [sum of drafted][vocab] the probabilities that each draft was drawn with (NULL: drafts were chosen
+ * without chance, all of the mass at the drafted token), u [rows][2] random numbers in [0, 1). drafted and temperature are host
+ * arrays.
+ * With p_j = softmax(l_j / temperature[i]), draft x_j is accepted while u[j][0] q_j(x_j) < p_j(x_j). At the first refusal the
+ * next token is drawn from max(0, p_j - q_j), normalised (from p_j where nothing of it is left), after all drafts from p_k: the
+ * first index whose cumulative weight exceeds u[j][1] times the total, else the last index that has weight. Weights and sums are
+ * in 64 bits. Temperature 0: all of the mass at the largest logit (ties -> lowest index). NaN logits count as -inf, probabilities
+ * that are negative or NaN as 0; a draft outside [0, vocab) is refused; a row without a logit above -inf gives INT32_MAX.
+ * tokens [rows]: the accepted drafts, the drawn token, -1 in the sequence's further rows; counts [nseq]: accepted drafts; logprobs
+ * (may be NULL) [rows]: log p_j of each token given (greedy: 0), 0 beside a -1. A sequence's results do not depend on the others.
+ * Workspace: 16-byte aligned, >= vq_verify_draft_workspace_bytes (0: invalid arguments), else VQ_ERR_WORKSPACE; one call at a
+ * time. Adds to: the row argmax that greedy verification uses (Runtime_argmax_rows, qwen_runtime.cu:2181-2197). */
+#define VQ_MAX_DRAFT 128
+size_t vq_verify_draft_workspace_bytes(int vocab, const int32_t *drafted, int nseq);
+int vq_verify_draft(const float *logits, const int32_t *draft, const float *probs, const float *u, int32_t *tokens, int32_t *counts,
+                    float *logprobs, int vocab, const int32_t *drafted, const double *temperature, int nseq, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

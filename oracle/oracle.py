@@ -334,3 +334,57 @@ def kv4_block(x, values: bool) -> np.ndarray:
     words[:, ((dim // (16 * w)) * 16 + dim % 16) * w + dim // 16 % w] = _kv4_words(c.reshape(p // 8, 8, hd).transpose(0, 2, 1))
     h = h.reshape(p // 8, 8, hd // 32).transpose(0, 2, 1).copy()
     return np.concatenate([words.view(np.uint8).reshape(-1), h.view(np.uint8).reshape(-1)])
+
+
+def verify_draft(logits, draft, probs, u, drafted, temperature):
+    """Verification of drafted tokens (the rule of vq_verify_draft in include/vq.h; the greedy case compares argmax_rows with the
+    drafts as qwen_speculative.py:211-222 does), in float64, row by row. Returns (tokens, counts, logprobs)."""
+    tokens, counts, logprobs = [], [], []
+    row = d = 0
+    for k, t in zip(drafted, temperature):
+        done = 0
+        for j in range(k + 1):
+            l = np.asarray(logits[row + j], np.float64)
+            l = np.where(np.isnan(l), -np.inf, l)
+            m = l.max()
+            if t == 0:
+                p = np.where(np.arange(l.size) == l.argmax(), 1.0, 0.0)
+                logp = np.zeros(l.size)
+            else:
+                e = np.where(l == m, 1.0, np.exp((np.where(l == m, 0, l) - (m if np.isfinite(m) else 0)) / t) if m < np.inf else 0.0)
+                p = e / e.sum()
+                with np.errstate(divide="ignore"):
+                    logp = np.log(p)
+            if m == -np.inf:
+                p = np.zeros(l.size)
+            if j < k:
+                x = int(draft[d + j])
+                ok = 0 <= x < l.size
+                q = np.zeros(l.size)
+                if probs is not None:
+                    q = np.where(np.asarray(probs[d + j]) > 0, probs[d + j], 0).astype(np.float64)
+                elif ok:
+                    q[x] = 1.0
+                if ok and (p[x] == 1.0 if t == 0 else float(u[row + j][0]) * q[x] < p[x]):
+                    tokens.append(x)
+                    logprobs.append(logp[x])
+                    continue
+                if t > 0:
+                    left = np.maximum(p - q, 0)
+                    p = left if left.sum() > 0 else p
+            done = j
+            if m == -np.inf:
+                tokens.append(2 ** 31 - 1)
+                logprobs.append(-np.inf)
+            else:
+                c = np.cumsum(p)
+                over = np.flatnonzero(c > float(u[row + j][1]) * c[-1])
+                x = int(over[0]) if over.size else int(np.flatnonzero(p > 0)[-1])
+                tokens.append(x)
+                logprobs.append(logp[x])
+            break
+        counts.append(done)
+        tokens += [-1] * (k - done)
+        logprobs += [0.0] * (k - done)
+        row, d = row + k + 1, d + k
+    return np.array(tokens, np.int32), np.array(counts, np.int32), np.array(logprobs)

@@ -17,6 +17,7 @@ VQ_QMV_ADD, VQ_QMV_NORM, VQ_QMV_SILU_MUL = 1, 2, 8
 
 # Sequence ops (include/vq.h).
 VQ_MAX_SEGMENTS, VQ_CONV_MAX_K = 64, 8
+VQ_MAX_DRAFT = 128
 
 # name -> (restype, argtypes); every symbol include/vq.h declares.
 SIGNATURES: dict[str, tuple[object, list]] = {
@@ -86,6 +87,8 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "vq_lmhead_argmax": (I, [I, P, I, I, P, I, P, P, P, SZ, P]),
     "vq_dequant_rows": (I, [I, P, I, I, P, P]),
     "vq_argmax_rows": (I, [P, I, I, P, P]),
+    "vq_verify_draft_workspace_bytes": (SZ, [I, P, I]),
+    "vq_verify_draft": (I, [P, P, P, P, P, P, P, I, P, P, I, P, SZ, P]),
 }
 
 VQ_OK, VQ_ERR_TYPE, VQ_ERR_SHAPE, VQ_ERR_WORKSPACE, VQ_ERR_ARG, VQ_ERR_NOT_INIT, VQ_ERR_TOO_LARGE = 0, -1, -2, -3, -4, -5, -6

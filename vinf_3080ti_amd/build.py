@@ -28,7 +28,7 @@ HIPCC_FLAGS = [
 
 
 def sources() -> list[Path]:
-    units = ("vq_api", "vq_ops", "vq_kv4", "vq_pages")
+    units = ("vq_api", "vq_ops", "vq_kv4", "vq_pages", "vq_verify")
     return [CSRC / f"{u}.hip" for u in units] + sorted(CSRC.glob("vq_t_*.hip"))
 
 

@@ -1,0 +1,370 @@
+// vq_verify.hip -- verification of drafted tokens against the target's logits from given random numbers, and sampling of the token
+// that follows them.
+//
+// Row j of a sequence gives p_j = softmax(l_j / T). Draft x_j is accepted while u_j q_j(x_j) < p_j(x_j); at the first refusal the
+// next token comes from max(0, p_j - q_j), normalised, and after all of them from p_k, by inverse CDF: the first index whose
+// cumulative weight exceeds v_j times the total. Everything from the exponent on is in 64 bits: a vocabulary of 248320 tokens
+// puts the borders of the cumulative sum 4e-6 apart on average and most of them far nearer, so sums of 32 bits would pick a
+// neighbour now and then, and no two orders of summation would agree.
+//
+// Three launches. Statistics: each row in chunks of kChunk logits, the chunk's maximum and sum of weights (one pass over the
+// logits, which bounds the whole). Residual: for the row where a sequence stopped, each chunk's sum of max(0, p - q); only where
+// something drafted may be refused. Pick: one workgroup per sequence finds the chunk by the chunks' sums, then the element. The
+// last two decide from the statistics what was accepted, each for itself. The chunks do not depend on the batch, so neither does
+// any bit of a sequence's results.
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include "../../include/vq.h"
+#include "vq_seq.h"
+
+namespace {
+
+constexpr int kThreads = 256, kEach = 8, kChunk = kThreads * kEach;
+
+struct VerSeq {
+    int row0, k;  // rows row0 .. row0 + k, the first k of them followed by drafts draft0 ..
+    int draft0;
+    double t;
+};
+struct VerTable {
+    int n;
+    VerSeq s[VQ_MAX_SEGMENTS];
+};
+
+// What a pass reads and writes; the workspace: statistics [row][chunk], residual sums [sequence][chunk].
+struct VerArgs {
+    const float *logits, *probs, *u;
+    const int32_t *draft;
+    int32_t *tokens, *counts;
+    float *logprobs;
+    double2 *stats;
+    double *residual;
+    int vocab, chunks;
+};
+
+// A logit as it counts: NaN never wins, like -inf.
+__device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY; }
+// exp((x - m) / T), 1 at the maximum whatever it is (all of the mass is at +inf where that is the maximum).
+__device__ __forceinline__ double weight(double x, double m, double inv_t) { return x == m ? 1.0 : exp((x - m) * inv_t); }
+
+// A thread's kEach neighbouring values from i on, `fill` past n.
+__device__ __forceinline__ void load_each(const float *p, int i, int n, float fill, float (&x)[kEach]) {
+    if (i + kEach <= n) {
+        __builtin_memcpy(x, p + i, sizeof(x));
+    } else {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) x[e] = i + e < n ? p[i + e] : fill;
+    }
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+// Over the workgroup's four waves, in wave order; every thread gets the result.
+__device__ __forceinline__ double group_sum(double v, double *lds) {
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return ((lds[0] + lds[1]) + lds[2]) + lds[3];
+}
+// Inclusive sum over the threads before and at this one.
+__device__ __forceinline__ double group_scan(double v, double *lds) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(v, o, 64);
+        if (lane >= o) v += up;
+    }
+    if (lane == 63) lds[wv] = v;
+    __syncthreads();
+    for (int w = 0; w < wv; ++w) v += lds[w];
+    return v;
+}
+
+// Workgroup (chunk, row): (maximum, sum of weights against it), for a greedy row (maximum, its lowest index).
+__global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerArgs a, VerTable T) {
+    __shared__ float smax[4];
+    __shared__ double ssum[4];
+    __shared__ int first;
+    int i = 0, row = blockIdx.y;
+    while (i + 1 < T.n && row > T.s[i].k) row -= T.s[i].k + 1, ++i;
+    const double t = T.s[i].t;
+    const int at = blockIdx.x * kChunk + threadIdx.x * kEach;
+    float x[kEach], m = -INFINITY;
+    load_each(a.logits + static_cast<size_t>(blockIdx.y) * a.vocab, at, a.vocab, -INFINITY, x);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) x[e] = logit(x[e]), m = fmaxf(m, x[e]);
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) smax[threadIdx.x >> 6] = m;
+    if (threadIdx.x == 0) first = INT_MAX;
+    __syncthreads();
+    m = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
+    double2 *out = a.stats + static_cast<size_t>(blockIdx.y) * a.chunks + blockIdx.x;
+    if (t == 0.0) {
+#pragma unroll
+        for (int e = kEach - 1; e >= 0; --e)
+            if (x[e] == m && m > -INFINITY) atomicMin(&first, at + e);
+        __syncthreads();
+        if (threadIdx.x == 0) *out = double2{m, static_cast<double>(first)};
+        return;
+    }
+    const double inv_t = 1.0 / t;
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) s += weight(x[e], m, inv_t);
+    s = group_sum(m > -INFINITY ? s : 0.0, ssum);
+    if (threadIdx.x == 0) *out = double2{m, s};
+}
+
+// What the statistics of a sequence's rows say: `stop`, the drafts accepted, and each row's maximum and total (greedy: its token).
+struct Decision {
+    int stop;
+    double m[VQ_MAX_DRAFT + 1], z[VQ_MAX_DRAFT + 1];
+};
+// Called by a whole workgroup; each wave takes rows in turn, its lanes the row's chunks.
+__device__ void decide(const VerArgs &a, const VerSeq &s, Decision &d) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const bool greedy = s.t == 0.0;
+    const double inv_t = greedy ? 0.0 : 1.0 / s.t;
+    if (threadIdx.x == 0) d.stop = s.k;
+    __syncthreads();
+    for (int j = wv; j <= s.k; j += kThreads / 64) {
+        const double2 *st = a.stats + static_cast<size_t>(s.row0 + j) * a.chunks;
+        double m = -INFINITY;
+        for (int c = lane; c < a.chunks; c += 64) m = fmax(m, st[c].x);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
+        double z;
+        if (greedy) {
+            z = static_cast<double>(INT_MAX);
+            for (int c = lane; c < a.chunks; c += 64)
+                if (st[c].x == m) z = fmin(z, st[c].y);
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) z = fmin(z, __shfl_xor(z, o, 64));
+        } else {
+            z = 0.0;
+            for (int c = lane; c < a.chunks; c += 64) z += st[c].y * weight(st[c].x, m, inv_t);
+            z = wave_sum(z);
+        }
+        if (lane == 0) {
+            d.m[j] = m;
+            d.z[j] = z;
+            if (j < s.k) {
+                const int x = a.draft[s.draft0 + j];
+                bool ok = x >= 0 && x < a.vocab;
+                if (ok && greedy) ok = x == static_cast<int>(z);
+                else if (ok) {
+                    const float l = logit(a.logits[static_cast<size_t>(s.row0 + j) * a.vocab + x]);
+                    double q = 1.0;
+                    if (a.probs) {
+                        const float given = a.probs[static_cast<size_t>(s.draft0 + j) * a.vocab + x];
+                        q = given > 0.0f ? given : 0.0;
+                    }
+                    ok = z > 0.0 && static_cast<double>(a.u[2 * static_cast<size_t>(s.row0 + j)]) * q * z < weight(l, m, inv_t);
+                }
+                if (!ok) atomicMin(&d.stop, j);
+            }
+        }
+    }
+    __syncthreads();
+}
+
+// Weights that the token after row j's accepted drafts is drawn with: the target's, or where a draft was refused what it has over
+// the draft's probabilities (a draft without probabilities: over all of the mass at the drafted token).
+struct Source {
+    const float *l, *q;  // q null: no draft's probabilities are taken off
+    int without;         // a token left out
+    double m, inv_t, inv_z;
+    __device__ __forceinline__ void each(int i, int n, double (&w)[kEach]) const {
+        float x[kEach], y[kEach];
+        load_each(l, i, n, -INFINITY, x);
+        if (q) load_each(q, i, n, 0.0f, y);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const double p = weight(logit(x[e]), m, inv_t) * inv_z;
+            w[e] = p;
+            if (q) w[e] = fmax(p - (y[e] > 0.0f ? static_cast<double>(y[e]) : 0.0), 0.0);
+            if (i + e >= n || i + e == without) w[e] = 0.0;
+        }
+    }
+};
+__device__ __forceinline__ Source source_of(const VerArgs &a, const VerSeq &s, const Decision &d, bool refused) {
+    const int j = d.stop;
+    Source r{a.logits + static_cast<size_t>(s.row0 + j) * a.vocab, nullptr, -1, d.m[j], 1.0 / s.t, 1.0 / d.z[j]};
+    if (refused) {
+        if (a.probs) r.q = a.probs + static_cast<size_t>(s.draft0 + j) * a.vocab;
+        else r.without = a.draft[s.draft0 + j];
+    }
+    return r;
+}
+
+// Workgroup (chunk, sequence): the chunk's sum of what is left over where a draft was refused.
+__global__ __launch_bounds__(kThreads) void verify_residual_kernel(VerArgs a, VerTable T) {
+    __shared__ Decision d;
+    __shared__ double ssum[4];
+    const VerSeq s = T.s[blockIdx.y];
+    if (s.k == 0 || s.t == 0.0) return;
+    decide(a, s, d);
+    if (d.stop == s.k || !(d.z[d.stop] > 0.0)) return;
+    double w[kEach], sum = 0.0;
+    source_of(a, s, d, true).each(blockIdx.x * kChunk + threadIdx.x * kEach, a.vocab, w);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sum += w[e];
+    sum = group_sum(sum, ssum);
+    if (threadIdx.x == 0) a.residual[static_cast<size_t>(blockIdx.y) * a.chunks + blockIdx.x] = sum;
+}
+
+// One workgroup per sequence: the token, and what the rows give.
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerArgs a, VerTable T) {
+    __shared__ Decision d;
+    __shared__ double scan[4], base, total;
+    __shared__ int chunk, last, token;
+    const VerSeq s = T.s[blockIdx.x];
+    const int tid = threadIdx.x;
+    decide(a, s, d);
+    const int j = d.stop;
+    const bool greedy = s.t == 0.0, some = greedy ? d.z[j] < INT_MAX : d.z[j] > 0.0;
+    const double inv_t = greedy ? 0.0 : 1.0 / s.t;
+    if (tid == 0) token = greedy && some ? static_cast<int>(d.z[j]) : INT_MAX;
+    if (!greedy && some) {
+        const double2 *st = a.stats + static_cast<size_t>(s.row0 + j) * a.chunks;
+        const double *left = a.residual + static_cast<size_t>(blockIdx.x) * a.chunks;
+        const double v = a.u[2 * static_cast<size_t>(s.row0 + j) + 1], inv_z = 1.0 / d.z[j];
+        const int per = (a.chunks + kThreads - 1) / kThreads, c0 = tid * per, c1 = min(c0 + per, a.chunks);
+        bool refused = j < s.k;
+        auto of_chunk = [&](int c) { return refused ? left[c] : st[c].y * weight(st[c].x, d.m[j], inv_t) * inv_z; };
+        for (;;) {
+            double mine = 0.0;
+            for (int c = c0; c < c1; ++c) mine += of_chunk(c);
+            const double upto = group_scan(mine, scan);
+            if (tid == kThreads - 1) total = upto;
+            if (tid == 0) chunk = INT_MAX, last = -1;
+            __syncthreads();
+            if (refused && !(total > 0.0)) {  // nothing is left over (p = q): from the target's own weights
+                refused = false;
+                __syncthreads();
+                continue;
+            }
+            // The first chunk whose cumulative sum exceeds the target, else the last with any weight.
+            const double target = v * total;
+            double before = upto - mine;
+            for (int c = c0; c < c1; ++c) {
+                const double w = of_chunk(c);
+                if (w > 0.0) atomicMax(&last, c);
+                before += w;
+                if (before > target) {
+                    atomicMin(&chunk, c);
+                    break;
+                }
+            }
+            __syncthreads();
+            if (chunk == INT_MAX && tid == 0) chunk = last;
+            __syncthreads();
+            before = upto - mine;
+            for (int c = c0; c < c1; ++c) {
+                if (c == chunk) base = before;
+                before += of_chunk(c);
+            }
+            __syncthreads();
+            // The same among the chunk's elements.
+            double w[kEach], in = 0.0;
+            const int at = chunk * kChunk + tid * kEach;
+            source_of(a, s, d, refused).each(at, a.vocab, w);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) in += w[e];
+            const double to = group_scan(in, scan);
+            if (tid == 0) last = -1;
+            __syncthreads();
+            before = base + (to - in);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                if (w[e] > 0.0) atomicMax(&last, at + e);
+                before += w[e];
+                if (before > target) {
+                    atomicMin(&token, at + e);
+                    break;
+                }
+            }
+            __syncthreads();
+            if (tid == 0 && token == INT_MAX) token = last >= 0 ? last : chunk * kChunk;
+            break;
+        }
+    }
+    __syncthreads();
+    for (int r = tid; r <= s.k; r += kThreads) {
+        const size_t row = static_cast<size_t>(s.row0) + r;
+        const int x = r < j ? a.draft[s.draft0 + r] : r == j ? token : -1;
+        a.tokens[row] = x;
+        if (!a.logprobs) continue;
+        float lp = 0.0f;
+        if (r == j && !some) lp = -INFINITY;
+        else if (r <= j && !greedy) {
+            const float l = logit(a.logits[row * a.vocab + x]);
+            lp = static_cast<float>((l == d.m[r] ? 0.0 : (l - d.m[r]) * inv_t) - log(d.z[r]));
+        }
+        a.logprobs[row] = lp;
+    }
+    if (tid == 0) a.counts[blockIdx.x] = j;
+}
+
+int make_pass(int vocab, const int32_t *drafted, const double *temperature, int nseq, VerTable &T, int &rows, int &drafts) {
+    if (!drafted || nseq < 1 || nseq > VQ_MAX_SEGMENTS) return VQ_ERR_ARG;
+    if (vocab < 1 || vocab > INT_MAX - 2 * kChunk) return VQ_ERR_SHAPE;
+    T.n = nseq;
+    rows = drafts = 0;
+    for (int i = 0; i < nseq; ++i) {
+        const double t = temperature ? temperature[i] : 1.0;
+        if (drafted[i] < 0 || drafted[i] > VQ_MAX_DRAFT || !(t >= 0.0 && t < INFINITY)) return VQ_ERR_SHAPE;
+        T.s[i] = VerSeq{rows, drafted[i], drafts, t};
+        rows += drafted[i] + 1;
+        drafts += drafted[i];
+    }
+    return VQ_OK;
+}
+size_t chunks_of(int vocab) { return (static_cast<size_t>(vocab) + kChunk - 1) / kChunk; }
+
+}  // namespace
+
+extern "C" {
+
+size_t vq_verify_draft_workspace_bytes(int vocab, const int32_t *drafted, int nseq) {
+    VerTable T;
+    int rows, drafts;
+    if (make_pass(vocab, drafted, nullptr, nseq, T, rows, drafts) != VQ_OK) return 0;
+    return chunks_of(vocab) * (sizeof(double2) * rows + sizeof(double) * nseq);
+}
+
+int vq_verify_draft(const float *logits, const int32_t *draft, const float *probs, const float *u, int32_t *tokens, int32_t *counts,
+                    float *logprobs, int vocab, const int32_t *drafted, const double *temperature, int nseq, void *workspace,
+                    size_t workspace_bytes, void *stream) {
+    if (!logits || !u || !tokens || !counts || !temperature) return VQ_ERR_ARG;
+    VerTable T;
+    int rows, drafts;
+    if (const int st = make_pass(vocab, drafted, temperature, nseq, T, rows, drafts); st != VQ_OK) return st;
+    if (drafts > 0 && !draft) return VQ_ERR_ARG;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+        workspace_bytes < vq_verify_draft_workspace_bytes(vocab, drafted, nseq))
+        return VQ_ERR_WORKSPACE;
+    const size_t chunks = chunks_of(vocab);
+    VerArgs a{logits, probs, u, draft, tokens, counts, logprobs, static_cast<double2 *>(workspace), nullptr, vocab,
+              static_cast<int>(chunks)};
+    a.residual = reinterpret_cast<double *>(a.stats + chunks * rows);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    verify_stats_kernel<<<dim3(chunks, rows), kThreads, 0, s>>>(a, T);
+    bool refusable = false;
+    for (int i = 0; i < nseq; ++i) refusable = refusable || (T.s[i].k > 0 && T.s[i].t > 0.0);
+    if (refusable) verify_residual_kernel<<<dim3(chunks, nseq), kThreads, 0, s>>>(a, T);
+    verify_pick_kernel<<<nseq, kThreads, 0, s>>>(a, T);
+    return status_of(hipGetLastError());
+}
+
+}  // extern "C"

@@ -1168,6 +1168,42 @@ class Runtime:
             _lib.check(self._lib.vq_argmax_rows(xb.ptr, n, ntok, sc.argmax_ptr, self._stream()), "argmax_rows")
             return sc.argmax[:ntok].tolist()
 
+    def verify_draft(self, logits: str, draft: str | None, uniforms: str, tokens: str, counts: str, vocab: int,
+                     drafted: Sequence[int], *, temperature: float | Sequence[float] = 1.0, probs: str | None = None,
+                     logprobs: str | None = None) -> None:
+        """Accept or refuse each sequence's drafted tokens against the target's logits and draw the token that follows, from given
+        random numbers (vq_verify_draft has the rule). Sequence i has drafted[i] drafts and drafted[i] + 1 rows, stacked in order:
+        logits [rows][vocab], draft int32 [sum(drafted)] (None where nothing is drafted: plain sampling), uniforms [rows][2] in
+        [0, 1), probs [sum(drafted)][vocab] what the drafts were drawn with (None: chosen without chance). temperature: one for
+        all or one each, 0 = greedy. Results, on the device (32-bit whole numbers by their bits, as in a page table): tokens
+        [rows], the accepted drafts, the drawn token, then -1; counts [sequences] accepted drafts; logprobs [rows]. The
+        reference's greedy verification compares argmax_rows with the drafts on the host (qwen_speculative.py:211-222)."""
+        ks = [int(k) for k in drafted]
+        if not ks or vocab < 1 or any(not 0 <= k <= _lib.VQ_MAX_DRAFT for k in ks):
+            raise ValueError(f"drafted must give 0 to {_lib.VQ_MAX_DRAFT} tokens for each sequence, of a positive vocab")
+        ts = [float(temperature)] * len(ks) if isinstance(temperature, (int, float)) else [float(t) for t in temperature]
+        if len(ts) != len(ks) or any(not 0.0 <= t < math.inf for t in ts):
+            raise ValueError("temperature must be one finite number >= 0, or one for each sequence")
+        total = sum(ks)
+        rows = total + len(ks)
+        if draft is None and total:
+            raise ValueError("drafted tokens need a draft buffer")
+        lb, ub = self._f32_buffer(logits, rows * vocab), self._f32_buffer(uniforms, 2 * rows)
+        tb, cb = self._f32_buffer(tokens, rows), self._f32_buffer(counts, len(ks))
+        dp = self._f32_buffer(draft, total).ptr if draft is not None else 0
+        pp = self._f32_buffer(probs, total * vocab).ptr if probs is not None else 0
+        op = self._f32_buffer(logprobs, rows).ptr if logprobs is not None else 0
+        row = d = 0
+        for i in range(0, len(ks), _lib.VQ_MAX_SEGMENTS):
+            part = ks[i:i + _lib.VQ_MAX_SEGMENTS]
+            n = len(part)
+            ka, ta = (ctypes.c_int32 * n)(*part), (ctypes.c_double * n)(*ts[i:i + n])
+            nws = self._lib.vq_verify_draft_workspace_bytes(vocab, ka, n)
+            st = self._launch(nws, self._lib.vq_verify_draft, lb.ptr + 4 * row * vocab, dp and dp + 4 * d, pp and pp + 4 * d * vocab,
+                              ub.ptr + 8 * row, tb.ptr + 4 * row, cb.ptr + 4 * i, op and op + 4 * row, vocab, ka, ta, n)
+            _lib.check(st, "verify_draft")
+            row, d = row + sum(part) + n, d + sum(part)
+
     def set_gemm_min_rows(self, n: int) -> None:
         """qmv calls with ntok >= n take the MFMA prefill contraction (0 = never) (qwen_runtime.cu:2324-2330)."""
         if n < 0:
