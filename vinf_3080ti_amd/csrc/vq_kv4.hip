@@ -207,68 +207,532 @@ __global__ __launch_bounds__(kMaxHd) void kv4_read_kernel(const uint8_t *__restr
 
 // ---- attention -----------------------------------------------------------------------------------------------
 
-// One workgroup of four waves per (head, row): wave w takes the 64-key chunks w, w + 4, ...; lane = key for q . k, lane = dims for
-// the sum over V; the waves' sums meet in wave order.
-constexpr int kWaves = 4;
-template <bool PAGED>
-__global__ __launch_bounds__(64 * kWaves) void attention4_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
-                                                                 const uint8_t *__restrict__ vc, float *__restrict__ out, SegTable T,
-                                                                 Map4 M, int heads, int hd, int bidirectional, int window) {
-    __shared__ float sq[kMaxHd], sp[kWaves][64], sm[kWaves], sl[kWaves], sacc[kWaves][kMaxHd];
-    int t;
-    const Seg &s = seg_of_row(T, blockIdx.y, t);
-    const int h = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const int qend = s.pos0 + 1 + t, end = bidirectional ? s.pos0 + s.rows : qend;
-    const int start = window > 0 && qend > window ? qend - window : 0;
-    const int kvh = h / (heads / M.kv_heads);
-    const size_t qrow = (static_cast<size_t>(s.row0 + t) * heads + h) * hd;
-    for (int d = threadIdx.x; d < hd; d += 64 * kWaves) sq[d] = q[qrow + d] * (1.0f / sqrtf(static_cast<float>(hd)));
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, acc[kMaxHd / 64] = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = start + 64 * wv; p0 < end; p0 += 64 * kWaves) {
-        const int p = p0 + lane;
-        float sc = -INFINITY;
-        if (p < end) {
-            const Place at = place<PAGED>(M, s.slot, kvh, p / kSlab);
-            sc = 0.0f;
-            for (int d = 0; d < hd; ++d) sc = fmaf(sq[d], k_value(kc, M, at, p % kSlab, hd, d), sc);
+typedef _Float16 fh2 __attribute__((ext_vector_type(2)));
+
+// A header pair's scales and 1024 + zero points. A code c in the low bits of the f16 1024 is 1024 + c, so (1024 + c) - (1024 + z)
+// and its product with the scale are exact.
+struct Heads2 {
+    fh2 d, z;
+};
+__device__ __forceinline__ Heads2 heads2(uint32_t h) {
+    return Heads2{__builtin_bit_cast(fh2, h & 0xFFF0FFF0u), __builtin_bit_cast(fh2, (h & 0x000F000Fu) | 0x64006400u)};
+}
+// The eight values of a word: elements 2 i, 2 i + 1 with h[i].
+__device__ __forceinline__ fh8 decode8(uint32_t w, const Heads2 (&h)[4]) {
+    fh8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const fh2 c = __builtin_bit_cast(fh2, ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u);
+        const fh2 v = (c - h[i].z) * h[i].d;
+        r[2 * i] = v[0];
+        r[2 * i + 1] = v[1];
+    }
+    return r;
+}
+// All of them with the low (or high) header of a pair.
+template <bool HIGH>
+__device__ __forceinline__ fh8 decode8_one(uint32_t w, const Heads2 &h) {
+    const Heads2 one{fh2{h.d[HIGH], h.d[HIGH]}, fh2{h.z[HIGH], h.z[HIGH]}};
+    const Heads2 all[4] = {one, one, one, one};
+    return decode8(w, all);
+}
+
+// N words (16 B aligned where N allows it) as N registers.
+template <int N>
+__device__ __forceinline__ void ld_words(const uint8_t *p, uint32_t (&w)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
         }
-        float mn = sc;
-        for (int o = 32; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o, 64));
-        mn = fmaxf(m, mn);
-        const float ms = mn == -INFINITY ? 0.0f : mn;
-        const float pr = p < end ? expf(sc - ms) : 0.0f, rs = expf(m - ms);
-        float ps = pr;
-        for (int o = 32; o > 0; o >>= 1) ps += __shfl_xor(ps, o, 64);
-        l = l * rs + ps;
-        m = mn;
-        sp[wv][lane] = pr;
-        __builtin_amdgcn_wave_barrier();
-        for (int r = 0; r < kMaxHd / 64; ++r) {
-            const int d = lane + 64 * r;
-            if (d >= hd) break;
-            acc[r] *= rs;
-            for (int j = 0; j < min(end - p0, 64); ++j)
-                acc[r] = fmaf(sp[wv][j], v_value(vc, M, place<PAGED>(M, s.slot, kvh, (p0 + j) / kSlab), (p0 + j) % kSlab, hd, d), acc[r]);
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const uint2 v = reinterpret_cast<const uint2 *>(p)[i];
+            w[2 * i] = v.x, w[2 * i + 1] = v.y;
         }
-        __builtin_amdgcn_wave_barrier();
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t *>(p)[i];
     }
-    if (lane == 0) sm[wv] = m, sl[wv] = l;
-    for (int r = 0; r < kMaxHd / 64; ++r)
-        if (lane + 64 * r < hd) sacc[wv][lane + 64 * r] = acc[r];
+}
+// U headers (two bytes each) as pairs.
+template <int U>
+__device__ __forceinline__ void ld_heads(const uint8_t *p, uint32_t (&h)[(U + 1) / 2]) {
+    if constexpr (U % 2 == 0) {
+        ld_words<U / 2>(p, h);
+    } else {
+#pragma unroll
+        for (int i = 0; i < (U + 1) / 2; ++i)
+            h[i] = reinterpret_cast<const uint16_t *>(p)[2 * i] |
+                   (2 * i + 1 < U ? static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(p)[2 * i + 1]) << 16 : 0u);
+    }
+}
+
+// Where the words and the headers of a slab begin: the same for K and V, whose slabs have the same sizes.
+struct SlabAt {
+    size_t words, heads;
+    bool bad;
+};
+template <int U, bool PAGED>
+__device__ __forceinline__ SlabAt slab_at(const Map4 &M, int slot, int kvh, int slab) {
+    const Place p = place<PAGED>(M, slot, kvh, slab);
+    return SlabAt{p.at + static_cast<size_t>(p.slab) * (128 * U), p.at + static_cast<size_t>(M.spp) * (128 * U) + static_cast<size_t>(p.slab) * (16 * U),
+                  p.bad};
+}
+
+// Operand layout of v_mfma_f32_16x16x32_f16: lane l = (c = l & 15, g = l >> 4) gives row c of A and column c of B at the same eight
+// k slots (g, j); the result has rows 4 g + r, column c. Over a block of 32 keys:
+//  - S^T of key half h: A row c is key 8 (c >> 2) + 4 h + (c & 3), dims 32 u + 8 g + j (one K word); lane (c, g) ends with the
+//    scores of keys 8 g + 4 h + r of query vector c.
+//  - O^T += V^T P^T: k slot (g, j) is key 8 g + j, so B is the lane's own eight weights in order and A, dims 16 b + c of V^T at
+//    positions 8 g .. 8 g + 7, is one V word of slab g.
+
+// The lane's query vector as B operands; returns the factor that brings a score to base-2 units (fa16_q_split).
+template <int U>
+__device__ __forceinline__ float load_query(const float *qrow, fh8 (&qh)[U], fh8 (&ql)[U]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    float4 qr[2 * U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        __builtin_memcpy(&qr[2 * u], qrow + 32 * u + 8 * g, 16);
+        __builtin_memcpy(&qr[2 * u + 1], qrow + 32 * u + 8 * g + 4, 16);
+    }
+    return fa16_q_split<32 * U>(qr, 1.0f / sqrtf(32.0f * U), qh, ql);
+}
+
+// Softmax step over a block's scores s[h][r] (key kb + 8 g + 4 h + r; keys outside [qs, qe) are masked): new running maximum and
+// sum, O rescaled where the maximum moved, the weights as an f16 pair. The sum is of the weights before they are split.
+template <int U>
+__device__ __forceinline__ void softmax_step(const fa4 (&s)[2], int kb, int qs, int qe, float &m, float &l, fa4 (&o)[2 * U], fh8 &ph,
+                                             fh8 &pl) {
+    const int g = (threadIdx.x & 63) >> 4;
+    float v[8], bm = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = s[j >> 2][j & 3];
+    if (__any(kb < qs || kb + 32 > qe)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int p = kb + 8 * g + j;
+            v[j] = p >= qs && p < qe ? v[j] : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bm = fmaxf(bm, v[j]);
+    bm = xor32_max(xor16_max(bm));
+    const float mn = fmaxf(m, bm), ms = mn == -INFINITY ? 0.0f : mn;  // ms: exp2(-inf - ms) is 0 also before any key
+    const float alpha = __builtin_amdgcn_exp2f(m - ms);
+    float ps = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float p = __builtin_amdgcn_exp2f(v[j] - ms);
+        ps += p;
+        _Float16 hh, ll;
+        split_h(p, hh, ll);
+        ph[j] = hh;
+        pl[j] = ll;
+    }
+    ps = xor32_add(xor16_add(ps));
+    l = l * alpha + ps;
+    m = mn;
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int b = 0; b < 2 * U; ++b) o[b] *= alpha;
+    }
+}
+
+// How a pass's contexts are cut: chunks of `len` keys (a multiple of 128) from each segment's first key rounded down to 32, all
+// segments' chunks in one list; segment i's begin at first[i], its partial results at base[i].
+struct Cuts {
+    int len, total;
+    int first[VQ_MAX_SEGMENTS + 1];
+    int base[VQ_MAX_SEGMENTS];
+};
+// First key that any row of a segment sees, rounded down to a block.
+__host__ __device__ __forceinline__ int first_key(const Seg &s, int window) {
+    return window > 0 && s.pos0 + 1 > window ? (s.pos0 + 1 - window) & ~31 : 0;
+}
+
+// The keys that query row t of a segment sees.
+struct Sees {
+    int from, to;
+};
+__device__ __forceinline__ Sees sees(const Seg &s, int t, int bidirectional, int window) {
+    const int end = s.pos0 + 1 + t;
+    return Sees{window > 0 && end > window ? end - window : 0, bidirectional ? s.pos0 + s.rows : end};
+}
+
+// A workgroup's results for up to 16 query vectors: W waves' sums (each wave's [16][HD] in `sums`, maxima and totals in sm, sl) meet
+// in wave order; written out, or as the chunk's unnormalised part where the context is cut.
+template <int HD, int W>
+__device__ __forceinline__ void meet(const float *sums, const float (&sm)[W][16], const float (&sl)[W][16], int threads, int tid, int j0,
+                                     int nvec, int G, int kvh, int heads, int row0, float *out, float *part, float *pml, int n, int ci) {
+    for (int e = tid; e < 16 * (HD / 4); e += threads) {
+        const int c = e / (HD / 4), d4 = 4 * (e - c * (HD / 4)), j = j0 + c;
+        if (j >= nvec) continue;
+        const int t = j / G, h = kvh * G + j - t * G;
+        float mx = sm[0][c];
+#pragma unroll
+        for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm[w][c]);
+        float L = 0.0f;
+        float4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float f = sm[w][c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][c] - mx);
+            L = fmaf(sl[w][c], f, L);
+            const float4 p = *reinterpret_cast<const float4 *>(sums + (w * 16 + c) * HD + d4);
+            acc.x = fmaf(p.x, f, acc.x);
+            acc.y = fmaf(p.y, f, acc.y);
+            acc.z = fmaf(p.z, f, acc.z);
+            acc.w = fmaf(p.w, f, acc.w);
+        }
+        if (n == 1) {
+            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+            const float4 r{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+            __builtin_memcpy(out + (static_cast<size_t>(row0 + t) * heads + h) * HD + d4, &r, 16);
+        } else {
+            const size_t at = (static_cast<size_t>(t) * heads + h) * n + ci;
+            *reinterpret_cast<float4 *>(part + at * HD + d4) = acc;
+            if (d4 == 0) pml[2 * at] = mx, pml[2 * at + 1] = L;
+        }
+    }
+}
+
+// A block's codes and headers in registers. Lane (c, g) has K rows 8 (c >> 2) + 4 h + (c & 3) at its dims, the V words of its dims in
+// slab g, and of slab g the headers of group c.
+template <int U>
+struct Raw4 {
+    uint32_t k[2][U], kh[2][(U + 1) / 2], v[2 * U];
+    uint4 vh;
+};
+template <int U, bool PAGED>
+__device__ __forceinline__ void issue_block(const uint8_t *__restrict__ kc, const uint8_t *__restrict__ vc, const Map4 &M, int slot,
+                                            int kvh, int kb, int last, Raw4<U> &r) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    // Slabs past the last key's read that one's (their keys are masked).
+    const SlabAt ks = slab_at<U, PAGED>(M, slot, kvh, min(kb / kSlab + (c >> 2), last));
+    const SlabAt vs = slab_at<U, PAGED>(M, slot, kvh, min(kb / kSlab + g, last));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = 4 * h + (c & 3);
+        ld_words<U>(kc + ks.words + row * (16 * U) + g * (4 * U), r.k[h]);
+        ld_heads<U>(kc + ks.heads + row * (2 * U), r.kh[h]);
+    }
+    constexpr int W = U % 2 == 0 ? 4 : 2;
+#pragma unroll
+    for (int i = 0; i < 2 * U / W; ++i) {
+        uint32_t w[W];
+        ld_words<W>(vc + vs.words + (16 * i + c) * (4 * W), w);
+#pragma unroll
+        for (int k = 0; k < W; ++k) r.v[W * i + k] = w[k];
+    }
+    r.vh = *reinterpret_cast<const uint4 *>(vc + vs.heads + 16 * min(c, U - 1));
+    if (ks.bad) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < (U + 1) / 2; ++i) r.kh[h][i] = kNanHeader | kNanHeader << 16;
+    }
+}
+
+// Lane n's value of each row of 16 lanes, to all of the row.
+template <int N>
+__device__ __forceinline__ uint32_t row_bcast(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x150 + N, 0xF, 0xF, true));
+}
+
+template <int U, int I>
+__device__ __forceinline__ void pv_groups(const Raw4<U> &r, const uint32_t (&d)[4], const uint32_t (&z)[4], const fh8 &ph, const fh8 &pl,
+                                          fa4 (&o)[2 * U]) {
+    if constexpr (I < U) {
+        Heads2 h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            h[i] = Heads2{__builtin_bit_cast(fh2, row_bcast<I>(d[i])), __builtin_bit_cast(fh2, row_bcast<I>(z[i]))};
+#pragma unroll
+        for (int b = 2 * I; b < 2 * I + 2; ++b) {
+            const fh8 a = decode8(r.v[b], h);
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[b], 0, 0, 0);
+        }
+        pv_groups<U, I + 1>(r, d, z, ph, pl, o);
+    }
+}
+
+template <int U>
+__device__ __forceinline__ void consume_block(const Raw4<U> &r, int kb, int qs, int qe, const fh8 (&qh)[U], const fh8 (&ql)[U], float sinv,
+                                              float &m, float &l, fa4 (&o)[2 * U]) {
+    fa4 s[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        fa4 a0{0.f, 0.f, 0.f, 0.f}, a1{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const Heads2 hd2 = heads2(r.kh[h][u / 2]);
+            const fh8 a = u % 2 == 0 ? decode8_one<false>(r.k[h][u], hd2) : decode8_one<true>(r.k[h][u], hd2);
+            a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[u], a0, 0, 0, 0);
+            a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[u], a1, 0, 0, 0);
+        }
+        s[h] = (a0 + a1) * sinv;
+    }
+    fh8 ph, pl;
+    softmax_step<U>(s, kb, qs, qe, m, l, o, ph, pl);
+    uint32_t d[4], z[4];
+    const uint32_t raw[4] = {r.vh.x, r.vh.y, r.vh.z, r.vh.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = raw[i] & 0xFFF0FFF0u, z[i] = (raw[i] & 0x000F000Fu) | 0x64006400u;
+    pv_groups<U, 0>(r, d, z, ph, pl, o);
+}
+
+// Decode and verify passes: one workgroup per (chunk, kv head, 16 query vectors); vector j of a segment is (row j / G, head j % G of
+// the kv head's group). Its four waves take the chunk's 32-key blocks in turn, straight from the cache into registers, decoded
+// there into MFMA operands, with an online softmax each; they meet in wave order.
+template <int U, bool PAGED>
+__global__ __launch_bounds__(256, 2) void attention4_split_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
+                                                                  const uint8_t *__restrict__ vc, float *__restrict__ part,
+                                                                  float *__restrict__ pml, float *__restrict__ out, SegTable T, Map4 M,
+                                                                  Cuts C, int heads, int bidirectional, int window) {
+    constexpr int HD = 32 * U;
+    __shared__ __align__(16) float sums[4 * 16 * HD];
+    __shared__ float sm[4][16], sl[4][16];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % M.kv_heads, list = blockIdx.x / M.kv_heads;
+    int si = 0;
+    while (list >= C.first[si + 1]) ++si;
+    const Seg &s = T.s[si];
+    const int ci = list - C.first[si], n = C.first[si + 1] - C.first[si];
+    const int G = heads / M.kv_heads, nvec = s.rows * G, j0 = blockIdx.y * 16;
+    if (j0 >= nvec) return;
+    const int j = min(j0 + c, nvec - 1), t = j / G, h = kvh * G + j - t * G;  // vectors past the last repeat it; not written
+    const Sees see = sees(s, t, bidirectional, window);
+    const int k_lo = first_key(s, window) + ci * C.len, k_hi = min(k_lo + C.len, s.pos0 + s.rows);
+    const int qe = min(see.to, k_hi), last = (k_hi - 1) / kSlab;
+    float m = -INFINITY, l = 0.0f;
+    fa4 o[2 * U];
+#pragma unroll
+    for (int b = 0; b < 2 * U; ++b) o[b] = fa4{0.f, 0.f, 0.f, 0.f};
+    int kb = k_lo + 32 * wv;
+    Raw4<U> r;
+    if (kb < k_hi) issue_block<U, PAGED>(kc, vc, M, s.slot, kvh, kb, last, r);
+    fh8 qh[U], ql[U];
+    const float sinv = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
+    for (; kb < k_hi; kb += 128) {
+        const Raw4<U> now = r;
+        if (kb + 128 < k_hi) issue_block<U, PAGED>(kc, vc, M, s.slot, kvh, kb + 128, last, r);
+        consume_block<U>(now, kb, see.from, qe, qh, ql, sinv, m, l, o);
+    }
+    float *ow = sums + wv * 16 * HD;
+#pragma unroll
+    for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(ow + c * HD + 16 * b + 4 * g) = o[b];
+    if (g == 0) sm[wv][c] = m, sl[wv][c] = l;
     __syncthreads();
-    if (wv != 0) return;
-    float mx = -INFINITY, L = 0.0f, f[kWaves];
-    for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm[w]);
-    for (int w = 0; w < kWaves; ++w) {
-        f[w] = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - mx);
-        L += sl[w] * f[w];
+    const size_t base = C.base[si];
+    meet<HD, 4>(sums, sm, sl, 256, threadIdx.x, j0, nvec, G, kvh, heads, s.row0, out, part + base * HD, pml + 2 * base, n, ci);
+}
+
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, for segments of more than one: one workgroup of four waves
+// per (row, head), wave w adds chunks w, w + 4, ..., the waves' sums in wave order.
+template <int HD>
+__global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
+                                                               float *__restrict__ out, SegTable T, Cuts C, int heads) {
+    constexpr int Q = HD / 4;
+    __shared__ float smx[4], sl[4];
+    __shared__ float4 sacc[4][Q];
+    int t = blockIdx.x / heads, si = 0;
+    const int h = blockIdx.x - t * heads;
+    while (si + 1 < T.n && t >= T.s[si].rows) t -= T.s[si++].rows;
+    const Seg &s = T.s[si];
+    const int n = C.first[si + 1] - C.first[si];
+    if (n == 1) return;
+    const size_t at = static_cast<size_t>(C.base[si]) + (static_cast<size_t>(t) * heads + h) * n;
+    const float *ml = pml + 2 * at;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    float mx = -INFINITY;
+    for (int c = tid; c < n; c += 256) mx = fmaxf(mx, ml[2 * c]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+    if (lane == 0) smx[wv] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(smx[0], smx[1]), fmaxf(smx[2], smx[3]));
+    float4 acc{0.f, 0.f, 0.f, 0.f};
+    float L = 0.0f;
+    if (lane < Q) {
+        for (int c0 = wv; c0 < n; c0 += 16) {
+            float4 p[4];
+            float mc[4], lc[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = c0 + 4 * k < n ? c0 + 4 * k : c0;
+                p[k] = *reinterpret_cast<const float4 *>(part + (at + c) * HD + 4 * lane);
+                mc[k] = ml[2 * c];
+                lc[k] = ml[2 * c + 1];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (c0 + 4 * k >= n) break;
+                const float f = mc[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc[k] - mx);
+                L = fmaf(lc[k], f, L);
+                acc.x = fmaf(p[k].x, f, acc.x);
+                acc.y = fmaf(p[k].y, f, acc.y);
+                acc.z = fmaf(p[k].z, f, acc.z);
+                acc.w = fmaf(p[k].w, f, acc.w);
+            }
+        }
+        sacc[wv][lane] = acc;
     }
-    for (int d = lane; d < hd; d += 64) {
-        float a = 0.0f;
-        for (int w = 0; w < kWaves; ++w) a += sacc[w][d] * f[w];
-        out[qrow + d] = a / L;
+    if (lane == 0) sl[wv] = L;
+    __syncthreads();
+    if (wv != 0 || lane >= Q) return;
+    const float lt = ((sl[0] + sl[1]) + sl[2]) + sl[3], inv = lt > 0.0f ? 1.0f / lt : 0.0f;
+    const float4 a = sacc[0][lane], b = sacc[1][lane], c = sacc[2][lane], d = sacc[3][lane];
+    const float4 r{(((a.x + b.x) + c.x) + d.x) * inv, (((a.y + b.y) + c.y) + d.y) * inv, (((a.z + b.z) + c.z) + d.z) * inv,
+                   (((a.w + b.w) + c.w) + d.w) * inv};
+    __builtin_memcpy(out + (static_cast<size_t>(s.row0 + t) * heads + h) * HD + 4 * lane, &r, 16);
+}
+
+// Prompt passes, and any pass without a workspace: a workgroup of NW waves takes NW / 2 tiles of 16 query vectors of a kv head, two
+// waves each, one for the 32-key blocks of each parity (blocks at multiples of 32 keys whatever the rows, so a row's sums do not
+// depend on the others); their sums meet at the end. Per step of 64 keys the threads load the next step's words, the waves consume
+// the present one from LDS, decoded once for all tiles: K rows of HD + 16 f16, V^T [dim][32 positions] with 16-byte pieces swizzled
+// by (dim >> 2) & 3; the loaded words are decoded into the other LDS buffer: one barrier per step.
+__device__ __forceinline__ int vt_at(int d, int octet) { return d * 32 + ((octet ^ ((d >> 2) & 3)) << 3); }
+
+template <int U, bool PAGED, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attention4_tiled_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
+                                                                      const uint8_t *__restrict__ vc, float *__restrict__ out,
+                                                                      SegTable T, Map4 M, int heads, int bidirectional, int window) {
+    constexpr int HD = 32 * U, LDK = HD + 16, TH = 64 * NW, TILES = NW / 2;
+    constexpr int KW = U % 4 == 0 ? 4 : U % 2 == 0 ? 2 : 1, W = U % 2 == 0 ? 4 : 2;  // words of a K unit, of a V unit
+    constexpr int KUN = 64 * 4 * (U / KW), VUN = 8 * 16 * (2 * U / W);               // units of a step
+    constexpr int KN = (KUN + TH - 1) / TH, VN = (VUN + TH - 1) / TH;                // of a thread
+    constexpr int KB = 32 * LDK, VB = HD * 32;                                       // f16 elements of a block
+    constexpr int BUF = 2 * (KB + VB), MEET = TILES * 2 * 16 * HD * 2;               // f16 elements: a buffer, the sums at the end
+    __shared__ __align__(16) _Float16 kv[2 * BUF > MEET ? 2 * BUF : MEET];
+    __shared__ SlabAt slabs[2][8];
+    __shared__ float sm[TILES][2][16], sl[TILES][2][16];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, c = lane & 15, g = lane >> 4, tile = wv >> 1, par = wv & 1;
+    const int kvh = blockIdx.x % M.kv_heads, G = heads / M.kv_heads;
+    // Workgroups take the kv heads in turn, the last rows, which see the most keys, first.
+    int tb = gridDim.x / M.kv_heads - 1 - blockIdx.x / M.kv_heads, si = 0;
+    while (si + 1 < T.n) {
+        const int nt = (T.s[si].rows * G + 16 * TILES - 1) / (16 * TILES);
+        if (tb < nt) break;
+        tb -= nt;
+        ++si;
     }
+    const Seg &s = T.s[si];
+    const int nvec = s.rows * G, first = tb * 16 * TILES, j0 = first + 16 * tile;
+    const bool on = j0 < nvec;
+    const int j = min(j0 + c, nvec - 1), t = j / G, h = kvh * G + j - t * G;
+    const Sees see = sees(s, t, bidirectional, window), a = sees(s, first / G, bidirectional, window),
+               z = sees(s, min(first + 16 * TILES - 1, nvec - 1) / G, bidirectional, window);
+    const int k0 = a.from & ~63, k_hi = z.to, steps = (k_hi - k0 + 63) / 64, s0 = a.from / kSlab, s1 = (k_hi - 1) / kSlab;
+    auto look = [&](int step) { return slab_at<U, PAGED>(M, s.slot, kvh, min(max((k0 + 64 * step) / kSlab + (tid & 7), s0), s1)); };
+    if (tid < 16) slabs[tid >> 3][tid & 7] = look(tid >> 3);
+    fh8 qh[U], ql[U];
+    const float sinv = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
+    __syncthreads();
+    uint32_t rk[KN][KW], rkh[KN][KW == 4 ? 2 : 1], rv[VN][W];
+    uint4 rvh[VN][W / 2];
+    auto issue = [&](int step) {
+        const SlabAt *sa = slabs[step & 1];
+#pragma unroll
+        for (int i = 0; i < KN; ++i) {  // unit: (key, word group of dims, run of KW words)
+            const int unit = (tid + TH * i) % KUN, key = unit / (4 * (U / KW)), rest = unit % (4 * (U / KW)), g4 = rest / (U / KW), u0 = rest % (U / KW) * KW;
+            const SlabAt &at = sa[key >> 3];
+            ld_words<KW>(kc + at.words + (key & 7) * (16 * U) + g4 * (4 * U) + 4 * u0, rk[i]);
+            const uint8_t *hp = kc + at.heads + (key & 7) * (2 * U) + 2 * u0;
+            if constexpr (KW == 4) ld_words<2>(hp, rkh[i]);
+            else if constexpr (KW == 2) ld_words<1>(hp, rkh[i]);
+            else rkh[i][0] = *reinterpret_cast<const uint16_t *>(hp);
+            if (at.bad)
+#pragma unroll
+                for (auto &x : rkh[i]) x = kNanHeader | kNanHeader << 16;
+        }
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {  // unit: (slab, run of W dim tiles, dim of a tile)
+            const int unit = (tid + TH * i) % VUN, slab = unit / (16 * (2 * U / W)), rest = unit % (16 * (2 * U / W));
+            const SlabAt &at = sa[slab];
+            ld_words<W>(vc + at.words + rest * (4 * W), rv[i]);
+#pragma unroll
+            for (int k = 0; k < W / 2; ++k) rvh[i][k] = *reinterpret_cast<const uint4 *>(vc + at.heads + 16 * ((rest >> 4) * (W / 2) + k));
+        }
+    };
+    auto stage = [&](int step) {
+        _Float16 *buf = kv + (step & 1) * BUF;
+#pragma unroll
+        for (int i = 0; i < KN; ++i) {
+            const int unit = tid + TH * i, key = unit / (4 * (U / KW)), rest = unit % (4 * (U / KW)), g4 = rest / (U / KW), u0 = rest % (U / KW) * KW;
+            if (KUN % TH && unit >= KUN) break;
+            const int row = 16 * ((key >> 2) & 1) + 4 * ((key >> 3) & 3) + (key & 3);  // of the block's S^T operand
+            _Float16 *kd = buf + (key >> 5) * (KB + VB) + row * LDK + 32 * u0 + 8 * g4;
+#pragma unroll
+            for (int k = 0; k < KW; ++k) {
+                const Heads2 hd2 = heads2(rkh[i][k / 2]);
+                *reinterpret_cast<fh8 *>(kd + 32 * k) = k % 2 == 0 ? decode8_one<false>(rk[i][k], hd2) : decode8_one<true>(rk[i][k], hd2);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+            const int unit = tid + TH * i, slab = unit / (16 * (2 * U / W)), rest = unit % (16 * (2 * U / W));
+            if (VUN % TH && unit >= VUN) break;
+            _Float16 *vd = buf + (slab >> 2) * (KB + VB) + KB;
+#pragma unroll
+            for (int k = 0; k < W; ++k) {
+                const uint4 x = rvh[i][k / 2];
+                const Heads2 hs[4] = {heads2(x.x), heads2(x.y), heads2(x.z), heads2(x.w)};
+                *reinterpret_cast<fh8 *>(vd + vt_at(16 * ((rest >> 4) * W + k) + (rest & 15), slab & 3)) = decode8(rv[i][k], hs);
+            }
+        }
+    };
+    issue(0);
+    float m = -INFINITY, l = 0.0f;
+    fa4 o[2 * U];
+#pragma unroll
+    for (int b = 0; b < 2 * U; ++b) o[b] = fa4{0.f, 0.f, 0.f, 0.f};
+    stage(0);
+    __syncthreads();
+    for (int step = 0; step < steps; ++step) {
+        const bool more = step + 1 < steps;
+        SlabAt next{};
+        if (tid < 8) next = look(step + 2);
+        if (more) issue(step + 1);
+        const int kb = k0 + 64 * step + 32 * par;
+        if (on && kb < k_hi) {
+            const _Float16 *ks = kv + (step & 1) * BUF + par * (KB + VB), *vt = ks + KB;
+            fa4 sc[2];
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                fa4 a0{0.f, 0.f, 0.f, 0.f}, a1{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const fh8 k8 = *reinterpret_cast<const fh8 *>(ks + (16 * hh + c) * LDK + 8 * g + 32 * u);
+                    a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[u], a0, 0, 0, 0);
+                    a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[u], a1, 0, 0, 0);
+                }
+                sc[hh] = (a0 + a1) * sinv;
+            }
+            fh8 ph, pl;
+            softmax_step<U>(sc, kb, see.from, see.to, m, l, o, ph, pl);
+#pragma unroll
+            for (int b = 0; b < 2 * U; ++b) {
+                const fh8 v8 = *reinterpret_cast<const fh8 *>(vt + vt_at(16 * b + c, g));
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[b], 0, 0, 0);
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[b], 0, 0, 0);
+            }
+        }
+        if (more) stage(step + 1);
+        if (tid < 8) slabs[step & 1][tid] = next;
+        __syncthreads();
+    }
+    float *sums = reinterpret_cast<float *>(kv);
+#pragma unroll
+    for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(sums + (wv * 16 + c) * HD + 16 * b + 4 * g) = o[b];
+    if (g == 0) sm[tile][par][c] = m, sl[tile][par][c] = l;
+    __syncthreads();
+    for (int i = 0; i < TILES; ++i)
+        meet<HD, 2>(sums + i * 32 * HD, sm[i], sl[i], TH, tid, first + 16 * i, nvec, G, kvh, heads, s.row0, out, nullptr, nullptr, 1, 0);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------
@@ -332,14 +796,103 @@ int launch_read4(const void *kc, const void *vc, float *k, float *v, const SegTa
     return status_of(hipGetLastError());
 }
 
+// Chunks for about a round or a few of the 512 workgroups that run at once (two per CU). `rounds` full rounds need chunks of at
+// least some length; among 1 to 4 rounds the least of rounds x (length + what a chunk costs besides its keys, in keys).
+Cuts make_cuts(const SegTable &T, int heads, int kv_heads, int window) {
+    constexpr int kSlots = 512, kFixed = 160;
+    int groups = 1;
+    long long keys = 0;
+    for (int i = 0; i < T.n; ++i) {
+        groups = max(groups, (T.s[i].rows * (heads / kv_heads) + 15) / 16);
+        keys += T.s[i].pos0 + T.s[i].rows - first_key(T.s[i], window);
+    }
+    auto count = [&](long long len) {
+        long long n = 0;
+        for (int i = 0; i < T.n; ++i) n += (T.s[i].pos0 + T.s[i].rows - first_key(T.s[i], window) + len - 1) / len;
+        return n * kv_heads * groups;
+    };
+    long long best = 0, cost = 0;
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+        long long len = (keys * kv_heads * groups / (kSlots * rounds) + 127) / 128 * 128;
+        len = len < 128 ? 128 : len;
+        for (int i = 0; i < 64 && count(len) > static_cast<long long>(kSlots) * rounds; ++i) len += 128;
+        const long long c = rounds * (len + kFixed);
+        if (best == 0 || c < cost) best = len, cost = c;
+    }
+    Cuts C;
+    C.len = static_cast<int>(best);
+    C.total = 0;
+    int base = 0;
+    for (int i = 0; i < T.n; ++i) {
+        const int n = (T.s[i].pos0 + T.s[i].rows - first_key(T.s[i], window) + C.len - 1) / C.len;
+        C.first[i] = C.total;
+        C.base[i] = base;
+        C.total += n;
+        if (n > 1) base += n * T.s[i].rows * heads;
+    }
+    for (int i = T.n; i <= VQ_MAX_SEGMENTS; ++i) C.first[i] = C.total;
+    return C;
+}
+// Partial results of the pass: vectors x chunks where a segment has more than one.
+size_t parts_of(const SegTable &T, const Cuts &C, int heads) {
+    size_t n = 0;
+    for (int i = 0; i < T.n; ++i) {
+        const size_t k = C.first[i + 1] - C.first[i];
+        if (k > 1) n += k * T.s[i].rows * heads;
+    }
+    return n;
+}
+size_t attention4_ws_bytes(const SegTable &T, int heads, int kv_heads, int hd, int window) {
+    if (max_seg_rows(T) > VQ_ATTN_ROW_MAX) return 0;
+    const size_t n = parts_of(T, make_cuts(T, heads, kv_heads, window), heads);
+    return n * (hd + 2) * 4 + 16;
+}
+
+template <typename F>
+void for_hd(int hd, F &&f) {
+    switch (hd / 32) {
+        case 1: f(std::integral_constant<int, 1>{}); break;
+        case 2: f(std::integral_constant<int, 2>{}); break;
+        case 3: f(std::integral_constant<int, 3>{}); break;
+        case 4: f(std::integral_constant<int, 4>{}); break;
+        case 5: f(std::integral_constant<int, 5>{}); break;
+        case 6: f(std::integral_constant<int, 6>{}); break;
+        case 7: f(std::integral_constant<int, 7>{}); break;
+        default: f(std::integral_constant<int, 8>{}); break;
+    }
+}
+
 int launch_attention4(const float *q, const void *kc, const void *vc, float *out, const SegTable &T, const Map4 &M, int heads, int hd,
-                      int bidirectional, int window, hipStream_t s) {
+                      int bidirectional, int window, void *ws, size_t ws_bytes, hipStream_t s) {
     if (!q || !out) return VQ_ERR_ARG;
     if (heads < M.kv_heads || heads % M.kv_heads || window < 0) return VQ_ERR_SHAPE;
-    const dim3 grid(heads, T.total);
+    const int G = heads / M.kv_heads;
     auto *kb = static_cast<const uint8_t *>(kc), *vb = static_cast<const uint8_t *>(vc);
-    if (M.pt) attention4_kernel<true><<<grid, 64 * kWaves, 0, s>>>(q, kb, vb, out, T, M, heads, hd, bidirectional, window);
-    else attention4_kernel<false><<<grid, 64 * kWaves, 0, s>>>(q, kb, vb, out, T, M, heads, hd, bidirectional, window);
+    if (ws != nullptr && max_seg_rows(T) <= VQ_ATTN_ROW_MAX) {
+        if ((reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < attention4_ws_bytes(T, heads, M.kv_heads, hd, window))
+            return VQ_ERR_WORKSPACE;
+        const Cuts C = make_cuts(T, heads, M.kv_heads, window);
+        const size_t parts = parts_of(T, C, heads);
+        float *part = static_cast<float *>(ws), *pml = part + parts * hd;
+        const dim3 grid(C.total * M.kv_heads, (max_seg_rows(T) * G + 15) / 16);
+        for_hd(hd, [&](auto u) {
+            constexpr int U = decltype(u)::value;
+            if (M.pt) attention4_split_kernel<U, true><<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window);
+            else attention4_split_kernel<U, false><<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window);
+            if (parts) attention4_merge_kernel<32 * U><<<T.total * heads, 256, 0, s>>>(part, pml, out, T, C, heads);
+        });
+        return status_of(hipGetLastError());
+    }
+    constexpr int NW = 8, PER = 16 * (NW / 2);
+    long long tiles = 0;
+    for (int i = 0; i < T.n; ++i) tiles += (static_cast<long long>(T.s[i].rows) * G + PER - 1) / PER;
+    if (tiles * M.kv_heads > INT32_MAX) return VQ_ERR_SHAPE;
+    const dim3 grid(static_cast<unsigned>(tiles * M.kv_heads));
+    for_hd(hd, [&](auto u) {
+        constexpr int U = decltype(u)::value;
+        if (M.pt) attention4_tiled_kernel<U, true, NW><<<grid, 64 * NW, 0, s>>>(q, kb, vb, out, T, M, heads, bidirectional, window);
+        else attention4_tiled_kernel<U, false, NW><<<grid, 64 * NW, 0, s>>>(q, kb, vb, out, T, M, heads, bidirectional, window);
+    });
     return status_of(hipGetLastError());
 }
 
@@ -390,35 +943,41 @@ int vq_kv4_read_seg(const void *kc, const void *vc, float *k, float *v, const in
 }
 
 size_t vq_attention4_workspace_bytes(int heads, int kv_heads, int hd, int seq_len, int ntok, int window) {
-    (void)heads, (void)kv_heads, (void)hd, (void)seq_len, (void)ntok, (void)window;
-    return 0;
+    if (kv_heads < 1 || heads < kv_heads || heads % kv_heads || !hd_ok(hd) || ntok < 1 || seq_len < 1 || window < 0 ||
+        seq_len > INT32_MAX - kSlab - ntok)
+        return 0;
+    return attention4_ws_bytes(one_segment(seq_len - 1, ntok), heads, kv_heads, hd, window);
 }
 
 size_t vq_attention4_seg_workspace_bytes(const int32_t *segs, int nseg, int heads, int kv_heads, int hd) {
-    (void)segs, (void)nseg, (void)heads, (void)kv_heads, (void)hd;
-    return 0;
+    SegTable T;
+    if (make_table(segs, nseg, T, nullptr) != VQ_OK) return 0;
+    if (kv_heads < 1 || heads < kv_heads || heads % kv_heads || !hd_ok(hd)) return 0;
+    for (int i = 0; i < T.n; ++i)
+        if (T.s[i].pos0 > INT32_MAX - kSlab - T.s[i].rows) return 0;
+    return attention4_ws_bytes(T, heads, kv_heads, hd, 0);
 }
 
 int vq_attention4_ws(const float *q, const void *kc, const void *vc, float *out, int heads, int kv_heads, int hd, int max_seq,
                      int seq_len, int ntok, int bidirectional, int window, void *workspace, size_t workspace_bytes,
                      void *stream) {
-    (void)workspace, (void)workspace_bytes;
     if (ntok < 1 || seq_len < 1 || ntok > max_seq || seq_len > max_seq - ntok + 1) return VQ_ERR_SHAPE;
     const SegTable T = one_segment(seq_len - 1, ntok);
     Map4 M;
     const int st = check_cache(kc, vc, kv_heads, hd, T, false, nullptr, 0, 0, 0, max_seq, M);
-    return st != VQ_OK ? st : launch_attention4(q, kc, vc, out, T, M, heads, hd, bidirectional, window, static_cast<hipStream_t>(stream));
+    return st != VQ_OK ? st : launch_attention4(q, kc, vc, out, T, M, heads, hd, bidirectional, window, workspace, workspace_bytes,
+                                                static_cast<hipStream_t>(stream));
 }
 
 int vq_attention4_seg_ws(const float *q, const void *kc, const void *vc, float *out, const int32_t *segs, int nseg, int heads,
                          int kv_heads, int hd, const int32_t *page_table, int page_size, int pages_per_seq, int pages,
                          void *workspace, size_t workspace_bytes, void *stream) {
-    (void)workspace, (void)workspace_bytes;
     SegTable T;
     Map4 M;
     int st = make_table(segs, nseg, T, nullptr);
     if (st == VQ_OK) st = check_cache(kc, vc, kv_heads, hd, T, true, page_table, page_size, pages_per_seq, pages, 0, M);
-    return st != VQ_OK ? st : launch_attention4(q, kc, vc, out, T, M, heads, hd, 0, 0, static_cast<hipStream_t>(stream));
+    return st != VQ_OK ? st : launch_attention4(q, kc, vc, out, T, M, heads, hd, 0, 0, workspace, workspace_bytes,
+                                                static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"
