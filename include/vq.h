@@ -38,6 +38,7 @@ extern "C" {
 #define VQ_ERR_ARG (-4)       /* NULL pointer or other invalid argument                     */
 #define VQ_ERR_NOT_INIT (-5)  /* vq_init() has not run on this device                        */
 #define VQ_ERR_TOO_LARGE (-6) /* the call needs more than VQ_NOALLOC_SCRATCH_BYTES of scratch   */
+#define VQ_ERR_NO_PAGES (-7)  /* fewer free pages than the call needs                            */
 
 /* GGUF type ids accepted by every entry point (qwen_quant.cuh:17-33, parser.py:33-63). */
 #define VQ_TYPE_F32 0
@@ -290,6 +291,34 @@ int vq_attention4_seg_ws(const float *q, const void *kc, const void *vc, float *
  * in the reference, whose page table is written by its caller (set_paging, qwen_runtime.cu:2333-2350). */
 int vq_move_pages(void *const *pools, const size_t *page_bytes, int npools, int pages, const int32_t *copies, int ncopies,
                   int32_t *page_table, int table_entries, const int32_t *entries, int nentries, void *stream);
+
+/* The book of a page pool: which pages each sequence slot holds. Host memory only, made for `pages` pages of page_size positions and
+ * the page table's slots and pages_per_seq (NULL: invalid shape or no memory); one thread's call at a time. A page may be held by
+ * several slots and is free again when the last lets go; fresh pages are the lowest free ones. A call checks everything first:
+ * a negative status (VQ_ERR_SHAPE, VQ_ERR_ARG, VQ_ERR_NO_PAGES; vq_book_error has the words) means that nothing has changed.
+ * Otherwise its plan, page copies and table entries as vq_move_pages takes them, stands until the book's next call, and
+ * vq_book_apply carries it out and clears it.
+ *   reserve  the pages that segments [n][4] (slot, pos0, rows, -) are about to write become the slot's own: missing ones are taken,
+ *            shared ones replaced, by a copy unless the segment writes the whole page
+ *   fork     empty slots dst hold the pages of src's first `length` positions too
+ *   copy     pairs [n][3] (src, dst, length): empty slot dst gets copies of src's first `length` positions
+ *   free     the slots keep the pages of their first `length` positions
+ *   compact  the pages in use become the lowest ids
+ * vq_book_row: a slot's page count, and where its pages stand until the next call. No counterpart in the reference. */
+typedef struct vq_book vq_book;
+vq_book *vq_book_create(int pages, int page_size, int pages_per_seq, int slots);
+void vq_book_destroy(vq_book *book);
+int vq_book_reserve(vq_book *book, const int32_t *segs, int nseg);
+int vq_book_fork(vq_book *book, int src, const int32_t *dst, int ndst, int length);
+int vq_book_copy(vq_book *book, const int32_t *pairs, int n);
+int vq_book_free(vq_book *book, const int32_t *slots, int n, int length);
+int vq_book_compact(vq_book *book);
+int vq_book_plan(const vq_book *book, const int32_t **copies, int *ncopies, const int32_t **entries, int *nentries);
+int vq_book_row(const vq_book *book, int slot, const int32_t **pages);
+int vq_book_available(const vq_book *book);
+int vq_book_holders(const vq_book *book, int page);
+const char *vq_book_error(const vq_book *book);
+int vq_book_apply(vq_book *book, void *const *pools, const size_t *page_bytes, int npools, int32_t *page_table, void *stream);
 
 /* Causal depthwise conv + SiLU over ntok tokens: per channel the state [channels][K] (K <= VQ_CONV_MAX_K) holds
  * the last K inputs; per token it shifts, appends x[t][c], and out[t][c] = silu(state . w[c]). snap (may be

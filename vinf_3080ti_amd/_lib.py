@@ -60,6 +60,19 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "vq_attention4_ws": (I, [P, P, P, P, I, I, I, I, I, I, I, I, P, SZ, P]),
     "vq_attention4_seg_ws": (I, [P, P, P, P, P, I, I, I, I, P, I, I, I, P, SZ, P]),
     "vq_move_pages": (I, [P, P, I, I, P, I, P, I, P, I, P]),
+    "vq_book_create": (P, [I, I, I, I]),
+    "vq_book_destroy": (None, [P]),
+    "vq_book_reserve": (I, [P, P, I]),
+    "vq_book_fork": (I, [P, I, P, I, I]),
+    "vq_book_copy": (I, [P, P, I]),
+    "vq_book_free": (I, [P, P, I, I]),
+    "vq_book_compact": (I, [P]),
+    "vq_book_plan": (I, [P, P, P, P, P]),
+    "vq_book_row": (I, [P, I, P]),
+    "vq_book_available": (I, [P]),
+    "vq_book_holders": (I, [P, I]),
+    "vq_book_error": (ctypes.c_char_p, [P]),
+    "vq_book_apply": (I, [P, P, P, I, P, P]),
     "vq_conv_update": (I, [P, P, P, P, I, I, I, P, I, P]),
     "vq_conv_update_seg": (I, [P, P, P, P, I, I, P, I, P, I, P]),
     "vq_gated_delta": (I, [P, P, P, P, P, P, I, P, I, I, I, I, F, I, I, P, I, P]),
@@ -91,7 +104,7 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "vq_verify_draft": (I, [P, P, P, P, P, P, P, I, P, P, I, P, SZ, P]),
 }
 
-VQ_OK, VQ_ERR_TYPE, VQ_ERR_SHAPE, VQ_ERR_WORKSPACE, VQ_ERR_ARG, VQ_ERR_NOT_INIT, VQ_ERR_TOO_LARGE = 0, -1, -2, -3, -4, -5, -6
+VQ_OK, VQ_ERR_TYPE, VQ_ERR_SHAPE, VQ_ERR_WORKSPACE, VQ_ERR_ARG, VQ_ERR_NOT_INIT, VQ_ERR_TOO_LARGE, VQ_ERR_NO_PAGES = 0, -1, -2, -3, -4, -5, -6, -7
 VQ_NOALLOC_SCRATCH_BYTES = 32 << 20
 VQ_GEMM_BATCH_INVARIANT = 1
 
@@ -141,6 +154,6 @@ def check(status: int, context: str) -> None:
     """Raise the reference's exception types for a non-zero status (qwen_runtime.cu:1100-1103)."""
     if status == VQ_OK:
         return
-    if status in (VQ_ERR_TYPE, VQ_ERR_SHAPE, VQ_ERR_ARG):
+    if status in (VQ_ERR_TYPE, VQ_ERR_SHAPE, VQ_ERR_ARG, VQ_ERR_NO_PAGES):
         raise ValueError(f"{context}: {status_text(status)}")
     raise RuntimeError(f"{context} failed: {status_text(status)}")

@@ -391,6 +391,7 @@ const char *vq_status_string(int status) {
         case VQ_ERR_ARG: return "invalid argument";
         case VQ_ERR_NOT_INIT: return "library not initialised on this device";
         case VQ_ERR_TOO_LARGE: return "needs more than the static scratch of the no-allocation entry point";
+        case VQ_ERR_NO_PAGES: return "page pool exhausted";
         default: return status > 0 ? hipGetErrorString(static_cast<hipError_t>(status)) : "unknown error";
     }
 }

@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from .gguf_types import HIP_MATVEC_TYPES, GGUFTensorType, traits
-from .pages import PageBook, as_pairs
+from .pages import PageBook
 
 MAX_TOKENS = 8  # tokens per matvec launch (kMaxTokens, qwen_runtime.cu:572)
 MAX_ARGMAX_ROWS = 256  # kMaxArgmaxRows (qwen_runtime.cu:573)
@@ -775,8 +775,8 @@ class Runtime:
         _, page, per_slot, slots = self._paging
         self._pages = (PageBook(int(pages), page, per_slot, slots), dict(zip(names, sizes)))
 
-    def _page_work(self, plan, what: str) -> int:
-        """plan(book) -> (copies, entries), then both on the device; returns the pages copied."""
+    def _page_work(self, what: str, plan, *args) -> int:
+        """PageBook's call plan(*args), then what it decided on the device; returns the pages copied."""
         if self._pages is None or self._paging is None:
             raise RuntimeError("set_page_pools first")
         with self._pages_lock:
@@ -790,44 +790,39 @@ class Runtime:
             table, _, _ = self._page_table()
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"{what}: page work cannot be captured")
-            copies, entries = plan(book)
-            if copies or entries:
-                n, ca, ea = len(ptrs), as_pairs(copies), as_pairs(entries)
-                st = self._lib.vq_move_pages((ctypes.c_void_p * n)(*ptrs), (ctypes.c_size_t * n)(*pools.values()), n, book.pages,
-                                             ca.ctypes.data, len(copies), table, book.per_slot * book.slots, ea.ctypes.data,
-                                             len(entries), self._stream())
-                _lib.check(st, what)
-            return len(copies)
+            plan(book, *args)
+            copied = book.copies()
+            book.apply(ptrs, pools.values(), table, self._stream())
+            return copied
 
     def pages_reserve(self, segments) -> None:
         """Make the rows that a pass is about to write ((slot, pos0, rows, ...) as in set_segments) the slot's own: pages that it
         lacks are taken, pages that it shares replaced by copies. ValueError when the pool has too few, and nothing changes."""
-        self._page_work(lambda book: book.reserve(segments), "pages_reserve")
+        self._page_work("pages_reserve", PageBook.reserve, segments)
 
     def pages_fork(self, src: int, dst: Sequence[int], length: int) -> None:
         """Empty slots dst begin as src's first `length` positions, in the same pages (pages_reserve parts them where one is
         written)."""
-        self._page_work(lambda book: ([], book.fork(src, dst, length)), "pages_fork")
+        self._page_work("pages_fork", PageBook.fork, src, dst, length)
 
     def pages_copy(self, pairs) -> None:
         """(src, dst, length) each: empty slot dst gets a copy of src's first `length` positions in pages of its own."""
-        self._page_work(lambda book: book.copy(pairs), "pages_copy")
+        self._page_work("pages_copy", PageBook.copy, pairs)
 
     def pages_free(self, slots: Sequence[int], length: int = 0) -> None:
         """The slots give back the pages behind their first `length` positions (all of them by default; after a verification that
         refused drafts, those behind what was accepted). Table entries are left as they are."""
-        self._page_work(lambda book: (book.free(slots, length), ([], []))[1], "pages_free")
+        self._page_work("pages_free", PageBook.free, slots, length)
 
     def pages_compact(self) -> int:
         """Move pages so that those in use are the lowest ids; returns how many moved."""
-        return self._page_work(lambda book: book.compact(), "pages_compact")
+        return self._page_work("pages_compact", PageBook.compact)
 
     def pages_of(self, slot: int) -> list[int]:
         """The pages that a slot holds, in the order of its positions."""
         if self._pages is None:
             raise RuntimeError("set_page_pools first")
-        book = self._pages[0]
-        return list(book.rows[book._slot(slot)])
+        return self._pages[0].row(slot)
 
     def pages_available(self) -> int:
         """Pages that no slot holds."""
