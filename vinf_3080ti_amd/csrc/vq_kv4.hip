@@ -209,21 +209,30 @@ __global__ __launch_bounds__(kMaxHd) void kv4_read_kernel(const uint8_t *__restr
 
 typedef _Float16 fh2 __attribute__((ext_vector_type(2)));
 
+// A 32-bit constant in a VGPR: a VOP3 instruction takes no literal and one SGPR at most, so (a & m) | b with two constants is one
+// instruction only where they are in VGPRs.
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t c) {
+    uint32_t r;
+    asm("v_mov_b32 %0, %1" : "=v"(r) : "i"(c));
+    return r;
+}
+// The low nibbles of a register's halves as the f16 pair 1024 + nibble.
+__device__ __forceinline__ fh2 plus_1024(uint32_t w) { return __builtin_bit_cast(fh2, (w & in_vgpr(0x000F000Fu)) | in_vgpr(0x64006400u)); }
+
 // A header pair's scales and 1024 + zero points. A code c in the low bits of the f16 1024 is 1024 + c, so (1024 + c) - (1024 + z)
 // and its product with the scale are exact.
 struct Heads2 {
     fh2 d, z;
 };
 __device__ __forceinline__ Heads2 heads2(uint32_t h) {
-    return Heads2{__builtin_bit_cast(fh2, h & 0xFFF0FFF0u), __builtin_bit_cast(fh2, (h & 0x000F000Fu) | 0x64006400u)};
+    return Heads2{__builtin_bit_cast(fh2, h & 0xFFF0FFF0u), plus_1024(h)};
 }
 // The eight values of a word: elements 2 i, 2 i + 1 with h[i].
 __device__ __forceinline__ fh8 decode8(uint32_t w, const Heads2 (&h)[4]) {
     fh8 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const fh2 c = __builtin_bit_cast(fh2, ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u);
-        const fh2 v = (c - h[i].z) * h[i].d;
+        const fh2 v = (plus_1024(w >> (4 * i)) - h[i].z) * h[i].d;
         r[2 * i] = v[0];
         r[2 * i + 1] = v[1];
     }
@@ -406,34 +415,34 @@ struct Raw4 {
     uint32_t k[2][U], kh[2][(U + 1) / 2], v[2 * U];
     uint4 vh;
 };
-template <int U, bool PAGED>
-__device__ __forceinline__ void issue_block(const uint8_t *__restrict__ kc, const uint8_t *__restrict__ vc, const Map4 &M, int slot,
-                                            int kvh, int kb, int last, Raw4<U> &r) {
+template <int U>
+__device__ __forceinline__ void issue_k(const uint8_t *__restrict__ kc, const SlabAt &at, Raw4<U> &r) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    // Slabs past the last key's read that one's (their keys are masked).
-    const SlabAt ks = slab_at<U, PAGED>(M, slot, kvh, min(kb / kSlab + (c >> 2), last));
-    const SlabAt vs = slab_at<U, PAGED>(M, slot, kvh, min(kb / kSlab + g, last));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int row = 4 * h + (c & 3);
-        ld_words<U>(kc + ks.words + row * (16 * U) + g * (4 * U), r.k[h]);
-        ld_heads<U>(kc + ks.heads + row * (2 * U), r.kh[h]);
+        ld_words<U>(kc + at.words + row * (16 * U) + g * (4 * U), r.k[h]);
+        ld_heads<U>(kc + at.heads + row * (2 * U), r.kh[h]);
     }
-    constexpr int W = U % 2 == 0 ? 4 : 2;
-#pragma unroll
-    for (int i = 0; i < 2 * U / W; ++i) {
-        uint32_t w[W];
-        ld_words<W>(vc + vs.words + (16 * i + c) * (4 * W), w);
-#pragma unroll
-        for (int k = 0; k < W; ++k) r.v[W * i + k] = w[k];
-    }
-    r.vh = *reinterpret_cast<const uint4 *>(vc + vs.heads + 16 * min(c, U - 1));
-    if (ks.bad) {
+    if (at.bad) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < (U + 1) / 2; ++i) r.kh[h][i] = kNanHeader | kNanHeader << 16;
     }
+}
+template <int U>
+__device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, const SlabAt &at, Raw4<U> &r) {
+    const int c = threadIdx.x & 15;
+    constexpr int W = U % 2 == 0 ? 4 : 2;
+#pragma unroll
+    for (int i = 0; i < 2 * U / W; ++i) {
+        uint32_t w[W];
+        ld_words<W>(vc + at.words + (16 * i + c) * (4 * W), w);
+#pragma unroll
+        for (int k = 0; k < W; ++k) r.v[W * i + k] = w[k];
+    }
+    r.vh = *reinterpret_cast<const uint4 *>(vc + at.heads + 16 * min(c, U - 1));
 }
 
 // Lane n's value of each row of 16 lanes, to all of the row.
@@ -461,9 +470,7 @@ __device__ __forceinline__ void pv_groups(const Raw4<U> &r, const uint32_t (&d)[
 }
 
 template <int U>
-__device__ __forceinline__ void consume_block(const Raw4<U> &r, int kb, int qs, int qe, const fh8 (&qh)[U], const fh8 (&ql)[U], float sinv,
-                                              float &m, float &l, fa4 (&o)[2 * U]) {
-    fa4 s[2];
+__device__ __forceinline__ void scores(const Raw4<U> &r, const fh8 (&qh)[U], const fh8 (&ql)[U], float sinv, fa4 (&s)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         fa4 a0{0.f, 0.f, 0.f, 0.f}, a1{0.f, 0.f, 0.f, 0.f};
@@ -476,12 +483,13 @@ __device__ __forceinline__ void consume_block(const Raw4<U> &r, int kb, int qs, 
         }
         s[h] = (a0 + a1) * sinv;
     }
-    fh8 ph, pl;
-    softmax_step<U>(s, kb, qs, qe, m, l, o, ph, pl);
+}
+template <int U>
+__device__ __forceinline__ void add_values(const Raw4<U> &r, const fh8 &ph, const fh8 &pl, fa4 (&o)[2 * U]) {
     uint32_t d[4], z[4];
     const uint32_t raw[4] = {r.vh.x, r.vh.y, r.vh.z, r.vh.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = raw[i] & 0xFFF0FFF0u, z[i] = (raw[i] & 0x000F000Fu) | 0x64006400u;
+    for (int i = 0; i < 4; ++i) d[i] = raw[i] & 0xFFF0FFF0u, z[i] = __builtin_bit_cast(uint32_t, plus_1024(raw[i]));
     pv_groups<U, 0>(r, d, z, ph, pl, o);
 }
 
@@ -512,15 +520,32 @@ __global__ __launch_bounds__(256, 2) void attention4_split_kernel(const float *_
     fa4 o[2 * U];
 #pragma unroll
     for (int b = 0; b < 2 * U; ++b) o[b] = fa4{0.f, 0.f, 0.f, 0.f};
+    // Lane (c, g) takes K rows of slab c >> 2 and V words of slab g of a block; slabs past the last key's read that one's (masked).
+    auto places = [&](int kb, SlabAt &ks, SlabAt &vs) {
+        ks = slab_at<U, PAGED>(M, s.slot, kvh, min(kb / kSlab + (c >> 2), last));
+        vs = slab_at<U, PAGED>(M, s.slot, kvh, min(kb / kSlab + g, last));
+    };
     int kb = k_lo + 32 * wv;
     Raw4<U> r;
-    if (kb < k_hi) issue_block<U, PAGED>(kc, vc, M, s.slot, kvh, kb, last, r);
+    SlabAt ks, vs;
+    if (kb < k_hi) {
+        places(kb, ks, vs);
+        issue_k<U>(kc, ks, r);
+        issue_v<U>(vc, vs, r);
+    }
     fh8 qh[U], ql[U];
     const float sinv = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
     for (; kb < k_hi; kb += 128) {
-        const Raw4<U> now = r;
-        if (kb + 128 < k_hi) issue_block<U, PAGED>(kc, vc, M, s.slot, kvh, kb + 128, last, r);
-        consume_block<U>(now, kb, see.from, qe, qh, ql, sinv, m, l, o);
+        // The next block's K and V come into the registers that this block's have left.
+        const bool more = kb + 128 < k_hi;
+        if (more) places(kb + 128, ks, vs);
+        fa4 sc[2];
+        scores<U>(r, qh, ql, sinv, sc);
+        if (more) issue_k<U>(kc, ks, r);
+        fh8 ph, pl;
+        softmax_step<U>(sc, kb, see.from, qe, m, l, o, ph, pl);
+        add_values<U>(r, ph, pl, o);
+        if (more) issue_v<U>(vc, vs, r);
     }
     float *ow = sums + wv * 16 * HD;
 #pragma unroll
