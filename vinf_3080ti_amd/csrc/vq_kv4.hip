@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "../../include/vq.h"
+#include "vq_lds.h"
 #include "vq_seq.h"
 
 namespace {
@@ -38,6 +39,32 @@ __device__ __forceinline__ Place place(const Map4 &M, int slot, int kvh, uint32_
     return Place{(static_cast<size_t>(bad ? 0 : pg) * M.kv_heads + kvh) * M.bytes, slab - p * M.spp, bad};
 }
 
+// ---- segments ----------------------------------------------------------------------------------------------
+
+// Where each segment's rows (or other units of a grid) begin, and how many there are in all.
+struct Starts {
+    int total;
+    int first[VQ_MAX_SEGMENTS];
+};
+
+// A segment as a workgroup finds it: the last one whose beginning is <= x. Lane i loads segment i and what goes with it, all at
+// once, and the found one's values come from its lane. Kernel arguments lie in host memory, 2 us away at the first touch, and one
+// load after the other (a walk over the segments, then their rows, then their bases) made up a third of a decode step's time.
+struct Found {
+    Seg s;
+    int index, first, next;  // beginning of the segment, and of the next one
+};
+__device__ __forceinline__ int from_lane(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ Found find_segment(const SegTable &T, const int *first, int total, int x) {
+    const int lane = threadIdx.x & 63;
+    const Seg mine = T.s[lane];
+    const int f = first[lane], n = T.n;
+    const int i = __builtin_popcountll(__ballot(lane < n && f <= x)) - 1;
+    return Found{Seg{from_lane(mine.slot, i), from_lane(mine.pos0, i), from_lane(mine.rows, i), from_lane(mine.row0, i)}, i,
+                 from_lane(f, i), i + 1 < n ? from_lane(f, i + 1 < 64 ? i + 1 : 63) : total};
+}
+// ---- values --------------------------------------------------------------------------------------------------
+
 // Word of dim d among a V slab's hd words.
 __device__ __forceinline__ int v_word(int d, int hd) {
     const int w = hd % 64 == 0 ? 4 : 2;
@@ -53,46 +80,42 @@ __device__ __forceinline__ float value_of(uint32_t header, uint32_t code) {
     return scale_of(header) * static_cast<float>(static_cast<int>(code) - static_cast<int>(header & 15u));
 }
 
-// Value of dim d at a slab's position r (place from place<>(); spp and bytes of the block from M).
-__device__ __forceinline__ float k_value(const uint8_t *kc, const Map4 &M, const Place &at, int r, int hd, int d) {
-    const uint8_t *b = kc + at.at;
-    const size_t pos = static_cast<size_t>(at.slab) * kSlab + r;
-    const uint32_t w = reinterpret_cast<const uint32_t *>(b)[pos * (hd / 8) + ((d >> 3) & 3) * (hd / 32) + (d >> 5)];
-    const uint16_t *h = reinterpret_cast<const uint16_t *>(b + static_cast<size_t>(M.spp) * kSlab * (hd / 2));
-    return value_of(at.bad ? kNanHeader : h[pos * (hd / 32) + (d >> 5)], (w >> nib(d & 7)) & 15u);
-}
-__device__ __forceinline__ float v_value(const uint8_t *vc, const Map4 &M, const Place &at, int r, int hd, int d) {
-    const uint8_t *b = vc + at.at;
-    const uint32_t w = reinterpret_cast<const uint32_t *>(b)[static_cast<size_t>(at.slab) * hd + v_word(d, hd)];
-    const uint16_t *h = reinterpret_cast<const uint16_t *>(b + static_cast<size_t>(M.spp) * kSlab * (hd / 2));
-    return value_of(at.bad ? kNanHeader : h[(static_cast<size_t>(at.slab) * (hd / 32) + (d >> 5)) * 8 + r], (w >> nib(r)) & 15u);
-}
-
 // ---- append ------------------------------------------------------------------------------------------------
 
 // x / d to the nearest whole number, ties to even, for |x / d| of up to 2^22: the rounded product with the reciprocal is at most
-// one off, and the remainder x - n d is exact where it decides (n d has at most 12 significant bits).
-__device__ __forceinline__ float nearest(float x, float d, float inv) {
-    float n = rintf(x * inv);
-    const float e = fmaf(-n, d, x), half = 0.5f * d;
-    const bool odd = n - 2.0f * floorf(0.5f * n) != 0.0f;
-    if (e > half || (e == half && odd)) n += 1.0f;
-    else if (e < -half || (e == -half && odd)) n -= 1.0f;
-    return n;
+// one off, and the remainder x - n d is exact where it decides (n d has at most 12 significant bits). Off it is only near a tie,
+// so the correction is behind a branch that few waves take.
+template <int N>
+__device__ __forceinline__ void nearest(const float (&x)[N], float d, float inv, float (&n)[N]) {
+    const float half = 0.5f * d;
+    bool near_tie = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        n[i] = rintf(x[i] * inv);
+        near_tie = near_tie || fabsf(fmaf(-n[i], d, x[i])) >= half;
+    }
+    if (!__any(near_tie)) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float e = fmaf(-n[i], d, x[i]);
+        const bool odd = n[i] - 2.0f * floorf(0.5f * n[i]) != 0.0f;
+        if (e > half || (e == half && odd)) n[i] += 1.0f;
+        else if (e < -half || (e == -half && odd)) n[i] -= 1.0f;
+    }
 }
 
 // Scale of a group whose values, with zero, span [lo, hi]: the smallest k 2^e, k < 128, e >= -20, with 15 k 2^e >= hi - lo. The
 // first guess from a rounded quotient is at most one k off; 15 k 2^e and the span are compared in 64 bits.
 __device__ __forceinline__ float scale_for(float lo, float hi) {
     const double span = static_cast<double>(hi) - static_cast<double>(lo);
-    const float t = static_cast<float>(span / 15.0);
+    const float t = static_cast<float>(span * (1.0 / 15.0));
     if (!(t < kMaxScale)) return kMaxScale;
-    int ex = -99;
-    if (t > 0.0f) frexpf(t, &ex);  // t = f 2^ex, f in [0.5, 1); a span too small for t takes the smallest step
-    const float step = ldexpf(1.0f, ex - 7 > -20 ? ex - 7 : -20);
-    float k = ceilf(t / step);  // exact: step is a power of two
-    while (k > 0.0f && 15.0 * static_cast<double>((k - 1.0f) * step) >= span) k -= 1.0f;
-    while (15.0 * static_cast<double>(k * step) < span) k += 1.0f;
+    // t = f 2^ex, f in [0.5, 1); a span too small for t takes the smallest step.
+    const int ex = t > 0.0f ? __builtin_amdgcn_frexp_expf(t) : -99, by = ex - 7 > -20 ? ex - 7 : -20;
+    const float step = __uint_as_float(static_cast<uint32_t>(127 + by) << 23);
+    float k = ceilf(t * __uint_as_float(static_cast<uint32_t>(127 - by) << 23));  // t / step, exact
+    if (15.0 * static_cast<double>((k - 1.0f) * step) >= span && k > 0.0f) k -= 1.0f;
+    if (15.0 * static_cast<double>(k * step) < span) k += 1.0f;
     return fminf(k * step, kMaxScale);
 }
 
@@ -108,16 +131,20 @@ __device__ __forceinline__ Group4 quantize_group4(const float (&x)[8]) {
     for (int e = 0; e < 8; ++e) lo = fminf(lo, x[e]), hi = fmaxf(hi, x[e]);
 #pragma unroll
     for (int o = 1; o <= 2; o <<= 1) lo = fminf(lo, __shfl_xor(lo, o, 64)), hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-    const float d = scale_for(lo, hi);
-    if (!(d > 0.0f)) return Group4{0u, 0u};
-    const float inv = 1.0f / d, z = fminf(nearest(-lo, d, inv), 15.0f);
+    float d = scale_for(lo, hi);
+    const bool some = d > 0.0f;
+    d = some ? d : 1.0f;
+    // Values past 16 steps, which only the largest scale leaves, are cut: their code is at an end of the range anyway.
+    float v[9], n[9];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fminf(fmaxf(x[e], -16.0f * d), 16.0f * d);
+    v[8] = fminf(-lo, 16.0f * d);
+    nearest(v, d, 1.0f / d, n);
+    const float z = fminf(n[8], 15.0f);
     uint32_t w = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        // Past the saturated range (d = 4352) only the sign of the quotient matters.
-        const float c = fminf(fmaxf(nearest(fminf(fmaxf(x[e], -16.0f * d), 16.0f * d), d, inv) + z, 0.0f), 15.0f);
-        w |= static_cast<uint32_t>(c) << nib(e);
-    }
+    for (int e = 0; e < 8; ++e) w |= static_cast<uint32_t>(fminf(fmaxf(n[e] + z, 0.0f), 15.0f)) << nib(e);
+    if (!some) return Group4{0u, 0u};
     return Group4{w, static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(d))) | static_cast<uint32_t>(z)};
 }
 
@@ -128,19 +155,14 @@ __device__ __forceinline__ Group4 quantize_group4(const float (&x)[8]) {
 // written for a (k, v) pair.
 template <bool PAGED>
 __global__ __launch_bounds__(kMaxHd) void kv4_append_kernel(const float *__restrict__ k, const float *__restrict__ v, uint8_t *kc,
-                                                            uint8_t *vc, SegTable T, Map4 M, int hd) {
+                                                            uint8_t *vc, SegTable T, Starts R, Map4 M, int hd) {
     __shared__ uint32_t vw[kSlab][kMaxHd / 8];
     __shared__ int broken[kSlab];
     const int kvh = blockIdx.y, tid = threadIdx.x;
-    int b = blockIdx.x, si = 0;  // (segment, slab of it)
-    while (si + 1 < T.n) {
-        const int n = (T.s[si].pos0 + T.s[si].rows - 1) / kSlab - T.s[si].pos0 / kSlab + 1;
-        if (b < n) break;
-        b -= n;
-        ++si;
-    }
-    const Seg &s = T.s[si];
-    const int slab = s.pos0 / kSlab + b, r0 = max(s.pos0 - slab * kSlab, 0), r1 = min(s.pos0 + s.rows - slab * kSlab, kSlab);
+    const Found found = find_segment(T, R.first, R.total, blockIdx.x);
+    const Seg s = found.s;
+    const int slab = s.pos0 / kSlab + (blockIdx.x - found.first);
+    const int r0 = max(s.pos0 - slab * kSlab, 0), r1 = min(s.pos0 + s.rows - slab * kSlab, kSlab);
     const Place at = place<PAGED>(M, s.slot, kvh, slab);
     if (at.bad) return;
     const int per = hd / 8, row = tid / per, i = tid - row * per;
@@ -149,17 +171,19 @@ __global__ __launch_bounds__(kMaxHd) void kv4_append_kernel(const float *__restr
     float x[2][8];
     if (tid < kSlab) broken[tid] = 0;
     __syncthreads();
+    // Threads without a row read the segment's first one of the slab, and count as zeros.
+    const size_t src = (static_cast<size_t>(s.row0 + slab * kSlab + (on ? row : r0) - s.pos0) * M.kv_heads + kvh) * hd + 8 * i;
+    __builtin_memcpy(x[0], k + src, 32);
+    __builtin_memcpy(x[1], v + src, 32);
+    bool ok = true;
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-        const size_t src = on ? (static_cast<size_t>(s.row0 + slab * kSlab + row - s.pos0) * M.kv_heads + kvh) * hd + 8 * i : 0;
-        bool ok = true;
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[a][e] = on ? (a == 0 ? k : v)[src + e] : 0.0f;
+            x[a][e] = on ? x[a][e] : 0.0f;
             ok = ok && fabsf(x[a][e]) < INFINITY;
         }
-        if (!ok) broken[row] = 1;
-    }
+    if (!ok) broken[row] = 1;
     __syncthreads();
     const bool nan = on && broken[row] != 0;
 #pragma unroll
@@ -191,18 +215,42 @@ __global__ __launch_bounds__(kMaxHd) void kv4_append_kernel(const float *__restr
     else atomicXor(to, (*to ^ w) & mine);
 }
 
-// The values held at the rows' positions: one workgroup per (row, kv head), thread d dim d.
+// The values held at the rows' positions, by the append kernel's workgroups: hd / 8 threads take a K row, a word each, and thread d
+// the V word of dim d, whose positions are as many rows of the output. Bound by bytes: 9/8 read, 8 written for a (k, v) pair.
 template <bool PAGED>
 __global__ __launch_bounds__(kMaxHd) void kv4_read_kernel(const uint8_t *__restrict__ kc, const uint8_t *__restrict__ vc,
-                                                          float *__restrict__ k, float *__restrict__ v, SegTable T, Map4 M, int hd) {
-    int t;
-    const Seg &s = seg_of_row(T, blockIdx.x, t);
-    const int pos = s.pos0 + t, d = threadIdx.x;
-    if (d >= hd) return;
-    const Place at = place<PAGED>(M, s.slot, blockIdx.y, pos / kSlab);
-    const size_t dst = (static_cast<size_t>(s.row0 + t) * M.kv_heads + blockIdx.y) * hd + d;
-    k[dst] = k_value(kc, M, at, pos % kSlab, hd, d);
-    v[dst] = v_value(vc, M, at, pos % kSlab, hd, d);
+                                                          float *__restrict__ k, float *__restrict__ v, SegTable T, Starts R, Map4 M,
+                                                          int hd) {
+    const int kvh = blockIdx.y, tid = threadIdx.x;
+    const Found found = find_segment(T, R.first, R.total, blockIdx.x);
+    const Seg s = found.s;
+    const int slab = s.pos0 / kSlab + (blockIdx.x - found.first);
+    const int r0 = max(s.pos0 - slab * kSlab, 0), r1 = min(s.pos0 + s.rows - slab * kSlab, kSlab);
+    const Place at = place<PAGED>(M, s.slot, kvh, slab);
+    const int per = hd / 8, row = tid / per, i = tid - row * per;
+    const size_t head = static_cast<size_t>(M.spp) * kSlab * (hd / 2);
+    const size_t stride = static_cast<size_t>(M.kv_heads) * hd;  // of a row of k and v
+    const size_t dst = (static_cast<size_t>(s.row0) * M.kv_heads + kvh) * hd;
+    auto row_at = [&](int r) { return dst + static_cast<size_t>(slab * kSlab + r - s.pos0) * stride; };
+    if (row >= r0 && row < r1) {
+        const size_t pos = static_cast<size_t>(at.slab) * kSlab + row;
+        const uint8_t *b = kc + at.at;
+        const uint32_t w = reinterpret_cast<const uint32_t *>(b)[pos * per + (i & 3) * (hd / 32) + (i >> 2)];
+        const uint32_t h = at.bad ? kNanHeader : reinterpret_cast<const uint16_t *>(b + head)[pos * (hd / 32) + (i >> 2)];
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = value_of(h, (w >> nib(e)) & 15u);
+        __builtin_memcpy(k + row_at(row) + 8 * i, x, 32);
+    }
+    if (tid >= hd) return;
+    const uint8_t *b = vc + at.at;
+    const uint32_t w = reinterpret_cast<const uint32_t *>(b)[static_cast<size_t>(at.slab) * hd + v_word(tid, hd)];
+    uint4 hv = *reinterpret_cast<const uint4 *>(b + head + (static_cast<size_t>(at.slab) * (hd / 32) + (tid >> 5)) * 16);
+    if (at.bad) hv = uint4{kNanHeader * 0x10001u, kNanHeader * 0x10001u, kNanHeader * 0x10001u, kNanHeader * 0x10001u};
+    const uint32_t h[4] = {hv.x, hv.y, hv.z, hv.w};
+#pragma unroll
+    for (int r = 0; r < kSlab; ++r)
+        if (r >= r0 && r < r1) v[row_at(r) + tid] = value_of(h[r / 2] >> (16 * (r & 1)) & 0xFFFFu, (w >> nib(r)) & 15u);
 }
 
 // ---- attention -----------------------------------------------------------------------------------------------
@@ -216,23 +264,22 @@ __device__ __forceinline__ uint32_t in_vgpr(uint32_t c) {
     asm("v_mov_b32 %0, %1" : "=v"(r) : "i"(c));
     return r;
 }
-// The low nibbles of a register's halves as the f16 pair 1024 + nibble.
+// A code c in the low bits of the f16 1024 is 1024 + c, one in bits 4 .. 7 of the f16 64 is 64 + c: the first and second nibble of a
+// register's halves become such pairs in one instruction. Less 1024 + z or 64 + z, and times the scale, both are exact.
 __device__ __forceinline__ fh2 plus_1024(uint32_t w) { return __builtin_bit_cast(fh2, (w & in_vgpr(0x000F000Fu)) | in_vgpr(0x64006400u)); }
+__device__ __forceinline__ fh2 plus_64(uint32_t w) { return __builtin_bit_cast(fh2, (w & in_vgpr(0x00F000F0u)) | in_vgpr(0x54005400u)); }
 
-// A header pair's scales and 1024 + zero points. A code c in the low bits of the f16 1024 is 1024 + c, so (1024 + c) - (1024 + z)
-// and its product with the scale are exact.
-struct Heads2 {
-    fh2 d, z;
-};
-__device__ __forceinline__ Heads2 heads2(uint32_t h) {
-    return Heads2{__builtin_bit_cast(fh2, h & 0xFFF0FFF0u), plus_1024(h)};
-}
-// The eight values of a word: elements 2 i, 2 i + 1 with h[i].
-__device__ __forceinline__ fh8 decode8(uint32_t w, const Heads2 (&h)[4]) {
+// A pair of headers' scales and zero points, in both forms.
+__device__ __forceinline__ fh2 scales2(uint32_t h) { return __builtin_bit_cast(fh2, h & 0xFFF0FFF0u); }
+__device__ __forceinline__ fh2 zeros2(uint32_t h, bool second) { return second ? plus_64(h << 4) : plus_1024(h); }
+
+// The eight values of a word: elements 2 i, 2 i + 1 with scales d[i] and zero points z[i], of the second form for odd i.
+__device__ __forceinline__ fh8 decode8(uint32_t w, const fh2 (&d)[4], const fh2 (&z)[4]) {
     fh8 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const fh2 v = (plus_1024(w >> (4 * i)) - h[i].z) * h[i].d;
+        const uint32_t x = i < 2 ? w : w >> 8;
+        const fh2 v = ((i % 2 == 0 ? plus_1024(x) : plus_64(x)) - z[i]) * d[i];
         r[2 * i] = v[0];
         r[2 * i + 1] = v[1];
     }
@@ -240,10 +287,11 @@ __device__ __forceinline__ fh8 decode8(uint32_t w, const Heads2 (&h)[4]) {
 }
 // All of them with the low (or high) header of a pair.
 template <bool HIGH>
-__device__ __forceinline__ fh8 decode8_one(uint32_t w, const Heads2 &h) {
-    const Heads2 one{fh2{h.d[HIGH], h.d[HIGH]}, fh2{h.z[HIGH], h.z[HIGH]}};
-    const Heads2 all[4] = {one, one, one, one};
-    return decode8(w, all);
+__device__ __forceinline__ fh8 decode8_one(uint32_t w, uint32_t h) {
+    const fh2 d = scales2(h), z0 = zeros2(h, false), z1 = zeros2(h, true);
+    const fh2 dd{d[HIGH], d[HIGH]}, a{z0[HIGH], z0[HIGH]}, b{z1[HIGH], z1[HIGH]};
+    const fh2 ds[4] = {dd, dd, dd, dd}, zs[4] = {a, b, a, b};
+    return decode8(w, ds, zs);
 }
 
 // N words (16 B aligned where N allows it) as N registers.
@@ -298,24 +346,45 @@ __device__ __forceinline__ SlabAt slab_at(const Map4 &M, int slot, int kvh, int 
 //  - O^T += V^T P^T: k slot (g, j) is key 8 g + j, so B is the lane's own eight weights in order and A, dims 16 b + c of V^T at
 //    positions 8 g .. 8 g + 7, is one V word of slab g.
 
-// The lane's query vector as B operands; returns the factor that brings a score to base-2 units (fa16_q_split).
+// The lane's query vector (column c, dims 32 u + 8 g + j) as B operands: times a power of two that brings its largest element near
+// 2^14, as f16 pairs hi + lo (22 significant bits). Returns the factor that takes a product back and into base-2 units of the
+// softmax, log2(e) / sqrt(hd) over that power. 230 instructions: a short context's workgroup runs this once for a block or two.
+__device__ __forceinline__ float max3_abs(float m, float a, float b) {
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(m) : "v"(m), "v"(a), "v"(b));
+    return m;
+}
 template <int U>
 __device__ __forceinline__ float load_query(const float *qrow, fh8 (&qh)[U], fh8 (&ql)[U]) {
     const int g = (threadIdx.x & 63) >> 4;
-    float4 qr[2 * U];
+    float x[U][8], amax = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        __builtin_memcpy(&qr[2 * u], qrow + 32 * u + 8 * g, 16);
-        __builtin_memcpy(&qr[2 * u + 1], qrow + 32 * u + 8 * g + 4, 16);
-    }
-    return fa16_q_split<32 * U>(qr, 1.0f / sqrtf(32.0f * U), qh, ql);
+    for (int u = 0; u < U; ++u) __builtin_memcpy(x[u], qrow + 32 * u + 8 * g, 32);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) amax = max3_abs(amax, x[u][j], x[u][j + 1]);
+    amax = xor32_max(xor16_max(amax));
+    // amax = f 2^ex, f in [0.5, 1). Capped at 2^126, so that the power and its inverse are finite for the smallest queries.
+    const int ex = amax > 0.0f && amax <= 3.0e38f ? __builtin_amdgcn_frexp_expf(amax) : 0, e2 = 14 - ex < 126 ? 14 - ex : 126;
+    const float up = ldexpf(1.0f, e2);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            _Float16 hi, lo;
+            split_h(x[u][j] * up, hi, lo);
+            qh[u][j] = hi;
+            ql[u][j] = lo;
+        }
+    return ldexpf(1.44269504088896341f / sqrtf(32.0f * U), -e2);
 }
 
-// Softmax step over a block's scores s[h][r] (key kb + 8 g + 4 h + r; keys outside [qs, qe) are masked): new running maximum and
-// sum, O rescaled where the maximum moved, the weights as an f16 pair. The sum is of the weights before they are split.
+// Softmax step over a block's products s[h][r] (key kb + 8 g + 4 h + r; keys outside [qs, qe) are masked), which times `unit` are
+// scores in base-2 units: new running maximum and sum, O rescaled where the maximum moved, the weights as an f16 pair (the first
+// half rounded towards zero, the second the rest: 22 significant bits). The sum is of the weights before they are split.
 template <int U>
-__device__ __forceinline__ void softmax_step(const fa4 (&s)[2], int kb, int qs, int qe, float &m, float &l, fa4 (&o)[2 * U], fh8 &ph,
-                                             fh8 &pl) {
+__device__ __forceinline__ void softmax_step(const fa4 (&s)[2], float unit, int kb, int qs, int qe, float &m, float &l, fa4 (&o)[2 * U],
+                                             fh8 &ph, fh8 &pl) {
     const int g = (threadIdx.x & 63) >> 4;
     float v[8], bm = -INFINITY;
 #pragma unroll
@@ -329,18 +398,19 @@ __device__ __forceinline__ void softmax_step(const fa4 (&s)[2], int kb, int qs, 
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) bm = fmaxf(bm, v[j]);
-    bm = xor32_max(xor16_max(bm));
+    bm = xor32_max(xor16_max(bm)) * unit;
     const float mn = fmaxf(m, bm), ms = mn == -INFINITY ? 0.0f : mn;  // ms: exp2(-inf - ms) is 0 also before any key
     const float alpha = __builtin_amdgcn_exp2f(m - ms);
     float ps = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float p = __builtin_amdgcn_exp2f(v[j] - ms);
-        ps += p;
-        _Float16 hh, ll;
-        split_h(p, hh, ll);
-        ph[j] = hh;
-        pl[j] = ll;
+    for (int j = 0; j < 8; j += 2) {
+        const float a = __builtin_amdgcn_exp2f(fmaf(v[j], unit, -ms)), b = __builtin_amdgcn_exp2f(fmaf(v[j + 1], unit, -ms));
+        ps += a;
+        ps += b;
+        const fh2 hi = __builtin_bit_cast(fh2, __builtin_amdgcn_cvt_pkrtz(a, b));
+        const fh2 lo = __builtin_bit_cast(fh2, __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(hi[0]), b - static_cast<float>(hi[1])));
+        ph[j] = hi[0], ph[j + 1] = hi[1];
+        pl[j] = lo[0], pl[j + 1] = lo[1];
     }
     ps = xor32_add(xor16_add(ps));
     l = l * alpha + ps;
@@ -354,9 +424,8 @@ __device__ __forceinline__ void softmax_step(const fa4 (&s)[2], int kb, int qs, 
 // How a pass's contexts are cut: chunks of `len` keys (a multiple of 128) from each segment's first key rounded down to 32, all
 // segments' chunks in one list; segment i's begin at first[i], its partial results at base[i].
 struct Cuts {
-    int len, total;
-    int first[VQ_MAX_SEGMENTS + 1];
-    int base[VQ_MAX_SEGMENTS];
+    int len, total, most;  // most: chunks of a segment
+    int first[VQ_MAX_SEGMENTS], base[VQ_MAX_SEGMENTS];
 };
 // First key that any row of a segment sees, rounded down to a block.
 __host__ __device__ __forceinline__ int first_key(const Seg &s, int window) {
@@ -445,52 +514,54 @@ __device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, const Sl
     r.vh = *reinterpret_cast<const uint4 *>(vc + at.heads + 16 * min(c, U - 1));
 }
 
-// Lane n's value of each row of 16 lanes, to all of the row.
-template <int N>
-__device__ __forceinline__ uint32_t row_bcast(uint32_t v) {
-    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x150 + N, 0xF, 0xF, true));
-}
-
-template <int U, int I>
-__device__ __forceinline__ void pv_groups(const Raw4<U> &r, const uint32_t (&d)[4], const uint32_t (&z)[4], const fh8 &ph, const fh8 &pl,
-                                          fa4 (&o)[2 * U]) {
-    if constexpr (I < U) {
-        Heads2 h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            h[i] = Heads2{__builtin_bit_cast(fh2, row_bcast<I>(d[i])), __builtin_bit_cast(fh2, row_bcast<I>(z[i]))};
-#pragma unroll
-        for (int b = 2 * I; b < 2 * I + 2; ++b) {
-            const fh8 a = decode8(r.v[b], h);
-            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[b], 0, 0, 0);
-            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[b], 0, 0, 0);
-        }
-        pv_groups<U, I + 1>(r, d, z, ph, pl, o);
-    }
-}
-
 template <int U>
-__device__ __forceinline__ void scores(const Raw4<U> &r, const fh8 (&qh)[U], const fh8 (&ql)[U], float sinv, fa4 (&s)[2]) {
+__device__ __forceinline__ void scores(const Raw4<U> &r, const fh8 (&qh)[U], const fh8 (&ql)[U], fa4 (&s)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         fa4 a0{0.f, 0.f, 0.f, 0.f}, a1{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const Heads2 hd2 = heads2(r.kh[h][u / 2]);
-            const fh8 a = u % 2 == 0 ? decode8_one<false>(r.k[h][u], hd2) : decode8_one<true>(r.k[h][u], hd2);
+            const fh8 a = u % 2 == 0 ? decode8_one<false>(r.k[h][u], r.kh[h][u / 2]) : decode8_one<true>(r.k[h][u], r.kh[h][u / 2]);
             a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[u], a0, 0, 0, 0);
             a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[u], a1, 0, 0, 0);
         }
-        s[h] = (a0 + a1) * sinv;
+        s[h] = a0 + a1;
     }
 }
+// O^T += V^T P^T. Every lane of a row of 16 needs the headers of all groups of its slab: lane c takes group c's apart and the others
+// read them from LDS (`hl`, the wave's own: [slab][group] scales, zero points; moving them by DPP costs 64 instructions a block of
+// the kind that bounds this kernel).
 template <int U>
-__device__ __forceinline__ void add_values(const Raw4<U> &r, const fh8 &ph, const fh8 &pl, fa4 (&o)[2 * U]) {
-    uint32_t d[4], z[4];
-    const uint32_t raw[4] = {r.vh.x, r.vh.y, r.vh.z, r.vh.w};
+constexpr int head_words = 4 * (8 * U + 8);
+template <int U>
+__device__ __forceinline__ void add_values(const Raw4<U> &r, const fh8 &ph, const fh8 &pl, uint32_t *hl, fa4 (&o)[2 * U]) {
+    const int lane = threadIdx.x & 63, c = lane & 15;
+    uint32_t *mine = hl + (lane >> 4) * (8 * U + 8);
+    if (c < U) {
+        const uint32_t raw[4] = {r.vh.x, r.vh.y, r.vh.z, r.vh.w};
+        uint32_t d[4], z[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[i] = raw[i] & 0xFFF0FFF0u, z[i] = __builtin_bit_cast(uint32_t, plus_1024(raw[i]));
-    pv_groups<U, 0>(r, d, z, ph, pl, o);
+        for (int i = 0; i < 4; ++i) d[i] = raw[i] & 0xFFF0FFF0u, z[i] = __builtin_bit_cast(uint32_t, zeros2(raw[i], i % 2 != 0));
+        *reinterpret_cast<uint4 *>(mine + 8 * c) = uint4{d[0], d[1], d[2], d[3]};
+        *reinterpret_cast<uint4 *>(mine + 8 * c + 4) = uint4{z[0], z[1], z[2], z[3]};
+    }
+    // A wave's LDS operations complete in order; the fence keeps the compiler from moving the reads above the writes.
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint4 dw = *reinterpret_cast<const uint4 *>(mine + 8 * u), zw = *reinterpret_cast<const uint4 *>(mine + 8 * u + 4);
+        const fh2 d[4] = {__builtin_bit_cast(fh2, dw.x), __builtin_bit_cast(fh2, dw.y), __builtin_bit_cast(fh2, dw.z), __builtin_bit_cast(fh2, dw.w)};
+        const fh2 z[4] = {__builtin_bit_cast(fh2, zw.x), __builtin_bit_cast(fh2, zw.y), __builtin_bit_cast(fh2, zw.z), __builtin_bit_cast(fh2, zw.w)};
+#pragma unroll
+        for (int b = 2 * u; b < 2 * u + 2; ++b) {
+            const fh8 a = decode8(r.v[b], d, z);
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[b], 0, 0, 0);
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");  // every lane has read before the next block's writes
+    __builtin_amdgcn_wave_barrier();
 }
 
 // Decode and verify passes: one workgroup per (chunk, kv head, 16 query vectors); vector j of a segment is (row j / G, head j % G of
@@ -504,12 +575,13 @@ __global__ __launch_bounds__(256, 2) void attention4_split_kernel(const float *_
     constexpr int HD = 32 * U;
     __shared__ __align__(16) float sums[4 * 16 * HD];
     __shared__ float sm[4][16], sl[4][16];
+    __shared__ __align__(16) uint32_t vheads[4][head_words<U>];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % M.kv_heads, list = blockIdx.x / M.kv_heads;
-    int si = 0;
-    while (list >= C.first[si + 1]) ++si;
-    const Seg &s = T.s[si];
-    const int ci = list - C.first[si], n = C.first[si + 1] - C.first[si];
+    const int bases = C.base[lane];
+    const Found found = find_segment(T, C.first, C.total, list);
+    const Seg s = found.s;
+    const int ci = list - found.first, n = found.next - found.first;
     const int G = heads / M.kv_heads, nvec = s.rows * G, j0 = blockIdx.y * 16;
     if (j0 >= nvec) return;
     const int j = min(j0 + c, nvec - 1), t = j / G, h = kvh * G + j - t * G;  // vectors past the last repeat it; not written
@@ -534,68 +606,257 @@ __global__ __launch_bounds__(256, 2) void attention4_split_kernel(const float *_
         issue_v<U>(vc, vs, r);
     }
     fh8 qh[U], ql[U];
-    const float sinv = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
+    const float unit = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
     for (; kb < k_hi; kb += 128) {
         // The next block's K and V come into the registers that this block's have left.
         const bool more = kb + 128 < k_hi;
         if (more) places(kb + 128, ks, vs);
         fa4 sc[2];
-        scores<U>(r, qh, ql, sinv, sc);
+        scores<U>(r, qh, ql, sc);
         if (more) issue_k<U>(kc, ks, r);
         fh8 ph, pl;
-        softmax_step<U>(sc, kb, see.from, qe, m, l, o, ph, pl);
-        add_values<U>(r, ph, pl, o);
+        softmax_step<U>(sc, unit, kb, see.from, qe, m, l, o, ph, pl);
+        add_values<U>(r, ph, pl, vheads[wv], o);
         if (more) issue_v<U>(vc, vs, r);
     }
     float *ow = sums + wv * 16 * HD;
+    if (j0 + c < nvec) {
 #pragma unroll
-    for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(ow + c * HD + 16 * b + 4 * g) = o[b];
-    if (g == 0) sm[wv][c] = m, sl[wv][c] = l;
+        for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(ow + c * HD + 16 * b + 4 * g) = o[b];
+        if (g == 0) sm[wv][c] = m, sl[wv][c] = l;
+    }
     __syncthreads();
-    const size_t base = C.base[si];
+    const size_t base = from_lane(bases, found.index);
     meet<HD, 4>(sums, sm, sl, 256, threadIdx.x, j0, nvec, G, kvh, heads, s.row0, out, part + base * HD, pml + 2 * base, n, ci);
 }
 
-// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, for segments of more than one: one workgroup of four waves
-// per (row, head), wave w adds chunks w, w + 4, ..., the waves' sums in wave order.
-template <int HD>
-__global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
-                                                               float *__restrict__ out, SegTable T, Cuts C, int heads) {
+// The same for hd 128 and 256, whose waves are few (hd 256: 2 per SIMD, for the registers of O and q): the blocks come to LDS by DMA,
+// kSlots of them for each wave, so that the loads of a whole block are in flight while another one is computed with, and no
+// registers are spent on them. A slot: K pieces of 16 bytes in the order that lanes read them, V pieces, headers (lanes 0 .. 31 bring
+// K's, row after row, the others V's). Page ids and addresses are wave-uniform and come by scalar loads: the only vector memory
+// operations of the loop are the DMA's, which the waits count.
+template <int U>
+struct Ring {
+    static constexpr int kSlots = U == 8 ? 2 : 3, kLoads = U + 1, kBytes = 1024 * kLoads;
+};
+// Where a block's slabs are. MODE: how many of the four slabs one look at the page table gives (4: pages of whole blocks, 2: of
+// pairs of slabs), 0: a contiguous cache.
+template <int MODE>
+struct Slab4 {
+    static constexpr int N = MODE == 0 ? 1 : 4 / MODE;
+    size_t block[N];  // first byte of the cache block
+    uint32_t slab[N];
+    uint32_t bad;  // a bit for each slab whose page is none
+};
+template <int MODE>
+__device__ __forceinline__ Slab4<MODE> look_up(const Map4 &M, int slot, int kvh, int kb, int last) {
+    Slab4<MODE> r;
+    r.bad = 0;
+    if constexpr (MODE == 0) {
+        r.block[0] = static_cast<size_t>(kvh) * M.bytes;
+        r.slab[0] = kb / kSlab;
+    } else {
+        const auto *pt = (const __attribute__((address_space(4))) int32_t *)(M.pt) + static_cast<size_t>(slot) * M.pps;
+#pragma unroll
+        for (int i = 0; i < Slab4<MODE>::N; ++i) {
+            // Slabs past the last key's: that one's page is read instead (their keys are masked).
+            const uint32_t slab = min(kb / kSlab + MODE * i, last & ~(MODE - 1));
+            const uint32_t p = static_cast<uint32_t>((static_cast<uint64_t>(slab) * M.mul) >> M.shift);
+            const int pg = pt[p];
+            const bool none = static_cast<uint32_t>(pg) >= static_cast<uint32_t>(M.pages);
+            r.bad |= none ? ((1u << MODE) - 1) << (MODE * i) : 0u;
+            r.block[i] = (static_cast<size_t>(none ? 0 : pg) * M.kv_heads + kvh) * M.bytes;
+            r.slab[i] = slab - p * M.spp;
+            // Opaque from here, or a lane's choice between two of them becomes one between addresses, in memory.
+            asm("" : "+s"(r.block[i]), "+s"(r.slab[i]));
+        }
+    }
+    return r;
+}
+// Slab i of the block, as a lane's own choice: (first byte of its block, slab in it).
+template <int MODE>
+__device__ __forceinline__ void choose(const Slab4<MODE> &s, int i, int last, size_t &block, uint32_t &slab) {
+    if constexpr (MODE == 0) {
+        block = s.block[0], slab = min(s.slab[0] + i, static_cast<uint32_t>(last));
+    } else if constexpr (MODE == 4) {
+        block = s.block[0], slab = s.slab[0] + i;
+    } else {
+        block = i & 2 ? s.block[1] : s.block[0], slab = (i & 2 ? s.slab[1] : s.slab[0]) + (i & 1);
+    }
+}
+// 64 lanes x 16 bytes from each lane's own address to LDS at (wave-uniform) dst, in lane order.
+__device__ __forceinline__ void dma16(const uint8_t *from, uint8_t *dst) {
+    const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(vq::lds_addr(dst))));
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at), "v"(dst) : "memory", "m0");
+}
+template <int U, int MODE>
+__device__ __forceinline__ void issue_dma(const uint8_t *kc, const uint8_t *vc, const Map4 &M, const Slab4<MODE> &at, int last, uint8_t *slot) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, piece = min(lane & 31, 4 * U - 1);
+    size_t block;
+    uint32_t slab;
+    choose<MODE>(at, c >> 2, last, block, slab);
+    const uint8_t *k = kc + block + static_cast<size_t>(slab) * (128 * U) + ((c & 3) * (16 * U) + g * (4 * U));
+    choose<MODE>(at, g, last, block, slab);
+    const uint8_t *v = vc + block + static_cast<size_t>(slab) * (128 * U) + c * 16;
+    choose<MODE>(at, piece / U, last, block, slab);
+    const uint8_t *h = (lane < 32 ? kc : vc) + block + static_cast<size_t>(M.spp) * (128 * U) + static_cast<size_t>(slab) * (16 * U) + piece % U * 16;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int i = 0; i < U / 4; ++i) dma16(k + half * (64 * U) + 16 * i, slot + 1024 * (half * (U / 4) + i));
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) dma16(v + 256 * i, slot + 1024 * (U / 2 + i));
+    dma16(h, slot + 1024 * U);
+}
+template <int U>
+__device__ __forceinline__ void read_k(const uint8_t *slot, Raw4<U> &r) {
+    const int lane = threadIdx.x & 63, c = lane & 15;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int i = 0; i < U / 4; ++i) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(slot + 1024 * (half * (U / 4) + i) + 16 * lane);
+            r.k[half][4 * i] = w.x, r.k[half][4 * i + 1] = w.y, r.k[half][4 * i + 2] = w.z, r.k[half][4 * i + 3] = w.w;
+        }
+        ld_words<U / 2>(slot + 1024 * U + (8 * (c >> 2) + 4 * half + (c & 3)) * (2 * U), r.kh[half]);
+    }
+}
+template <int U>
+__device__ __forceinline__ void read_v(const uint8_t *slot, Raw4<U> &r) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(slot + 1024 * (U / 2 + i) + 16 * lane);
+        r.v[4 * i] = w.x, r.v[4 * i + 1] = w.y, r.v[4 * i + 2] = w.z, r.v[4 * i + 3] = w.w;
+    }
+    r.vh = *reinterpret_cast<const uint4 *>(slot + 1024 * U + 512 + 16 * (g * U + min(c, U - 1)));
+}
+
+template <int U, int MODE>
+__global__ __launch_bounds__(256, 2) void attention4_stream_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
+                                                                   const uint8_t *__restrict__ vc, float *__restrict__ part,
+                                                                   float *__restrict__ pml, float *__restrict__ out, SegTable T, Map4 M,
+                                                                   Cuts C, int heads, int bidirectional, int window) {
+    constexpr int HD = 32 * U, SLOTS = Ring<U>::kSlots, BYTES = Ring<U>::kBytes, LOADS = Ring<U>::kLoads;
+    static_assert(SLOTS * BYTES >= 16 * HD * 4, "the waves' sums go where their slots were");
+    __shared__ __align__(16) uint8_t ring[4][SLOTS * BYTES];
+    __shared__ float sm[4][16], sl[4][16];
+    __shared__ __align__(16) uint32_t vheads[4][head_words<U>];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % M.kv_heads, list = blockIdx.x / M.kv_heads;
+    const int bases = C.base[lane];
+    const Found found = find_segment(T, C.first, C.total, list);
+    const Seg s = found.s;
+    const int ci = list - found.first, n = found.next - found.first;
+    const int G = heads / M.kv_heads, nvec = s.rows * G, j0 = blockIdx.y * 16;
+    if (j0 >= nvec) return;
+    const int k_lo = first_key(s, window) + ci * C.len, k_hi = min(k_lo + C.len, s.pos0 + s.rows), last = (k_hi - 1) / kSlab;
+    int kb = k_lo + 32 * wv;
+    uint8_t *const mine = ring[wv];
+    auto fetch = [&](int block, int slot) {
+        const Slab4<MODE> at = look_up<MODE>(M, s.slot, kvh, block, last);
+        issue_dma<U, MODE>(kc, vc, M, at, last, mine + slot * BYTES);
+        return at.bad;
+    };
+    uint32_t bad[SLOTS] = {};
+    if (kb < k_hi) bad[0] = fetch(kb, 0);
+    const int j = min(j0 + c, nvec - 1), t = j / G, h = kvh * G + j - t * G;  // vectors past the last repeat it; not written
+    const Sees see = sees(s, t, bidirectional, window);
+    const int qe = min(see.to, k_hi);
+    fh8 qh[U], ql[U];
+    const float unit = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
+    float m = -INFINITY, l = 0.0f;
+    fa4 o[2 * U];
+#pragma unroll
+    for (int b = 0; b < 2 * U; ++b) o[b] = fa4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 1; i < SLOTS; ++i)
+        if (kb + 128 * i < k_hi) bad[i] = fetch(kb + 128 * i, i);
+    while (kb < k_hi) {
+#pragma unroll
+        for (int slot = 0; slot < SLOTS; ++slot) {
+            if (kb >= k_hi) break;
+            // Landed: all but the loads of the blocks behind this one.
+            const int behind = min((k_hi - 1 - kb) / 128, SLOTS - 1);
+            if (behind == 0) vq::wait_vm<0>();
+            else if (behind == 1) vq::wait_vm<LOADS>();
+            else vq::wait_vm<2 * LOADS>();
+            Raw4<U> r;
+            uint8_t *const from = mine + slot * BYTES;
+            read_k<U>(from, r);
+            if (MODE != 0 && bad[slot] != 0 && (bad[slot] >> (c >> 2) & 1)) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int x = 0; x < U / 2; ++x) r.kh[half][x] = kNanHeader | kNanHeader << 16;
+            }
+            fa4 sc[2];
+            scores<U>(r, qh, ql, sc);
+            fh8 ph, pl;
+            softmax_step<U>(sc, unit, kb, see.from, qe, m, l, o, ph, pl);
+            read_v<U>(from, r);
+            add_values<U>(r, ph, pl, vheads[wv], o);
+            vq::wait_lgkm0();  // the slot has been read
+            if (kb + 128 * SLOTS < k_hi) bad[slot] = fetch(kb + 128 * SLOTS, slot);
+            kb += 128;
+        }
+    }
+    __syncthreads();  // every slot of every wave has been read
+    float *sums = reinterpret_cast<float *>(&ring[0][0]), *ow = sums + wv * 16 * HD;
+    if (j0 + c < nvec) {
+#pragma unroll
+        for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(ow + c * HD + 16 * b + 4 * g) = o[b];
+        if (g == 0) sm[wv][c] = m, sl[wv][c] = l;
+    }
+    __syncthreads();
+    const size_t base = from_lane(bases, found.index);
+    meet<HD, 4>(sums, sm, sl, 256, threadIdx.x, j0, nvec, G, kvh, heads, s.row0, out, part + base * HD, pml + 2 * base, n, ci);
+}
+
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, for segments of more than one: one workgroup of W waves per
+// (row, head); a wave takes every W-th chunk (lane = four dims), four of them in flight, the waves' sums meet in wave order. Many
+// chunks take more waves: it is latency that this kernel spends.
+template <int HD, int W>
+__global__ __launch_bounds__(64 * W) void attention4_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
+                                                                  float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads) {
     constexpr int Q = HD / 4;
-    __shared__ float smx[4], sl[4];
-    __shared__ float4 sacc[4][Q];
-    int t = blockIdx.x / heads, si = 0;
-    const int h = blockIdx.x - t * heads;
-    while (si + 1 < T.n && t >= T.s[si].rows) t -= T.s[si++].rows;
-    const Seg &s = T.s[si];
-    const int n = C.first[si + 1] - C.first[si];
-    if (n == 1) return;
-    const size_t at = static_cast<size_t>(C.base[si]) + (static_cast<size_t>(t) * heads + h) * n;
-    const float *ml = pml + 2 * at;
+    __shared__ float smx[W], sl[W];
+    __shared__ float4 sacc[W][Q];
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int row = blockIdx.x / heads, h = blockIdx.x - row * heads;
+    const int chunks = C.first[lane], bases = C.base[lane];
+    const Found found = find_segment(T, R.first, R.total, row);
+    const Seg s = found.s;
+    const int t = row - found.first, i = found.index;
+    const int n = (i + 1 < T.n ? from_lane(chunks, i + 1 < 64 ? i + 1 : 63) : C.total) - from_lane(chunks, i);
+    if (n == 1) return;
+    const size_t at = static_cast<size_t>(from_lane(bases, i)) + (static_cast<size_t>(t) * heads + h) * n;
+    const float *ml = pml + 2 * at;
     float mx = -INFINITY;
-    for (int c = tid; c < n; c += 256) mx = fmaxf(mx, ml[2 * c]);
+    for (int c = tid; c < n; c += 64 * W) mx = fmaxf(mx, ml[2 * c]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
     if (lane == 0) smx[wv] = mx;
     __syncthreads();
-    mx = fmaxf(fmaxf(smx[0], smx[1]), fmaxf(smx[2], smx[3]));
+    mx = smx[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) mx = fmaxf(mx, smx[w]);
     float4 acc{0.f, 0.f, 0.f, 0.f};
     float L = 0.0f;
     if (lane < Q) {
-        for (int c0 = wv; c0 < n; c0 += 16) {
+        for (int c0 = wv; c0 < n; c0 += 4 * W) {
             float4 p[4];
             float mc[4], lc[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int c = c0 + 4 * k < n ? c0 + 4 * k : c0;
+                const int c = c0 + W * k < n ? c0 + W * k : c0;
                 p[k] = *reinterpret_cast<const float4 *>(part + (at + c) * HD + 4 * lane);
                 mc[k] = ml[2 * c];
                 lc[k] = ml[2 * c + 1];
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                if (c0 + 4 * k >= n) break;
+                if (c0 + W * k >= n) break;
                 const float f = mc[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc[k] - mx);
                 L = fmaf(lc[k], f, L);
                 acc.x = fmaf(p[k].x, f, acc.x);
@@ -609,10 +870,16 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
     if (lane == 0) sl[wv] = L;
     __syncthreads();
     if (wv != 0 || lane >= Q) return;
-    const float lt = ((sl[0] + sl[1]) + sl[2]) + sl[3], inv = lt > 0.0f ? 1.0f / lt : 0.0f;
-    const float4 a = sacc[0][lane], b = sacc[1][lane], c = sacc[2][lane], d = sacc[3][lane];
-    const float4 r{(((a.x + b.x) + c.x) + d.x) * inv, (((a.y + b.y) + c.y) + d.y) * inv, (((a.z + b.z) + c.z) + d.z) * inv,
-                   (((a.w + b.w) + c.w) + d.w) * inv};
+    L = sl[0];
+    acc = sacc[0][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+        const float4 a = sacc[w][lane];
+        L += sl[w];
+        acc = float4{acc.x + a.x, acc.y + a.y, acc.z + a.z, acc.w + a.w};
+    }
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    const float4 r{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
     __builtin_memcpy(out + (static_cast<size_t>(s.row0 + t) * heads + h) * HD + 4 * lane, &r, 16);
 }
 
@@ -626,7 +893,7 @@ __device__ __forceinline__ int vt_at(int d, int octet) { return d * 32 + ((octet
 template <int U, bool PAGED, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void attention4_tiled_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
                                                                       const uint8_t *__restrict__ vc, float *__restrict__ out,
-                                                                      SegTable T, Map4 M, int heads, int bidirectional, int window) {
+                                                                      SegTable T, Starts R, Map4 M, int heads, int bidirectional, int window) {
     constexpr int HD = 32 * U, LDK = HD + 16, TH = 64 * NW, TILES = NW / 2;
     constexpr int KW = U % 4 == 0 ? 4 : U % 2 == 0 ? 2 : 1, W = U % 2 == 0 ? 4 : 2;  // words of a K unit, of a V unit
     constexpr int KUN = 64 * 4 * (U / KW), VUN = 8 * 16 * (2 * U / W);               // units of a step
@@ -639,14 +906,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attention4_tiled_kernel(const floa
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, c = lane & 15, g = lane >> 4, tile = wv >> 1, par = wv & 1;
     const int kvh = blockIdx.x % M.kv_heads, G = heads / M.kv_heads;
     // Workgroups take the kv heads in turn, the last rows, which see the most keys, first.
-    int tb = gridDim.x / M.kv_heads - 1 - blockIdx.x / M.kv_heads, si = 0;
-    while (si + 1 < T.n) {
-        const int nt = (T.s[si].rows * G + 16 * TILES - 1) / (16 * TILES);
-        if (tb < nt) break;
-        tb -= nt;
-        ++si;
-    }
-    const Seg &s = T.s[si];
+    const int group = R.total - 1 - blockIdx.x / M.kv_heads;
+    const Found found = find_segment(T, R.first, R.total, group);
+    const Seg s = found.s;
+    const int tb = group - found.first;
     const int nvec = s.rows * G, first = tb * 16 * TILES, j0 = first + 16 * tile;
     const bool on = j0 < nvec;
     const int j = min(j0 + c, nvec - 1), t = j / G, h = kvh * G + j - t * G;
@@ -656,7 +919,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attention4_tiled_kernel(const floa
     auto look = [&](int step) { return slab_at<U, PAGED>(M, s.slot, kvh, min(max((k0 + 64 * step) / kSlab + (tid & 7), s0), s1)); };
     if (tid < 16) slabs[tid >> 3][tid & 7] = look(tid >> 3);
     fh8 qh[U], ql[U];
-    const float sinv = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
+    const float unit = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
     __syncthreads();
     uint32_t rk[KN][KW], rkh[KN][KW == 4 ? 2 : 1], rv[VN][W];
     uint4 rvh[VN][W / 2];
@@ -694,8 +957,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attention4_tiled_kernel(const floa
             _Float16 *kd = buf + (key >> 5) * (KB + VB) + row * LDK + 32 * u0 + 8 * g4;
 #pragma unroll
             for (int k = 0; k < KW; ++k) {
-                const Heads2 hd2 = heads2(rkh[i][k / 2]);
-                *reinterpret_cast<fh8 *>(kd + 32 * k) = k % 2 == 0 ? decode8_one<false>(rk[i][k], hd2) : decode8_one<true>(rk[i][k], hd2);
+                const uint32_t h2 = rkh[i][k / 2];
+                *reinterpret_cast<fh8 *>(kd + 32 * k) = k % 2 == 0 ? decode8_one<false>(rk[i][k], h2) : decode8_one<true>(rk[i][k], h2);
             }
         }
 #pragma unroll
@@ -706,8 +969,9 @@ __global__ __launch_bounds__(64 * NW, 2) void attention4_tiled_kernel(const floa
 #pragma unroll
             for (int k = 0; k < W; ++k) {
                 const uint4 x = rvh[i][k / 2];
-                const Heads2 hs[4] = {heads2(x.x), heads2(x.y), heads2(x.z), heads2(x.w)};
-                *reinterpret_cast<fh8 *>(vd + vt_at(16 * ((rest >> 4) * W + k) + (rest & 15), slab & 3)) = decode8(rv[i][k], hs);
+                const fh2 ds[4] = {scales2(x.x), scales2(x.y), scales2(x.z), scales2(x.w)};
+                const fh2 zs[4] = {zeros2(x.x, false), zeros2(x.y, true), zeros2(x.z, false), zeros2(x.w, true)};
+                *reinterpret_cast<fh8 *>(vd + vt_at(16 * ((rest >> 4) * W + k) + (rest & 15), slab & 3)) = decode8(rv[i][k], ds, zs);
             }
         }
     };
@@ -736,10 +1000,10 @@ __global__ __launch_bounds__(64 * NW, 2) void attention4_tiled_kernel(const floa
                     a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[u], a0, 0, 0, 0);
                     a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[u], a1, 0, 0, 0);
                 }
-                sc[hh] = (a0 + a1) * sinv;
+                sc[hh] = a0 + a1;
             }
             fh8 ph, pl;
-            softmax_step<U>(sc, kb, see.from, see.to, m, l, o, ph, pl);
+            softmax_step<U>(sc, unit, kb, see.from, see.to, m, l, o, ph, pl);
 #pragma unroll
             for (int b = 0; b < 2 * U; ++b) {
                 const fh8 v8 = *reinterpret_cast<const fh8 *>(vt + vt_at(16 * b + c, g));
@@ -799,32 +1063,50 @@ int check_cache(const void *kc, const void *vc, int kv_heads, int hd, const SegT
     return VQ_OK;
 }
 
+Starts starts_of(const SegTable &T, int (*units)(const Seg &, int), int arg) {
+    Starts R;
+    R.total = 0;
+    for (int i = 0; i < VQ_MAX_SEGMENTS; ++i) {
+        R.first[i] = R.total;
+        if (i < T.n) R.total += units(T.s[i], arg);
+    }
+    return R;
+}
+int slabs_of(const Seg &s, int) { return (s.pos0 + s.rows - 1) / kSlab - s.pos0 / kSlab + 1; }
+int rows_of(const Seg &s, int) { return s.rows; }
+
 int launch_append4(const float *k, const float *v, void *kc, void *vc, const SegTable &T, const Map4 &M, int hd, hipStream_t s) {
     if (!k || !v) return VQ_ERR_ARG;
-    unsigned slabs = 0;
-    for (int i = 0; i < T.n; ++i) slabs += (T.s[i].pos0 + T.s[i].rows - 1) / kSlab - T.s[i].pos0 / kSlab + 1;
-    const dim3 grid(slabs, M.kv_heads);
+    const Starts R = starts_of(T, slabs_of, 0);
+    const dim3 grid(R.total, M.kv_heads);
     const int threads = (hd + 63) / 64 * 64;
     auto *kb = static_cast<uint8_t *>(kc), *vb = static_cast<uint8_t *>(vc);
-    if (M.pt) kv4_append_kernel<true><<<grid, threads, 0, s>>>(k, v, kb, vb, T, M, hd);
-    else kv4_append_kernel<false><<<grid, threads, 0, s>>>(k, v, kb, vb, T, M, hd);
+    if (M.pt) kv4_append_kernel<true><<<grid, threads, 0, s>>>(k, v, kb, vb, T, R, M, hd);
+    else kv4_append_kernel<false><<<grid, threads, 0, s>>>(k, v, kb, vb, T, R, M, hd);
     return status_of(hipGetLastError());
 }
 
 int launch_read4(const void *kc, const void *vc, float *k, float *v, const SegTable &T, const Map4 &M, int hd, hipStream_t s) {
     if (!k || !v) return VQ_ERR_ARG;
-    const dim3 grid(T.total, M.kv_heads);
+    const Starts R = starts_of(T, slabs_of, 0);
+    const dim3 grid(R.total, M.kv_heads);
     const int threads = (hd + 63) / 64 * 64;
     auto *kb = static_cast<const uint8_t *>(kc), *vb = static_cast<const uint8_t *>(vc);
-    if (M.pt) kv4_read_kernel<true><<<grid, threads, 0, s>>>(kb, vb, k, v, T, M, hd);
-    else kv4_read_kernel<false><<<grid, threads, 0, s>>>(kb, vb, k, v, T, M, hd);
+    if (M.pt) kv4_read_kernel<true><<<grid, threads, 0, s>>>(kb, vb, k, v, T, R, M, hd);
+    else kv4_read_kernel<false><<<grid, threads, 0, s>>>(kb, vb, k, v, T, R, M, hd);
     return status_of(hipGetLastError());
 }
 
 // Chunks for about a round or a few of the 512 workgroups that run at once (two per CU). `rounds` full rounds need chunks of at
 // least some length; among 1 to 4 rounds the least of rounds x (length + what a chunk costs besides its keys, in keys).
+int chunks_of(const SegTable &T, int i, long long len, int window) {
+    return static_cast<int>((T.s[i].pos0 + T.s[i].rows - first_key(T.s[i], window) + len - 1) / len);
+}
 Cuts make_cuts(const SegTable &T, int heads, int kv_heads, int window) {
-    constexpr int kSlots = 512, kFixed = 160;
+    #ifndef KFIX
+#define KFIX 160
+#endif
+    constexpr int kSlots = 512, kFixed = KFIX;
     int groups = 1;
     long long keys = 0;
     for (int i = 0; i < T.n; ++i) {
@@ -833,7 +1115,7 @@ Cuts make_cuts(const SegTable &T, int heads, int kv_heads, int window) {
     }
     auto count = [&](long long len) {
         long long n = 0;
-        for (int i = 0; i < T.n; ++i) n += (T.s[i].pos0 + T.s[i].rows - first_key(T.s[i], window) + len - 1) / len;
+        for (int i = 0; i < T.n; ++i) n += chunks_of(T, i, len, window);
         return n * kv_heads * groups;
     };
     long long best = 0, cost = 0;
@@ -846,30 +1128,31 @@ Cuts make_cuts(const SegTable &T, int heads, int kv_heads, int window) {
     }
     Cuts C;
     C.len = static_cast<int>(best);
-    C.total = 0;
+    C.total = C.most = 0;
     int base = 0;
-    for (int i = 0; i < T.n; ++i) {
-        const int n = (T.s[i].pos0 + T.s[i].rows - first_key(T.s[i], window) + C.len - 1) / C.len;
+    for (int i = 0; i < VQ_MAX_SEGMENTS; ++i) {
         C.first[i] = C.total;
         C.base[i] = base;
-        C.total += n;
+        if (i >= T.n) continue;
+        const int n = chunks_of(T, i, C.len, window);
         if (n > 1) base += n * T.s[i].rows * heads;
+        C.total += n;
+        C.most = max(C.most, n);
     }
-    for (int i = T.n; i <= VQ_MAX_SEGMENTS; ++i) C.first[i] = C.total;
     return C;
 }
 // Partial results of the pass: vectors x chunks where a segment has more than one.
-size_t parts_of(const SegTable &T, const Cuts &C, int heads) {
+size_t parts_of(const SegTable &T, const Cuts &C, int heads, int window) {
     size_t n = 0;
     for (int i = 0; i < T.n; ++i) {
-        const size_t k = C.first[i + 1] - C.first[i];
+        const size_t k = chunks_of(T, i, C.len, window);
         if (k > 1) n += k * T.s[i].rows * heads;
     }
     return n;
 }
 size_t attention4_ws_bytes(const SegTable &T, int heads, int kv_heads, int hd, int window) {
     if (max_seg_rows(T) > VQ_ATTN_ROW_MAX) return 0;
-    const size_t n = parts_of(T, make_cuts(T, heads, kv_heads, window), heads);
+    const size_t n = parts_of(T, make_cuts(T, heads, kv_heads, window), heads, window);
     return n * (hd + 2) * 4 + 16;
 }
 
@@ -897,26 +1180,38 @@ int launch_attention4(const float *q, const void *kc, const void *vc, float *out
         if ((reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < attention4_ws_bytes(T, heads, M.kv_heads, hd, window))
             return VQ_ERR_WORKSPACE;
         const Cuts C = make_cuts(T, heads, M.kv_heads, window);
-        const size_t parts = parts_of(T, C, heads);
+        const Starts R = starts_of(T, rows_of, 0);
+        const size_t parts = parts_of(T, C, heads, window);
         float *part = static_cast<float *>(ws), *pml = part + parts * hd;
         const dim3 grid(C.total * M.kv_heads, (max_seg_rows(T) * G + 15) / 16);
         for_hd(hd, [&](auto u) {
             constexpr int U = decltype(u)::value;
-            if (M.pt) attention4_split_kernel<U, true><<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window);
-            else attention4_split_kernel<U, false><<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window);
-            if (parts) attention4_merge_kernel<32 * U><<<T.total * heads, 256, 0, s>>>(part, pml, out, T, C, heads);
+            auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window); };
+            if constexpr (U % 4 == 0) {
+                if (!M.pt) return go(attention4_stream_kernel<U, 0>);
+                if (M.spp % 4 == 0) return go(attention4_stream_kernel<U, 4>);
+                if (M.spp % 2 == 0) return go(attention4_stream_kernel<U, 2>);
+            }
+            if (M.pt) go(attention4_split_kernel<U, true>);
+            else if constexpr (U % 4 != 0) go(attention4_split_kernel<U, false>);
+        });
+        for_hd(hd, [&](auto u) {
+            constexpr int U = decltype(u)::value;
+            if (C.most > 16) attention4_merge_kernel<32 * U, 16><<<T.total * heads, 1024, 0, s>>>(part, pml, out, T, C, R, heads);
+            else if (parts) attention4_merge_kernel<32 * U, 4><<<T.total * heads, 256, 0, s>>>(part, pml, out, T, C, R, heads);
         });
         return status_of(hipGetLastError());
     }
     constexpr int NW = 8, PER = 16 * (NW / 2);
-    long long tiles = 0;
-    for (int i = 0; i < T.n; ++i) tiles += (static_cast<long long>(T.s[i].rows) * G + PER - 1) / PER;
-    if (tiles * M.kv_heads > INT32_MAX) return VQ_ERR_SHAPE;
-    const dim3 grid(static_cast<unsigned>(tiles * M.kv_heads));
+    long long vectors = 0;
+    for (int i = 0; i < T.n; ++i) vectors += static_cast<long long>(T.s[i].rows) * G + PER;
+    if (vectors / PER * M.kv_heads > INT32_MAX) return VQ_ERR_SHAPE;
+    const Starts R = starts_of(T, [](const Seg &x, int g) { return static_cast<int>((static_cast<long long>(x.rows) * g + PER - 1) / PER); }, G);
+    const dim3 grid(static_cast<unsigned>(R.total) * M.kv_heads);
     for_hd(hd, [&](auto u) {
         constexpr int U = decltype(u)::value;
-        if (M.pt) attention4_tiled_kernel<U, true, NW><<<grid, 64 * NW, 0, s>>>(q, kb, vb, out, T, M, heads, bidirectional, window);
-        else attention4_tiled_kernel<U, false, NW><<<grid, 64 * NW, 0, s>>>(q, kb, vb, out, T, M, heads, bidirectional, window);
+        if (M.pt) attention4_tiled_kernel<U, true, NW><<<grid, 64 * NW, 0, s>>>(q, kb, vb, out, T, R, M, heads, bidirectional, window);
+        else attention4_tiled_kernel<U, false, NW><<<grid, 64 * NW, 0, s>>>(q, kb, vb, out, T, R, M, heads, bidirectional, window);
     });
     return status_of(hipGetLastError());
 }
