@@ -689,13 +689,22 @@ __device__ __forceinline__ void dma16(const uint8_t *from, uint8_t *dst) {
     const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(vq::lds_addr(dst))));
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at), "v"(dst) : "memory", "m0");
 }
+// Operand row c's pieces (eight of 16 bytes, two rows to the 64 banks) change places by this.
+__device__ __forceinline__ int k_swizzle(int c) { return c >> 1 & 7; }
 template <int U, int MODE>
 __device__ __forceinline__ void issue_dma(const uint8_t *kc, const uint8_t *vc, const Map4 &M, const Slab4<MODE> &at, int last, uint8_t *slot) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, piece = min(lane & 31, 4 * U - 1);
     size_t block;
     uint32_t slab;
-    choose<MODE>(at, c >> 2, last, block, slab);
-    const uint8_t *k = kc + block + static_cast<size_t>(slab) * (128 * U) + ((c & 3) * (16 * U) + g * (4 * U));
+    // K, hd 256: a load brings eight rows of 128 bytes whole, operand rows 8 x + r (x: the load's half of them), pieces swizzled so that
+    // the operand's reads spread over the banks. hd 128: a load brings the half's 16 rows of 64 bytes in operand order.
+    const int r = U == 8 ? lane >> 3 : c, s = U == 8 ? lane & 7 : g;
+    const uint8_t *k[2];
+#pragma unroll
+    for (int x = 0; x < U / 4; ++x) {
+        choose<MODE>(at, U == 8 ? 2 * x + (r >> 2) : r >> 2, last, block, slab);
+        k[x] = kc + block + static_cast<size_t>(slab) * (128 * U) + ((r & 3) * (16 * U) + (U == 8 ? s ^ k_swizzle(8 * x + r) : s) * 16);
+    }
     choose<MODE>(at, g, last, block, slab);
     const uint8_t *v = vc + block + static_cast<size_t>(slab) * (128 * U) + c * 16;
     choose<MODE>(at, piece / U, last, block, slab);
@@ -703,19 +712,20 @@ __device__ __forceinline__ void issue_dma(const uint8_t *kc, const uint8_t *vc, 
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int i = 0; i < U / 4; ++i) dma16(k + half * (64 * U) + 16 * i, slot + 1024 * (half * (U / 4) + i));
+        for (int x = 0; x < U / 4; ++x) dma16(k[x] + half * (64 * U), slot + 1024 * (half * (U / 4) + x));
 #pragma unroll
     for (int i = 0; i < U / 2; ++i) dma16(v + 256 * i, slot + 1024 * (U / 2 + i));
     dma16(h, slot + 1024 * U);
 }
 template <int U>
 __device__ __forceinline__ void read_k(const uint8_t *slot, Raw4<U> &r) {
-    const int lane = threadIdx.x & 63, c = lane & 15;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int i = 0; i < U / 4; ++i) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(slot + 1024 * (half * (U / 4) + i) + 16 * lane);
+            const int at = U == 8 ? 128 * c + 16 * ((2 * g + i) ^ k_swizzle(c)) : 16 * lane;
+            const uint4 w = *reinterpret_cast<const uint4 *>(slot + 256 * U * half + at);
             r.k[half][4 * i] = w.x, r.k[half][4 * i + 1] = w.y, r.k[half][4 * i + 2] = w.z, r.k[half][4 * i + 3] = w.w;
         }
         ld_words<U / 2>(slot + 1024 * U + (8 * (c >> 2) + 4 * half + (c & 3)) * (2 * U), r.kh[half]);
@@ -813,17 +823,18 @@ __global__ __launch_bounds__(256, 2) void attention4_stream_kernel(const float *
     meet<HD, 4>(sums, sm, sl, 256, threadIdx.x, j0, nvec, G, kvh, heads, s.row0, out, part + base * HD, pml + 2 * base, n, ci);
 }
 
-// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, for segments of more than one: one workgroup of W waves per
-// (row, head); a wave takes every W-th chunk (lane = four dims), four of them in flight, the waves' sums meet in wave order. Many
-// chunks take more waves: it is latency that this kernel spends.
-template <int HD, int W>
-__global__ __launch_bounds__(64 * W) void attention4_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
-                                                                  float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads) {
-    constexpr int Q = HD / 4;
-    __shared__ float smx[W], sl[W];
-    __shared__ float4 sacc[W][Q];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int row = blockIdx.x / heads, h = blockIdx.x - row * heads;
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, for segments of more than one. It is latency that this
+// kernel spends, so a workgroup takes 64 dims of a (row, head) (32 where hd is no multiple of 64), a thread four dims of every 16th
+// (32nd) chunk, four of them in flight, under a running maximum; the 16 (32) sums meet in order. 24 rows of 128 chunks, hd 256: 4 us;
+// one workgroup of four waves for a row took 11.
+template <int HD>
+__global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
+                                                               float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads) {
+    constexpr int Q = HD % 64 == 0 ? 16 : 8, GROUPS = 256 / Q;
+    __shared__ float sm[GROUPS], sl[GROUPS];
+    __shared__ float4 sacc[GROUPS][Q];
+    const int tid = threadIdx.x, lane = tid & 63, grp = tid / Q, quad = tid - grp * Q;
+    const int row = blockIdx.x / heads, h = blockIdx.x - row * heads, d = 4 * (Q * blockIdx.y + quad);
     const int chunks = C.first[lane], bases = C.base[lane];
     const Found found = find_segment(T, R.first, R.total, row);
     const Seg s = found.s;
@@ -832,55 +843,56 @@ __global__ __launch_bounds__(64 * W) void attention4_merge_kernel(const float *_
     if (n == 1) return;
     const size_t at = static_cast<size_t>(from_lane(bases, i)) + (static_cast<size_t>(t) * heads + h) * n;
     const float *ml = pml + 2 * at;
-    float mx = -INFINITY;
-    for (int c = tid; c < n; c += 64 * W) mx = fmaxf(mx, ml[2 * c]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-    if (lane == 0) smx[wv] = mx;
-    __syncthreads();
-    mx = smx[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) mx = fmaxf(mx, smx[w]);
+    float m = -INFINITY, L = 0.0f;
     float4 acc{0.f, 0.f, 0.f, 0.f};
-    float L = 0.0f;
-    if (lane < Q) {
-        for (int c0 = wv; c0 < n; c0 += 4 * W) {
-            float4 p[4];
-            float mc[4], lc[4];
+    auto scale = [](float x, float to) { return x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - to); };
+    for (int c0 = grp; c0 < n; c0 += 4 * GROUPS) {
+        float4 p[4];
+        float mc[4], lc[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int c = c0 + W * k < n ? c0 + W * k : c0;
-                p[k] = *reinterpret_cast<const float4 *>(part + (at + c) * HD + 4 * lane);
-                mc[k] = ml[2 * c];
-                lc[k] = ml[2 * c + 1];
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (c0 + W * k >= n) break;
-                const float f = mc[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mc[k] - mx);
-                L = fmaf(lc[k], f, L);
-                acc.x = fmaf(p[k].x, f, acc.x);
-                acc.y = fmaf(p[k].y, f, acc.y);
-                acc.z = fmaf(p[k].z, f, acc.z);
-                acc.w = fmaf(p[k].w, f, acc.w);
-            }
+        for (int k = 0; k < 4; ++k) {
+            const int c = c0 + GROUPS * k < n ? c0 + GROUPS * k : c0;
+            p[k] = *reinterpret_cast<const float4 *>(part + (at + c) * HD + d);
+            mc[k] = c0 + GROUPS * k < n ? ml[2 * c] : -INFINITY;
+            lc[k] = ml[2 * c + 1];
         }
-        sacc[wv][lane] = acc;
-    }
-    if (lane == 0) sl[wv] = L;
-    __syncthreads();
-    if (wv != 0 || lane >= Q) return;
-    L = sl[0];
-    acc = sacc[0][lane];
+        const float mn = fmaxf(fmaxf(m, fmaxf(mc[0], mc[1])), fmaxf(mc[2], mc[3])), f0 = scale(m, mn);
+        m = mn;
+        L *= f0;
+        acc = float4{acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0};
 #pragma unroll
-    for (int w = 1; w < W; ++w) {
-        const float4 a = sacc[w][lane];
-        L += sl[w];
-        acc = float4{acc.x + a.x, acc.y + a.y, acc.z + a.z, acc.w + a.w};
+        for (int k = 0; k < 4; ++k) {
+            if (c0 + GROUPS * k >= n) break;
+            const float f = scale(mc[k], mn);
+            L = fmaf(lc[k], f, L);
+            acc.x = fmaf(p[k].x, f, acc.x);
+            acc.y = fmaf(p[k].y, f, acc.y);
+            acc.z = fmaf(p[k].z, f, acc.z);
+            acc.w = fmaf(p[k].w, f, acc.w);
+        }
+    }
+    sacc[grp][quad] = acc;
+    if (quad == 0) sm[grp] = m, sl[grp] = L;
+    __syncthreads();
+    if (tid >= Q) return;
+    m = sm[0];
+#pragma unroll
+    for (int w = 1; w < GROUPS; ++w) m = fmaxf(m, sm[w]);
+    L = 0.0f;
+    acc = float4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < GROUPS; ++w) {
+        const float4 a = sacc[w][quad];
+        const float f = scale(sm[w], m);
+        L = fmaf(sl[w], f, L);
+        acc.x = fmaf(a.x, f, acc.x);
+        acc.y = fmaf(a.y, f, acc.y);
+        acc.z = fmaf(a.z, f, acc.z);
+        acc.w = fmaf(a.w, f, acc.w);
     }
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
     const float4 r{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-    __builtin_memcpy(out + (static_cast<size_t>(s.row0 + t) * heads + h) * HD + 4 * lane, &r, 16);
+    __builtin_memcpy(out + (static_cast<size_t>(s.row0 + t) * heads + h) * HD + d, &r, 16);
 }
 
 // Prompt passes, and any pass without a workspace: a workgroup of NW waves takes NW / 2 tiles of 16 query vectors of a kv head, two
@@ -1197,8 +1209,7 @@ int launch_attention4(const float *q, const void *kc, const void *vc, float *out
         });
         for_hd(hd, [&](auto u) {
             constexpr int U = decltype(u)::value;
-            if (C.most > 16) attention4_merge_kernel<32 * U, 16><<<T.total * heads, 1024, 0, s>>>(part, pml, out, T, C, R, heads);
-            else if (parts) attention4_merge_kernel<32 * U, 4><<<T.total * heads, 256, 0, s>>>(part, pml, out, T, C, R, heads);
+            if (parts) attention4_merge_kernel<32 * U><<<dim3(T.total * heads, U % 2 == 0 ? U / 2 : U), 256, 0, s>>>(part, pml, out, T, C, R, heads);
         });
         return status_of(hipGetLastError());
     }

@@ -79,8 +79,8 @@ class _Buffer:
     # data was handed out (buffer_tensor): its storage may be exchanged or resized, so every use asks for the address
     # (0.1 us), and for the size where that has changed. A storage that is this entry's alone keeps both.
     lent: bool = False
-    # A 4-bit KV cache (alloc_kv4): its blocks, positions of a block and head dims. elem is 1 then: sizes are in bytes.
-    kv4: tuple[int, int, int] | None = None
+    # A 4-bit KV cache (alloc_kv4): its blocks, positions of a block, head dims and bytes. elem is 1 then: sizes are in bytes.
+    kv4: tuple[int, int, int, int] | None = None
 
     def __post_init__(self) -> None:
         self.address = self.data.data_ptr
@@ -438,7 +438,7 @@ class Runtime:
         if not n:
             raise ValueError(f"4-bit cache {name}: invalid shape ({blocks} blocks, {positions} positions, {hd} dims)")
         data = torch.zeros(n, dtype=torch.uint8, device=self.device)
-        self.buffers[name] = _Buffer(data, 1, kv4=(int(blocks), -(-int(positions) // 8) * 8, int(hd)))
+        self.buffers[name] = _Buffer(data, 1, kv4=(int(blocks), -(-int(positions) // 8) * 8, int(hd), n))
 
     def zero(self, name: str) -> None:
         buf = self._any_buffer(name)
@@ -768,7 +768,7 @@ class Runtime:
         sizes = []
         for name in names:
             b = self._any_buffer(name)
-            n = self._lib.vq_kv4_bytes(*b.kv4) if b.kv4 else b.n * b.elem
+            n = b.kv4[3] if b.kv4 else b.n * b.elem
             if n % pages:
                 raise ValueError(f"device buffer {name} is not {pages} pages of one size")
             sizes.append(n // pages)
@@ -890,12 +890,13 @@ class Runtime:
         both hold."""
         if not (kcb.kv4 and vcb.kv4):
             raise TypeError("K and V caches differ in precision")
-        blocks = min(kcb.kv4[0], vcb.kv4[0])
+        full = -(-positions // 8) * 8
         for name, b in ((kc, kcb), (vc, vcb)):
-            if b.kv4[1] != -(-positions // 8) * 8 or b.kv4[2] != hd:
+            if b.kv4[1] != full or b.kv4[2] != hd:
                 raise ValueError(f"4-bit cache {name} has blocks of {b.kv4[1]} positions of {b.kv4[2]} dims, not {positions} of {hd}")
-            if b.lent and b.n < self._lib.vq_kv4_bytes(*b.kv4):
-                raise ValueError(f"device buffer {name} has {b.n} bytes, need {self._lib.vq_kv4_bytes(*b.kv4)}")
+            if b.n < b.kv4[3]:
+                raise ValueError(f"device buffer {name} has {b.n} bytes, need {b.kv4[3]}")
+        blocks = min(kcb.kv4[0], vcb.kv4[0])
         if kv_heads < 1 or blocks < kv_heads:
             raise ValueError(f"4-bit caches {kc}, {vc} hold {blocks} blocks, need {kv_heads}")
         return blocks // kv_heads
