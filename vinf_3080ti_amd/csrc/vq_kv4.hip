@@ -421,10 +421,11 @@ __device__ __forceinline__ void softmax_step(const fa4 (&s)[2], float unit, int 
     }
 }
 
-// How a pass's contexts are cut: chunks of `len` keys (a multiple of 128) from each segment's first key rounded down to 32, all
-// segments' chunks in one list; segment i's begin at first[i], its partial results at base[i].
+// How a pass is cut: each segment's query vectors in groups of 16 NT, its keys in chunks of `len` (a multiple of 128) from its first
+// key rounded down to 32; segment i's groups x chunks begin at first[i] of one list, its partial results at base[i] (where it has
+// more than one chunk).
 struct Cuts {
-    int len, total, most;  // most: chunks of a segment
+    int len, total;
     int first[VQ_MAX_SEGMENTS], base[VQ_MAX_SEGMENTS];
 };
 // First key that any row of a segment sees, rounded down to a block.
@@ -441,39 +442,48 @@ __device__ __forceinline__ Sees sees(const Seg &s, int t, int bidirectional, int
     return Sees{window > 0 && end > window ? end - window : 0, bidirectional ? s.pos0 + s.rows : end};
 }
 
-// A workgroup's results for up to 16 query vectors: W waves' sums (each wave's [16][HD] in `sums`, maxima and totals in sm, sl) meet
-// in wave order; written out, or as the chunk's unnormalised part where the context is cut.
-template <int HD, int W>
-__device__ __forceinline__ void meet(const float *sums, const float (&sm)[W][16], const float (&sl)[W][16], int threads, int tid, int j0,
-                                     int nvec, int G, int kvh, int heads, int row0, float *out, float *part, float *pml, int n, int ci) {
-    for (int e = tid; e < 16 * (HD / 4); e += threads) {
-        const int c = e / (HD / 4), d4 = 4 * (e - c * (HD / 4)), j = j0 + c;
-        if (j >= nvec) continue;
+// Where a group's results go: the output where the segment has one chunk, else the chunk's unnormalised part.
+struct Dest {
+    float *out, *part, *pml;
+    size_t base;
+    int heads, G, kvh, row0, nvec, n, ci;
+    template <int HD>
+    __device__ __forceinline__ void put(int j, int d, const float4 &acc, float m, float l) const {
         const int t = j / G, h = kvh * G + j - t * G;
-        float mx = sm[0][c];
-#pragma unroll
-        for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm[w][c]);
+        if (n == 1) {
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const float4 r{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+            __builtin_memcpy(out + (static_cast<size_t>(row0 + t) * heads + h) * HD + d, &r, 16);
+        } else {
+            const size_t at = base + (static_cast<size_t>(t) * heads + h) * n + ci;
+            *reinterpret_cast<float4 *>(part + at * HD + d) = acc;
+            if (d == 0) pml[2 * at] = m, pml[2 * at + 1] = l;
+        }
+    }
+};
+// A sum's share against maximum m where it was kept against `own`.
+__device__ __forceinline__ float share(float own, float m) { return own == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(own - m); }
+
+// Four waves' sums of 16 vectors (each wave's [16][HD], maxima and totals) meet in wave order.
+template <int HD>
+__device__ __forceinline__ void meet4(const float *sums, const float (&sm)[4][2][16], const float (&sl)[4][2][16], int j0, const Dest &to) {
+    for (int e = threadIdx.x; e < 16 * (HD / 4); e += 256) {
+        const int c = e / (HD / 4), d4 = 4 * (e - c * (HD / 4));
+        if (j0 + c >= to.nvec) continue;
+        const float mx = fmaxf(fmaxf(sm[0][0][c], sm[1][0][c]), fmaxf(sm[2][0][c], sm[3][0][c]));
         float L = 0.0f;
         float4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = sm[w][c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][c] - mx);
-            L = fmaf(sl[w][c], f, L);
+        for (int w = 0; w < 4; ++w) {
+            const float f = share(sm[w][0][c], mx);
+            L = fmaf(sl[w][0][c], f, L);
             const float4 p = *reinterpret_cast<const float4 *>(sums + (w * 16 + c) * HD + d4);
             acc.x = fmaf(p.x, f, acc.x);
             acc.y = fmaf(p.y, f, acc.y);
             acc.z = fmaf(p.z, f, acc.z);
             acc.w = fmaf(p.w, f, acc.w);
         }
-        if (n == 1) {
-            const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-            const float4 r{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-            __builtin_memcpy(out + (static_cast<size_t>(row0 + t) * heads + h) * HD + d4, &r, 16);
-        } else {
-            const size_t at = (static_cast<size_t>(t) * heads + h) * n + ci;
-            *reinterpret_cast<float4 *>(part + at * HD + d4) = acc;
-            if (d4 == 0) pml[2 * at] = mx, pml[2 * at + 1] = L;
-        }
+        to.put<HD>(j0 + c, d4, acc, mx, L);
     }
 }
 
@@ -485,6 +495,13 @@ struct Raw4 {
     uint4 vh;
 };
 template <int U>
+__device__ __forceinline__ void no_page(Raw4<U> &r) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < (U + 1) / 2; ++i) r.kh[h][i] = kNanHeader | kNanHeader << 16;
+}
+template <int U>
 __device__ __forceinline__ void issue_k(const uint8_t *__restrict__ kc, const SlabAt &at, Raw4<U> &r) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -493,12 +510,7 @@ __device__ __forceinline__ void issue_k(const uint8_t *__restrict__ kc, const Sl
         ld_words<U>(kc + at.words + row * (16 * U) + g * (4 * U), r.k[h]);
         ld_heads<U>(kc + at.heads + row * (2 * U), r.kh[h]);
     }
-    if (at.bad) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < (U + 1) / 2; ++i) r.kh[h][i] = kNanHeader | kNanHeader << 16;
-    }
+    if (at.bad) no_page<U>(r);
 }
 template <int U>
 __device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, const SlabAt &at, Raw4<U> &r) {
@@ -514,27 +526,194 @@ __device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, const Sl
     r.vh = *reinterpret_cast<const uint4 *>(vc + at.heads + 16 * min(c, U - 1));
 }
 
-template <int U>
-__device__ __forceinline__ void scores(const Raw4<U> &r, const fh8 (&qh)[U], const fh8 (&ql)[U], fa4 (&s)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        fa4 a0{0.f, 0.f, 0.f, 0.f}, a1{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const fh8 a = u % 2 == 0 ? decode8_one<false>(r.k[h][u], r.kh[h][u / 2]) : decode8_one<true>(r.k[h][u], r.kh[h][u / 2]);
-            a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[u], a0, 0, 0, 0);
-            a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[u], a1, 0, 0, 0);
+// ---- blocks by DMA ----
+
+// For hd 128 and 256, whose waves are few (hd 256: 2 per SIMD, for the registers of O and q): the blocks come to LDS by DMA, kSlots of
+// them for each wave, so that the loads of one are in flight while another is computed with, and no registers are spent on them. A
+// slot is K's words in the order of the loads, V's words, and 512 bytes each of K's and of V's headers, slab after slab. Page ids and
+// addresses are wave-uniform and come by scalar loads: the only vector memory operations of the loop are the DMA's, which the waits
+// count.
+template <int U, int NT>
+struct Ring {
+    static constexpr int kSlots = U == 8 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2);
+    static constexpr int kWords = 512 * U, kBytes = 2 * kWords + 1024;
+    static constexpr int kLoads = kSlots == 1 ? U / 2 + 1 : U + 1;  // of half a slot that is filled by halves, or of a slot
+};
+// Where a block's slabs are. MODE: how many of the four slabs one look at the page table gives (4: pages of whole blocks, 2: of
+// pairs of slabs), 0: a contiguous cache.
+struct Slab4 {
+    size_t block0, block1;  // first byte of the cache block of the first slab and (MODE 2) of the third
+    uint32_t slab0, slab1;
+    uint32_t bad;  // a bit for each slab whose page is none
+};
+// Slabs past the last key's: that one's page is read instead (their keys are masked).
+template <int MODE>
+__device__ __forceinline__ uint32_t look_up_page(const Map4 &M, int slot, int kvh, int slab, int last, size_t &block, uint32_t &at) {
+    const auto *pt = (const __attribute__((address_space(4))) int32_t *)(M.pt) + static_cast<size_t>(slot) * M.pps;
+    const uint32_t want = min(slab, last & ~(MODE - 1)), p = static_cast<uint32_t>((static_cast<uint64_t>(want) * M.mul) >> M.shift);
+    const int pg = pt[p];
+    const bool none = static_cast<uint32_t>(pg) >= static_cast<uint32_t>(M.pages);
+    block = (static_cast<size_t>(none ? 0 : pg) * M.kv_heads + kvh) * M.bytes;
+    at = want - p * M.spp;
+    return none ? (1u << MODE) - 1 : 0u;
+}
+template <int MODE>
+__device__ __forceinline__ Slab4 look_up(const Map4 &M, int slot, int kvh, int kb, int last) {
+    Slab4 r{};
+    if constexpr (MODE == 0) {
+        r.block0 = static_cast<size_t>(kvh) * M.bytes;
+        r.slab0 = kb / kSlab;
+    } else {
+        r.bad = look_up_page<MODE>(M, slot, kvh, kb / kSlab, last, r.block0, r.slab0);
+        if constexpr (MODE == 2) {
+            r.bad |= look_up_page<MODE>(M, slot, kvh, kb / kSlab + 2, last, r.block1, r.slab1) << 2;
         }
-        s[h] = a0 + a1;
     }
+    return r;
+}
+// Slab i of the block, as a lane's own choice: (first byte of its block, slab in it).
+template <int MODE>
+__device__ __forceinline__ void choose(const Slab4 &s, int i, int last, size_t &block, uint32_t &slab) {
+    if constexpr (MODE == 0) {
+        block = s.block0, slab = min(s.slab0 + i, static_cast<uint32_t>(last));
+    } else if constexpr (MODE == 4) {
+        block = s.block0, slab = s.slab0 + i;
+    } else {
+        // Both are read, or the choice becomes one between their addresses, which puts them in memory.
+        const size_t b0 = s.block0, b1 = s.block1;
+        const uint32_t s0 = s.slab0, s1 = s.slab1;
+        block = i & 2 ? b1 : b0, slab = (i & 2 ? s1 : s0) + (i & 1);
+    }
+}
+// The active lanes x 16 bytes from each lane's own address to LDS at (wave-uniform) dst + 16 lane.
+__device__ __forceinline__ void dma16(const uint8_t *from, uint8_t *dst) {
+    const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(vq::lds_addr(dst))));
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at), "v"(dst) : "memory", "m0");
+}
+// Operand row c's pieces (eight of 16 bytes, two rows to the 64 banks) change places by this.
+__device__ __forceinline__ int k_swizzle(int c) { return c >> 1 & 7; }
+// The headers by lanes 0 to 31 (K's) and 32 to 63 (V's), or one of the two.
+template <int U, int MODE>
+__device__ __forceinline__ void dma_heads(const uint8_t *kc, const uint8_t *vc, const Map4 &M, const Slab4 &at, int last, uint8_t *to,
+                                          bool k, bool v) {
+    const int lane = threadIdx.x & 63, piece = min(lane & 31, 4 * U - 1);
+    size_t block;
+    uint32_t slab;
+    choose<MODE>(at, piece / U, last, block, slab);
+    if (k && v || (lane < 32) == k)
+        dma16((lane < 32 ? kc : vc) + block + static_cast<size_t>(M.spp) * (128 * U) + static_cast<size_t>(slab) * (16 * U) + piece % U * 16, to);
+}
+template <int U, int MODE>
+__device__ __forceinline__ void dma_k(const uint8_t *kc, const Map4 &M, const Slab4 &at, int last, uint8_t *part) {
+    const int lane = threadIdx.x & 63;
+    // hd 256: a load brings eight rows of 128 bytes whole, operand rows 8 x + r (x: the load's half of them), pieces swizzled so that
+    // the operand's reads spread over the banks. hd 128: a load brings the half's 16 rows of 64 bytes in operand order.
+    const int r = U == 8 ? lane >> 3 : lane & 15, s = U == 8 ? lane & 7 : lane >> 4;
+#pragma unroll
+    for (int x = 0; x < U / 4; ++x) {
+        size_t block;
+        uint32_t slab;
+        choose<MODE>(at, U == 8 ? 2 * x + (r >> 2) : r >> 2, last, block, slab);
+        const uint8_t *k = kc + block + static_cast<size_t>(slab) * (128 * U) + ((r & 3) * (16 * U) + (U == 8 ? s ^ k_swizzle(8 * x + r) : s) * 16);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) dma16(k + half * (64 * U), part + 1024 * (half * (U / 4) + x));
+    }
+}
+template <int U, int MODE>
+__device__ __forceinline__ void dma_v(const uint8_t *vc, const Map4 &M, const Slab4 &at, int last, uint8_t *part) {
+    const int lane = threadIdx.x & 63;
+    size_t block;
+    uint32_t slab;
+    choose<MODE>(at, lane >> 4, last, block, slab);
+    const uint8_t *v = vc + block + static_cast<size_t>(slab) * (128 * U) + (lane & 15) * 16;
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) dma16(v + 256 * i, part + 1024 * i);
+}
+template <int U>
+__device__ __forceinline__ void read_k(const uint8_t *words, const uint8_t *heads, Raw4<U> &r) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int i = 0; i < U / 4; ++i) {
+            const int at = U == 8 ? 128 * c + 16 * ((2 * g + i) ^ k_swizzle(c)) : 16 * lane;
+            const uint4 w = *reinterpret_cast<const uint4 *>(words + 256 * U * half + at);
+            r.k[half][4 * i] = w.x, r.k[half][4 * i + 1] = w.y, r.k[half][4 * i + 2] = w.z, r.k[half][4 * i + 3] = w.w;
+        }
+        ld_words<U / 2>(heads + (8 * (c >> 2) + 4 * half + (c & 3)) * (2 * U), r.kh[half]);
+    }
+}
+template <int U>
+__device__ __forceinline__ void read_v(const uint8_t *words, const uint8_t *heads, Raw4<U> &r) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < U / 2; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(words + 1024 * i + 16 * lane);
+        r.v[4 * i] = w.x, r.v[4 * i + 1] = w.y, r.v[4 * i + 2] = w.z, r.v[4 * i + 3] = w.w;
+    }
+    r.vh = *reinterpret_cast<const uint4 *>(heads + 16 * (g * U + min(c, U - 1)));
+}
+// At most N loads outstanding, for the few N that occur.
+__device__ __forceinline__ void wait_loads(int n) {
+    switch (n) {
+        case 0: vq::wait_vm<0>(); break;
+        case 5: vq::wait_vm<5>(); break;
+        case 9: vq::wait_vm<9>(); break;
+        default: vq::wait_vm<10>(); break;
+    }
+}
+
+// ---- the products ----
+
+// Query operands of NT tiles: in registers, or (more than 8 operand steps) in LDS, [u][tile][hi, lo][lane].
+template <int U, int NT>
+struct Query {
+    static constexpr bool kLds = NT * U > 8;
+    fh8 h[kLds ? 1 : NT][kLds ? 1 : U], l[kLds ? 1 : NT][kLds ? 1 : U];
+};
+
+// The NT tiles' products of a block: K decoded once for all of them.
+template <int U, int NT>
+__device__ __forceinline__ void scores(const Raw4<U> &r, const Query<U, NT> &q, const uint8_t *qlds, fa4 (&s)[NT][2]) {
+    const int lane = threadIdx.x & 63;
+    fa4 a[2][NT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) a[h][n][0] = a[h][n][1] = fa4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        fh8 qh[NT], ql[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if constexpr (Query<U, NT>::kLds) {
+                qh[n] = *reinterpret_cast<const fh8 *>(qlds + ((u * NT + n) * 2) * 1024 + 16 * lane);
+                ql[n] = *reinterpret_cast<const fh8 *>(qlds + ((u * NT + n) * 2 + 1) * 1024 + 16 * lane);
+            } else {
+                qh[n] = q.h[n][u], ql[n] = q.l[n][u];
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const fh8 k = u % 2 == 0 ? decode8_one<false>(r.k[h][u], r.kh[h][u / 2]) : decode8_one<true>(r.k[h][u], r.kh[h][u / 2]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) a[h][n][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[n], a[h][n][0], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) a[h][n][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[n], a[h][n][1], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[n][h] = a[h][n][0] + a[h][n][1];
 }
 // O^T += V^T P^T. Every lane of a row of 16 needs the headers of all groups of its slab: lane c takes group c's apart and the others
 // read them from LDS (`hl`, the wave's own: [slab][group] scales, zero points; moving them by DPP costs 64 instructions a block of
 // the kind that bounds this kernel).
 template <int U>
 constexpr int head_words = 4 * (8 * U + 8);
-template <int U>
-__device__ __forceinline__ void add_values(const Raw4<U> &r, const fh8 &ph, const fh8 &pl, uint32_t *hl, fa4 (&o)[2 * U]) {
+template <int U, int NT>
+__device__ __forceinline__ void add_values(const Raw4<U> &r, const fh8 (&ph)[NT], const fh8 (&pl)[NT], uint32_t *hl, fa4 (&o)[NT][2 * U]) {
     const int lane = threadIdx.x & 63, c = lane & 15;
     uint32_t *mine = hl + (lane >> 4) * (8 * U + 8);
     if (c < U) {
@@ -556,235 +735,126 @@ __device__ __forceinline__ void add_values(const Raw4<U> &r, const fh8 &ph, cons
 #pragma unroll
         for (int b = 2 * u; b < 2 * u + 2; ++b) {
             const fh8 a = decode8(r.v[b], d, z);
-            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[b], 0, 0, 0);
-            o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[b], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[n], o[n][b], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[n], o[n][b], 0, 0, 0);
         }
     }
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");  // every lane has read before the next block's writes
     __builtin_amdgcn_wave_barrier();
 }
 
-// Decode and verify passes: one workgroup per (chunk, kv head, 16 query vectors); vector j of a segment is (row j / G, head j % G of
-// the kv head's group). Its four waves take the chunk's 32-key blocks in turn, straight from the cache into registers, decoded
-// there into MFMA operands, with an online softmax each; they meet in wave order.
-template <int U, bool PAGED>
-__global__ __launch_bounds__(256, 2) void attention4_split_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
-                                                                  const uint8_t *__restrict__ vc, float *__restrict__ part,
-                                                                  float *__restrict__ pml, float *__restrict__ out, SegTable T, Map4 M,
-                                                                  Cuts C, int heads, int bidirectional, int window) {
-    constexpr int HD = 32 * U;
-    __shared__ __align__(16) float sums[4 * 16 * HD];
-    __shared__ float sm[4][16], sl[4][16];
-    __shared__ __align__(16) uint32_t vheads[4][head_words<U>];
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x % M.kv_heads, list = blockIdx.x / M.kv_heads;
-    const int bases = C.base[lane];
-    const Found found = find_segment(T, C.first, C.total, list);
-    const Seg s = found.s;
-    const int ci = list - found.first, n = found.next - found.first;
-    const int G = heads / M.kv_heads, nvec = s.rows * G, j0 = blockIdx.y * 16;
-    if (j0 >= nvec) return;
-    const int j = min(j0 + c, nvec - 1), t = j / G, h = kvh * G + j - t * G;  // vectors past the last repeat it; not written
-    const Sees see = sees(s, t, bidirectional, window);
-    const int k_lo = first_key(s, window) + ci * C.len, k_hi = min(k_lo + C.len, s.pos0 + s.rows);
-    const int qe = min(see.to, k_hi), last = (k_hi - 1) / kSlab;
-    float m = -INFINITY, l = 0.0f;
-    fa4 o[2 * U];
-#pragma unroll
-    for (int b = 0; b < 2 * U; ++b) o[b] = fa4{0.f, 0.f, 0.f, 0.f};
-    // Lane (c, g) takes K rows of slab c >> 2 and V words of slab g of a block; slabs past the last key's read that one's (masked).
-    auto places = [&](int kb, SlabAt &ks, SlabAt &vs) {
-        ks = slab_at<U, PAGED>(M, s.slot, kvh, min(kb / kSlab + (c >> 2), last));
-        vs = slab_at<U, PAGED>(M, s.slot, kvh, min(kb / kSlab + g, last));
-    };
-    int kb = k_lo + 32 * wv;
-    Raw4<U> r;
-    SlabAt ks, vs;
-    if (kb < k_hi) {
-        places(kb, ks, vs);
-        issue_k<U>(kc, ks, r);
-        issue_v<U>(vc, vs, r);
-    }
-    fh8 qh[U], ql[U];
-    const float unit = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
-    for (; kb < k_hi; kb += 128) {
-        // The next block's K and V come into the registers that this block's have left.
-        const bool more = kb + 128 < k_hi;
-        if (more) places(kb + 128, ks, vs);
-        fa4 sc[2];
-        scores<U>(r, qh, ql, sc);
-        if (more) issue_k<U>(kc, ks, r);
-        fh8 ph, pl;
-        softmax_step<U>(sc, unit, kb, see.from, qe, m, l, o, ph, pl);
-        add_values<U>(r, ph, pl, vheads[wv], o);
-        if (more) issue_v<U>(vc, vs, r);
-    }
-    float *ow = sums + wv * 16 * HD;
-    if (j0 + c < nvec) {
-#pragma unroll
-        for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(ow + c * HD + 16 * b + 4 * g) = o[b];
-        if (g == 0) sm[wv][c] = m, sl[wv][c] = l;
-    }
-    __syncthreads();
-    const size_t base = from_lane(bases, found.index);
-    meet<HD, 4>(sums, sm, sl, 256, threadIdx.x, j0, nvec, G, kvh, heads, s.row0, out, part + base * HD, pml + 2 * base, n, ci);
-}
-
-// The same for hd 128 and 256, whose waves are few (hd 256: 2 per SIMD, for the registers of O and q): the blocks come to LDS by DMA,
-// kSlots of them for each wave, so that the loads of a whole block are in flight while another one is computed with, and no
-// registers are spent on them. A slot: K pieces of 16 bytes in the order that lanes read them, V pieces, headers (lanes 0 .. 31 bring
-// K's, row after row, the others V's). Page ids and addresses are wave-uniform and come by scalar loads: the only vector memory
-// operations of the loop are the DMA's, which the waits count.
-template <int U>
-struct Ring {
-    static constexpr int kSlots = U == 8 ? 2 : 3, kLoads = U + 1, kBytes = 1024 * kLoads;
-};
-// Where a block's slabs are. MODE: how many of the four slabs one look at the page table gives (4: pages of whole blocks, 2: of
-// pairs of slabs), 0: a contiguous cache.
-template <int MODE>
-struct Slab4 {
-    static constexpr int N = MODE == 0 ? 1 : 4 / MODE;
-    size_t block[N];  // first byte of the cache block
-    uint32_t slab[N];
-    uint32_t bad;  // a bit for each slab whose page is none
-};
-template <int MODE>
-__device__ __forceinline__ Slab4<MODE> look_up(const Map4 &M, int slot, int kvh, int kb, int last) {
-    Slab4<MODE> r;
-    r.bad = 0;
-    if constexpr (MODE == 0) {
-        r.block[0] = static_cast<size_t>(kvh) * M.bytes;
-        r.slab[0] = kb / kSlab;
-    } else {
-        const auto *pt = (const __attribute__((address_space(4))) int32_t *)(M.pt) + static_cast<size_t>(slot) * M.pps;
-#pragma unroll
-        for (int i = 0; i < Slab4<MODE>::N; ++i) {
-            // Slabs past the last key's: that one's page is read instead (their keys are masked).
-            const uint32_t slab = min(kb / kSlab + MODE * i, last & ~(MODE - 1));
-            const uint32_t p = static_cast<uint32_t>((static_cast<uint64_t>(slab) * M.mul) >> M.shift);
-            const int pg = pt[p];
-            const bool none = static_cast<uint32_t>(pg) >= static_cast<uint32_t>(M.pages);
-            r.bad |= none ? ((1u << MODE) - 1) << (MODE * i) : 0u;
-            r.block[i] = (static_cast<size_t>(none ? 0 : pg) * M.kv_heads + kvh) * M.bytes;
-            r.slab[i] = slab - p * M.spp;
-            // Opaque from here, or a lane's choice between two of them becomes one between addresses, in memory.
-            asm("" : "+s"(r.block[i]), "+s"(r.slab[i]));
-        }
-    }
-    return r;
-}
-// Slab i of the block, as a lane's own choice: (first byte of its block, slab in it).
-template <int MODE>
-__device__ __forceinline__ void choose(const Slab4<MODE> &s, int i, int last, size_t &block, uint32_t &slab) {
-    if constexpr (MODE == 0) {
-        block = s.block[0], slab = min(s.slab[0] + i, static_cast<uint32_t>(last));
-    } else if constexpr (MODE == 4) {
-        block = s.block[0], slab = s.slab[0] + i;
-    } else {
-        block = i & 2 ? s.block[1] : s.block[0], slab = (i & 2 ? s.slab[1] : s.slab[0]) + (i & 1);
-    }
-}
-// 64 lanes x 16 bytes from each lane's own address to LDS at (wave-uniform) dst, in lane order.
-__device__ __forceinline__ void dma16(const uint8_t *from, uint8_t *dst) {
-    const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(vq::lds_addr(dst))));
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at), "v"(dst) : "memory", "m0");
-}
-// Operand row c's pieces (eight of 16 bytes, two rows to the 64 banks) change places by this.
-__device__ __forceinline__ int k_swizzle(int c) { return c >> 1 & 7; }
-template <int U, int MODE>
-__device__ __forceinline__ void issue_dma(const uint8_t *kc, const uint8_t *vc, const Map4 &M, const Slab4<MODE> &at, int last, uint8_t *slot) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, piece = min(lane & 31, 4 * U - 1);
-    size_t block;
-    uint32_t slab;
-    // K, hd 256: a load brings eight rows of 128 bytes whole, operand rows 8 x + r (x: the load's half of them), pieces swizzled so that
-    // the operand's reads spread over the banks. hd 128: a load brings the half's 16 rows of 64 bytes in operand order.
-    const int r = U == 8 ? lane >> 3 : c, s = U == 8 ? lane & 7 : g;
-    const uint8_t *k[2];
-#pragma unroll
-    for (int x = 0; x < U / 4; ++x) {
-        choose<MODE>(at, U == 8 ? 2 * x + (r >> 2) : r >> 2, last, block, slab);
-        k[x] = kc + block + static_cast<size_t>(slab) * (128 * U) + ((r & 3) * (16 * U) + (U == 8 ? s ^ k_swizzle(8 * x + r) : s) * 16);
-    }
-    choose<MODE>(at, g, last, block, slab);
-    const uint8_t *v = vc + block + static_cast<size_t>(slab) * (128 * U) + c * 16;
-    choose<MODE>(at, piece / U, last, block, slab);
-    const uint8_t *h = (lane < 32 ? kc : vc) + block + static_cast<size_t>(M.spp) * (128 * U) + static_cast<size_t>(slab) * (16 * U) + piece % U * 16;
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int x = 0; x < U / 4; ++x) dma16(k[x] + half * (64 * U), slot + 1024 * (half * (U / 4) + x));
-#pragma unroll
-    for (int i = 0; i < U / 2; ++i) dma16(v + 256 * i, slot + 1024 * (U / 2 + i));
-    dma16(h, slot + 1024 * U);
-}
-template <int U>
-__device__ __forceinline__ void read_k(const uint8_t *slot, Raw4<U> &r) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int i = 0; i < U / 4; ++i) {
-            const int at = U == 8 ? 128 * c + 16 * ((2 * g + i) ^ k_swizzle(c)) : 16 * lane;
-            const uint4 w = *reinterpret_cast<const uint4 *>(slot + 256 * U * half + at);
-            r.k[half][4 * i] = w.x, r.k[half][4 * i + 1] = w.y, r.k[half][4 * i + 2] = w.z, r.k[half][4 * i + 3] = w.w;
-        }
-        ld_words<U / 2>(slot + 1024 * U + (8 * (c >> 2) + 4 * half + (c & 3)) * (2 * U), r.kh[half]);
-    }
-}
-template <int U>
-__device__ __forceinline__ void read_v(const uint8_t *slot, Raw4<U> &r) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int i = 0; i < U / 2; ++i) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(slot + 1024 * (U / 2 + i) + 16 * lane);
-        r.v[4 * i] = w.x, r.v[4 * i + 1] = w.y, r.v[4 * i + 2] = w.z, r.v[4 * i + 3] = w.w;
-    }
-    r.vh = *reinterpret_cast<const uint4 *>(slot + 1024 * U + 512 + 16 * (g * U + min(c, U - 1)));
-}
-
-template <int U, int MODE>
-__global__ __launch_bounds__(256, 2) void attention4_stream_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
-                                                                   const uint8_t *__restrict__ vc, float *__restrict__ part,
-                                                                   float *__restrict__ pml, float *__restrict__ out, SegTable T, Map4 M,
-                                                                   Cuts C, int heads, int bidirectional, int window) {
-    constexpr int HD = 32 * U, SLOTS = Ring<U>::kSlots, BYTES = Ring<U>::kBytes, LOADS = Ring<U>::kLoads;
-    static_assert(SLOTS * BYTES >= 16 * HD * 4, "the waves' sums go where their slots were");
-    __shared__ __align__(16) uint8_t ring[4][SLOTS * BYTES];
-    __shared__ float sm[4][16], sl[4][16];
+// One workgroup of four waves per (chunk of keys, kv head, group of 16 NT query vectors); vector j of a segment is (row j / G, head
+// j % G of the kv head's group). The waves take the 32-key blocks in turn (wave w those whose index is w modulo 4, whatever the
+// chunk: with one chunk a row's sums do not depend on the other rows of its pass), decode them once into MFMA operands for all of
+// the group's tiles, with an online softmax each, and meet at the end.
+//
+// Bound by vector instructions: 640 a block and wave at hd 256 for one tile, 500 of them for the 16384 values decoded, 64 MFMAs
+// beside them; a second tile adds 140 and 64. So groups of more than 16 vectors take two tiles (q in LDS then, for hd 256: O alone
+// is half of the registers of two waves per SIMD). Keys by LDS tiles decoded once for 64 vectors (8 waves, a barrier per 64 keys)
+// took 94 us for 512 rows over 2048 keys, its two waves per SIMD in step; this takes 74.
+// MODE: see Slab4; -1 and -2: blocks by vector loads, in pages and contiguous.
+template <int U, int NT, int MODE>
+__global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
+                                                            const uint8_t *__restrict__ vc, float *__restrict__ part,
+                                                            float *__restrict__ pml, float *__restrict__ out, SegTable T, Map4 M, Cuts C,
+                                                            int heads, int bidirectional, int window) {
+    constexpr bool DMA = MODE >= 0, QLDS = Query<U, NT>::kLds;
+    constexpr int HD = 32 * U, S = DMA ? Ring<U, NT>::kSlots : 1, LD = Ring<U, NT>::kLoads, WORDS = Ring<U, NT>::kWords;
+    // One slot only: its K part and its V part are filled again each as soon as it has been read.
+    constexpr bool SPLIT = DMA && S == 1;
+    constexpr int BYTES = Ring<U, NT>::kBytes, RING = DMA ? S * BYTES : 0, QB = QLDS ? U * NT * 2048 : 0, SUMS = 256 * HD;
+    __shared__ __align__(16) uint8_t lds[4 * RING + QB > SUMS ? 4 * RING + QB : SUMS];
+    __shared__ float sm[4][2][16], sl[4][2][16];
     __shared__ __align__(16) uint32_t vheads[4][head_words<U>];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % M.kv_heads, list = blockIdx.x / M.kv_heads;
     const int bases = C.base[lane];
     const Found found = find_segment(T, C.first, C.total, list);
     const Seg s = found.s;
-    const int ci = list - found.first, n = found.next - found.first;
-    const int G = heads / M.kv_heads, nvec = s.rows * G, j0 = blockIdx.y * 16;
-    if (j0 >= nvec) return;
-    const int k_lo = first_key(s, window) + ci * C.len, k_hi = min(k_lo + C.len, s.pos0 + s.rows), last = (k_hi - 1) / kSlab;
-    int kb = k_lo + 32 * wv;
-    uint8_t *const mine = ring[wv];
-    auto fetch = [&](int block, int slot) {
-        const Slab4<MODE> at = look_up<MODE>(M, s.slot, kvh, block, last);
-        issue_dma<U, MODE>(kc, vc, M, at, last, mine + slot * BYTES);
-        return at.bad;
+    const int G = heads / M.kv_heads, nvec = s.rows * G, units = found.next - found.first, at = list - found.first;
+    // One tile holds a segment's vectors whole. Of several groups the last rows, which see the most keys, come first.
+    const int groups = NT == 1 ? 1 : (nvec + 16 * NT - 1) / (16 * NT), n = NT == 1 ? units : units / groups;
+    const int ci = NT == 1 ? at : at % n, j0 = NT == 1 ? 0 : (groups - 1 - at / n) * 16 * NT;
+    const Sees lo = sees(s, NT == 1 ? 0 : j0 / G, bidirectional, window);
+    const Sees hi = sees(s, NT == 1 ? s.rows - 1 : min(j0 + 16 * NT - 1, nvec - 1) / G, bidirectional, window);
+    const int c_lo = first_key(s, window) + ci * C.len;
+    const int k_lo = max(c_lo, lo.from & ~31), k_hi = n == 1 ? hi.to : min(c_lo + C.len, hi.to), last = (k_hi - 1) / kSlab;
+    if (k_lo >= k_hi) return;
+    int kb = k_lo + 32 * ((wv - (k_lo >> 5)) & 3);
+    uint8_t *const ring = lds + wv * RING, *const qlds = lds + 4 * RING;
+    Raw4<U> r;
+    SlabAt ks, vs;
+    uint32_t bad = 0;  // four bits a slot
+    // Lane (c, g) takes K rows of slab c >> 2 and V words of slab g of a block; slabs past the last key's read that one's (masked).
+    auto places = [&](int block) {
+        ks = slab_at<U, MODE == -1>(M, s.slot, kvh, min(block / kSlab + (c >> 2), last));
+        vs = slab_at<U, MODE == -1>(M, s.slot, kvh, min(block / kSlab + g, last));
     };
-    uint32_t bad[SLOTS] = {};
-    if (kb < k_hi) bad[0] = fetch(kb, 0);
-    const int j = min(j0 + c, nvec - 1), t = j / G, h = kvh * G + j - t * G;  // vectors past the last repeat it; not written
-    const Sees see = sees(s, t, bidirectional, window);
-    const int qe = min(see.to, k_hi);
-    fh8 qh[U], ql[U];
-    const float unit = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
-    float m = -INFINITY, l = 0.0f;
-    fa4 o[2 * U];
+    auto fetch = [&](int block, int slot) {
+        if constexpr (DMA) {
+            const Slab4 where = look_up<MODE>(M, s.slot, kvh, block, last);
+            uint8_t *const to = ring + slot * BYTES;
+            dma_k<U, MODE>(kc, M, where, last, to);
+            if constexpr (SPLIT) dma_heads<U, MODE>(kc, vc, M, where, last, to + 2 * WORDS, true, false);
+            dma_v<U, MODE>(vc, M, where, last, to + WORDS);
+            dma_heads<U, MODE>(kc, vc, M, where, last, to + 2 * WORDS, !SPLIT, true);
+            bad = (bad & ~(15u << 4 * slot)) | where.bad << 4 * slot;
+        } else {
+            places(block);
+            issue_k<U>(kc, ks, r);
+            issue_v<U>(vc, vs, r);
+        }
+    };
+    if (kb < k_hi) fetch(kb, 0);
+    // Vectors past the last one repeat it; they are not written.
+    auto vector = [&](int tile) { return min(j0 + 16 * tile + c, nvec - 1); };
+    auto qrow = [&](int j) {
+        const int t = j / G;
+        return q + (static_cast<size_t>(s.row0 + t) * heads + kvh * G + j - t * G) * HD;
+    };
+    Query<U, NT> qr;
+    float unit[NT];
+    Sees see[NT];
 #pragma unroll
-    for (int b = 0; b < 2 * U; ++b) o[b] = fa4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < NT; ++i) {
+        see[i] = sees(s, vector(i) / G, bidirectional, window);
+        see[i].to = min(see[i].to, k_hi);
+    }
+    if constexpr (QLDS) {  // a wave makes every second step's operands of a tile
+        __shared__ float units[NT][16];
+        const int tile = wv % NT;
+        fh8 h[U], l[U];
+        const float x = load_query<U>(qrow(vector(tile)), h, l);
+        if (wv < NT && g == 0) units[tile][c] = x;
 #pragma unroll
-    for (int i = 1; i < SLOTS; ++i)
-        if (kb + 128 * i < k_hi) bad[i] = fetch(kb + 128 * i, i);
+        for (int u = 0; u < U; ++u) {
+            if (u % (4 / NT) != wv / NT) continue;
+            *reinterpret_cast<fh8 *>(qlds + ((u * NT + tile) * 2) * 1024 + 16 * lane) = h[u];
+            *reinterpret_cast<fh8 *>(qlds + ((u * NT + tile) * 2 + 1) * 1024 + 16 * lane) = l[u];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NT; ++i) unit[i] = units[i][c];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) unit[i] = load_query<U>(qrow(vector(i)), qr.h[i], qr.l[i]);
+    }
+    float m[NT], l[NT];
+    fa4 o[NT][2 * U];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < 2 * U; ++b) o[i][b] = fa4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int i = 1; i < S; ++i)
+        if (kb + 128 * i < k_hi) fetch(kb + 128 * i, i);
     while (kb < k_hi) {
 #pragma unroll
-        for (int slot = 0; slot < SLOTS; ++slot) {
+        for (int slot = 0; slot < S; ++slot) {
             if (kb >= k_hi) break;
             // A SIMD serves its older wave first, which left the younger one to finish alone, 11 of 40 us (131071 keys). A wave
             // that nears its end steps back, so that they finish together.
@@ -793,50 +863,116 @@ __global__ __launch_bounds__(256, 2) void attention4_stream_kernel(const float *
             else if (left == 2) __builtin_amdgcn_s_setprio(2);
             else if (left == 1) __builtin_amdgcn_s_setprio(1);
             else __builtin_amdgcn_s_setprio(0);
-            // Landed: all but the loads of the blocks behind this one.
-            const int behind = min(left, SLOTS - 1);
-            if (behind == 0) vq::wait_vm<0>();
-            else if (behind == 1) vq::wait_vm<LOADS>();
-            else vq::wait_vm<2 * LOADS>();
-            Raw4<U> r;
-            uint8_t *const from = mine + slot * BYTES;
-            read_k<U>(from, r);
-            if (MODE != 0 && bad[slot] != 0 && (bad[slot] >> (c >> 2) & 1)) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int x = 0; x < U / 2; ++x) r.kh[half][x] = kNanHeader | kNanHeader << 16;
+            const bool more = left >= S;
+            uint8_t *const from = ring + slot * BYTES;
+            Slab4 where;
+            if constexpr (DMA) {
+                // Landed: all but this block's V and the blocks behind it. The page of the block that comes into the slot meanwhile.
+                wait_loads(SPLIT ? LD : LD * min(left, S - 1));
+                if (SPLIT && more) where = look_up<MODE>(M, s.slot, kvh, kb + 128 * S, last);
+                read_k<U>(from, from + 2 * WORDS, r);
+                if (MODE != 0 && bad != 0 && (bad >> (4 * slot + (c >> 2)) & 1)) no_page<U>(r);
+            } else {
+                if (more) places(kb + 128);
             }
-            fa4 sc[2];
-            scores<U>(r, qh, ql, sc);
-            fh8 ph, pl;
-            softmax_step<U>(sc, unit, kb, see.from, qe, m, l, o, ph, pl);
-            read_v<U>(from, r);
-            add_values<U>(r, ph, pl, vheads[wv], o);
-            vq::wait_lgkm0();  // the slot has been read
-            if (kb + 128 * SLOTS < k_hi) bad[slot] = fetch(kb + 128 * SLOTS, slot);
+            fa4 sc[NT][2];
+            scores<U, NT>(r, qr, qlds, sc);
+            if (more) {
+                if constexpr (SPLIT) {
+                    vq::wait_lgkm0();  // the part has been read
+                    dma_k<U, MODE>(kc, M, where, last, from);
+                    dma_heads<U, MODE>(kc, vc, M, where, last, from + 2 * WORDS, true, false);
+                    bad = (bad & ~(15u << 4 * slot)) | where.bad << 4 * slot;
+                } else if constexpr (!DMA) {
+                    issue_k<U>(kc, ks, r);
+                }
+            }
+            fh8 ph[NT], pl[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) softmax_step<U>(sc[i], unit[i], kb, see[i].from, see[i].to, m[i], l[i], o[i], ph[i], pl[i]);
+            if constexpr (DMA) {
+                if (SPLIT) wait_loads(more ? LD : 0);
+                read_v<U>(from + WORDS, from + 2 * WORDS + 512, r);
+            }
+            add_values<U, NT>(r, ph, pl, vheads[wv], o);
+            if (more) {
+                if constexpr (DMA) {
+                    vq::wait_lgkm0();
+                    if constexpr (SPLIT) {
+                        dma_v<U, MODE>(vc, M, where, last, from + WORDS);
+                        dma_heads<U, MODE>(kc, vc, M, where, last, from + 2 * WORDS, false, true);
+                    } else {
+                        fetch(kb + 128 * S, slot);
+                    }
+                } else {
+                    issue_v<U>(vc, vs, r);
+                }
+            }
             kb += 128;
         }
     }
-    __syncthreads();  // every slot of every wave has been read
-    float *sums = reinterpret_cast<float *>(&ring[0][0]), *ow = sums + wv * 16 * HD;
-    if (j0 + c < nvec) {
+    __builtin_amdgcn_s_setprio(0);
+    __syncthreads();  // every slot of every wave, and the queries, have been read
+    float *sums = reinterpret_cast<float *>(lds);
+    const Dest to{out, part, pml, static_cast<size_t>(from_lane(bases, found.index)), heads, G, kvh, s.row0, nvec, n, ci};
+    if constexpr (NT == 1) {
+        if (j0 + c < nvec) {
 #pragma unroll
-        for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(ow + c * HD + 16 * b + 4 * g) = o[b];
-        if (g == 0) sm[wv][c] = m, sl[wv][c] = l;
+            for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(sums + (wv * 16 + c) * HD + 16 * b + 4 * g) = o[0][b];
+            if (g == 0) sm[wv][0][c] = m[0], sl[wv][0][c] = l[0];
+        }
+        __syncthreads();
+        meet4<HD>(sums, sm, sl, j0, to);
+    } else {
+        // Waves 2 and 3 hand their sums to waves 0 and 1, then those two exchange a tile each. [wave or its partner][tile][lane's
+        // values]: a lane reads what the same lane of the other wave wrote.
+        auto give = [&](int box, int i) {
+            float *to_box = sums + (box * 2 + i) * 16 * HD;
+#pragma unroll
+            for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(to_box + 256 * b + 4 * lane) = o[i][b];
+            if (g == 0) sm[wv][i][c] = m[i], sl[wv][i][c] = l[i];
+        };
+        auto take = [&](int box, int i, int from, bool first) {  // `first`: the other wave's sums count as the left operand
+            const float *box_at = sums + (box * 2 + i) * 16 * HD;
+            const float om = sm[from][i][c], ol = sl[from][i][c], mx = fmaxf(m[i], om);
+            const float own = share(m[i], mx), other = share(om, mx), fl = first ? other : own, fr = first ? own : other;
+            l[i] = fmaf(first ? l[i] : ol, fr, (first ? ol : l[i]) * fl);
+#pragma unroll
+            for (int b = 0; b < 2 * U; ++b) {
+                const fa4 x = *reinterpret_cast<const fa4 *>(box_at + 256 * b + 4 * lane);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][b][e] = first ? fmaf(o[i][b][e], fr, x[e] * fl) : fmaf(x[e], fr, o[i][b][e] * fl);
+            }
+            m[i] = mx;
+        };
+        if (wv >= 2) give(wv - 2, 0), give(wv - 2, 1);
+        __syncthreads();
+        if (wv < 2) take(wv, 0, wv + 2, false), take(wv, 1, wv + 2, false);
+        __syncthreads();
+        if (wv == 0) give(0, 1);
+        if (wv == 1) give(1, 0);
+        __syncthreads();
+        if (wv >= 2) return;
+        if (wv == 0) take(1, 0, 1, false);
+        else take(0, 1, 0, true);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int j = j0 + 16 * i + c;
+            if (wv != i || j >= nvec) continue;
+#pragma unroll
+            for (int b = 0; b < 2 * U; ++b) to.put<HD>(j, 16 * b + 4 * g, float4{o[i][b][0], o[i][b][1], o[i][b][2], o[i][b][3]}, m[i], l[i]);
+        }
     }
-    __syncthreads();
-    const size_t base = from_lane(bases, found.index);
-    meet<HD, 4>(sums, sm, sl, 256, threadIdx.x, j0, nvec, G, kvh, heads, s.row0, out, part + base * HD, pml + 2 * base, n, ci);
 }
 
 // out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, for segments of more than one. It is latency that this
 // kernel spends, so a workgroup takes 64 dims of a (row, head) (32 where hd is no multiple of 64), a thread four dims of every 16th
 // (32nd) chunk, four of them in flight, under a running maximum; the 16 (32) sums meet in order. 24 rows of 128 chunks, hd 256: 4 us;
 // one workgroup of four waves for a row took 11.
-template <int HD>
+template <int HD, int NT>
 __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
-                                                               float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads) {
+                                                               float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads,
+                                                               int G, int bidirectional, int window) {
     constexpr int Q = HD % 64 == 0 ? 16 : 8, GROUPS = 256 / Q;
     __shared__ float sm[GROUPS], sl[GROUPS];
     __shared__ float4 sacc[GROUPS][Q];
@@ -846,21 +982,29 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
     const Found found = find_segment(T, R.first, R.total, row);
     const Seg s = found.s;
     const int t = row - found.first, i = found.index;
-    const int n = (i + 1 < T.n ? from_lane(chunks, i + 1 < 64 ? i + 1 : 63) : C.total) - from_lane(chunks, i);
+    const int units = (i + 1 < T.n ? from_lane(chunks, i + 1 < 64 ? i + 1 : 63) : C.total) - from_lane(chunks, i);
+    const int n = NT == 1 ? units : units / ((s.rows * G + 16 * NT - 1) / (16 * NT));
     if (n == 1) return;
+    // One tile: every chunk has been written. Several groups: those that hold keys of this row.
+    int c_lo = 0, c_hi = n;
+    if (NT != 1) {
+        const Sees see = sees(s, t, bidirectional, window);
+        const int k0 = first_key(s, window);
+        c_lo = (see.from - k0) / C.len, c_hi = min((see.to - 1 - k0) / C.len + 1, n);
+    }
     const size_t at = static_cast<size_t>(from_lane(bases, i)) + (static_cast<size_t>(t) * heads + h) * n;
     const float *ml = pml + 2 * at;
     float m = -INFINITY, L = 0.0f;
     float4 acc{0.f, 0.f, 0.f, 0.f};
     auto scale = [](float x, float to) { return x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - to); };
-    for (int c0 = grp; c0 < n; c0 += 4 * GROUPS) {
+    for (int c0 = c_lo + grp; c0 < c_hi; c0 += 4 * GROUPS) {
         float4 p[4];
         float mc[4], lc[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int c = c0 + GROUPS * k < n ? c0 + GROUPS * k : c0;
+            const int c = c0 + GROUPS * k < c_hi ? c0 + GROUPS * k : c0;
             p[k] = *reinterpret_cast<const float4 *>(part + (at + c) * HD + d);
-            mc[k] = c0 + GROUPS * k < n ? ml[2 * c] : -INFINITY;
+            mc[k] = c0 + GROUPS * k < c_hi ? ml[2 * c] : -INFINITY;
             lc[k] = ml[2 * c + 1];
         }
         const float mn = fmaxf(fmaxf(m, fmaxf(mc[0], mc[1])), fmaxf(mc[2], mc[3])), f0 = scale(m, mn);
@@ -869,7 +1013,7 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
         acc = float4{acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if (c0 + GROUPS * k >= n) break;
+            if (c0 + GROUPS * k >= c_hi) break;
             const float f = scale(mc[k], mn);
             L = fmaf(lc[k], f, L);
             acc.x = fmaf(p[k].x, f, acc.x);
@@ -900,147 +1044,6 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
     const float4 r{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
     __builtin_memcpy(out + (static_cast<size_t>(s.row0 + t) * heads + h) * HD + d, &r, 16);
-}
-
-// Prompt passes, and any pass without a workspace: a workgroup of NW waves takes NW / 2 tiles of 16 query vectors of a kv head, two
-// waves each, one for the 32-key blocks of each parity (blocks at multiples of 32 keys whatever the rows, so a row's sums do not
-// depend on the others); their sums meet at the end. Per step of 64 keys the threads load the next step's words, the waves consume
-// the present one from LDS, decoded once for all tiles: K rows of HD + 16 f16, V^T [dim][32 positions] with 16-byte pieces swizzled
-// by (dim >> 2) & 3; the loaded words are decoded into the other LDS buffer: one barrier per step.
-__device__ __forceinline__ int vt_at(int d, int octet) { return d * 32 + ((octet ^ ((d >> 2) & 3)) << 3); }
-
-template <int U, bool PAGED, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attention4_tiled_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
-                                                                      const uint8_t *__restrict__ vc, float *__restrict__ out,
-                                                                      SegTable T, Starts R, Map4 M, int heads, int bidirectional, int window) {
-    constexpr int HD = 32 * U, LDK = HD + 16, TH = 64 * NW, TILES = NW / 2;
-    constexpr int KW = U % 4 == 0 ? 4 : U % 2 == 0 ? 2 : 1, W = U % 2 == 0 ? 4 : 2;  // words of a K unit, of a V unit
-    constexpr int KUN = 64 * 4 * (U / KW), VUN = 8 * 16 * (2 * U / W);               // units of a step
-    constexpr int KN = (KUN + TH - 1) / TH, VN = (VUN + TH - 1) / TH;                // of a thread
-    constexpr int KB = 32 * LDK, VB = HD * 32;                                       // f16 elements of a block
-    constexpr int BUF = 2 * (KB + VB), MEET = TILES * 2 * 16 * HD * 2;               // f16 elements: a buffer, the sums at the end
-    __shared__ __align__(16) _Float16 kv[2 * BUF > MEET ? 2 * BUF : MEET];
-    __shared__ SlabAt slabs[2][8];
-    __shared__ float sm[TILES][2][16], sl[TILES][2][16];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, c = lane & 15, g = lane >> 4, tile = wv >> 1, par = wv & 1;
-    const int kvh = blockIdx.x % M.kv_heads, G = heads / M.kv_heads;
-    // Workgroups take the kv heads in turn, the last rows, which see the most keys, first.
-    const int group = R.total - 1 - blockIdx.x / M.kv_heads;
-    const Found found = find_segment(T, R.first, R.total, group);
-    const Seg s = found.s;
-    const int tb = group - found.first;
-    const int nvec = s.rows * G, first = tb * 16 * TILES, j0 = first + 16 * tile;
-    const bool on = j0 < nvec;
-    const int j = min(j0 + c, nvec - 1), t = j / G, h = kvh * G + j - t * G;
-    const Sees see = sees(s, t, bidirectional, window), a = sees(s, first / G, bidirectional, window),
-               z = sees(s, min(first + 16 * TILES - 1, nvec - 1) / G, bidirectional, window);
-    const int k0 = a.from & ~63, k_hi = z.to, steps = (k_hi - k0 + 63) / 64, s0 = a.from / kSlab, s1 = (k_hi - 1) / kSlab;
-    auto look = [&](int step) { return slab_at<U, PAGED>(M, s.slot, kvh, min(max((k0 + 64 * step) / kSlab + (tid & 7), s0), s1)); };
-    if (tid < 16) slabs[tid >> 3][tid & 7] = look(tid >> 3);
-    fh8 qh[U], ql[U];
-    const float unit = load_query<U>(q + (static_cast<size_t>(s.row0 + t) * heads + h) * HD, qh, ql);
-    __syncthreads();
-    uint32_t rk[KN][KW], rkh[KN][KW == 4 ? 2 : 1], rv[VN][W];
-    uint4 rvh[VN][W / 2];
-    auto issue = [&](int step) {
-        const SlabAt *sa = slabs[step & 1];
-#pragma unroll
-        for (int i = 0; i < KN; ++i) {  // unit: (key, word group of dims, run of KW words)
-            const int unit = (tid + TH * i) % KUN, key = unit / (4 * (U / KW)), rest = unit % (4 * (U / KW)), g4 = rest / (U / KW), u0 = rest % (U / KW) * KW;
-            const SlabAt &at = sa[key >> 3];
-            ld_words<KW>(kc + at.words + (key & 7) * (16 * U) + g4 * (4 * U) + 4 * u0, rk[i]);
-            const uint8_t *hp = kc + at.heads + (key & 7) * (2 * U) + 2 * u0;
-            if constexpr (KW == 4) ld_words<2>(hp, rkh[i]);
-            else if constexpr (KW == 2) ld_words<1>(hp, rkh[i]);
-            else rkh[i][0] = *reinterpret_cast<const uint16_t *>(hp);
-            if (at.bad)
-#pragma unroll
-                for (auto &x : rkh[i]) x = kNanHeader | kNanHeader << 16;
-        }
-#pragma unroll
-        for (int i = 0; i < VN; ++i) {  // unit: (slab, run of W dim tiles, dim of a tile)
-            const int unit = (tid + TH * i) % VUN, slab = unit / (16 * (2 * U / W)), rest = unit % (16 * (2 * U / W));
-            const SlabAt &at = sa[slab];
-            ld_words<W>(vc + at.words + rest * (4 * W), rv[i]);
-#pragma unroll
-            for (int k = 0; k < W / 2; ++k) rvh[i][k] = *reinterpret_cast<const uint4 *>(vc + at.heads + 16 * ((rest >> 4) * (W / 2) + k));
-        }
-    };
-    auto stage = [&](int step) {
-        _Float16 *buf = kv + (step & 1) * BUF;
-#pragma unroll
-        for (int i = 0; i < KN; ++i) {
-            const int unit = tid + TH * i, key = unit / (4 * (U / KW)), rest = unit % (4 * (U / KW)), g4 = rest / (U / KW), u0 = rest % (U / KW) * KW;
-            if (KUN % TH && unit >= KUN) break;
-            const int row = 16 * ((key >> 2) & 1) + 4 * ((key >> 3) & 3) + (key & 3);  // of the block's S^T operand
-            _Float16 *kd = buf + (key >> 5) * (KB + VB) + row * LDK + 32 * u0 + 8 * g4;
-#pragma unroll
-            for (int k = 0; k < KW; ++k) {
-                const uint32_t h2 = rkh[i][k / 2];
-                *reinterpret_cast<fh8 *>(kd + 32 * k) = k % 2 == 0 ? decode8_one<false>(rk[i][k], h2) : decode8_one<true>(rk[i][k], h2);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < VN; ++i) {
-            const int unit = tid + TH * i, slab = unit / (16 * (2 * U / W)), rest = unit % (16 * (2 * U / W));
-            if (VUN % TH && unit >= VUN) break;
-            _Float16 *vd = buf + (slab >> 2) * (KB + VB) + KB;
-#pragma unroll
-            for (int k = 0; k < W; ++k) {
-                const uint4 x = rvh[i][k / 2];
-                const fh2 ds[4] = {scales2(x.x), scales2(x.y), scales2(x.z), scales2(x.w)};
-                const fh2 zs[4] = {zeros2(x.x, false), zeros2(x.y, true), zeros2(x.z, false), zeros2(x.w, true)};
-                *reinterpret_cast<fh8 *>(vd + vt_at(16 * ((rest >> 4) * W + k) + (rest & 15), slab & 3)) = decode8(rv[i][k], ds, zs);
-            }
-        }
-    };
-    issue(0);
-    float m = -INFINITY, l = 0.0f;
-    fa4 o[2 * U];
-#pragma unroll
-    for (int b = 0; b < 2 * U; ++b) o[b] = fa4{0.f, 0.f, 0.f, 0.f};
-    stage(0);
-    __syncthreads();
-    for (int step = 0; step < steps; ++step) {
-        const bool more = step + 1 < steps;
-        SlabAt next{};
-        if (tid < 8) next = look(step + 2);
-        if (more) issue(step + 1);
-        const int kb = k0 + 64 * step + 32 * par;
-        if (on && kb < k_hi) {
-            const _Float16 *ks = kv + (step & 1) * BUF + par * (KB + VB), *vt = ks + KB;
-            fa4 sc[2];
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                fa4 a0{0.f, 0.f, 0.f, 0.f}, a1{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const fh8 k8 = *reinterpret_cast<const fh8 *>(ks + (16 * hh + c) * LDK + 8 * g + 32 * u);
-                    a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[u], a0, 0, 0, 0);
-                    a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[u], a1, 0, 0, 0);
-                }
-                sc[hh] = a0 + a1;
-            }
-            fh8 ph, pl;
-            softmax_step<U>(sc, unit, kb, see.from, see.to, m, l, o, ph, pl);
-#pragma unroll
-            for (int b = 0; b < 2 * U; ++b) {
-                const fh8 v8 = *reinterpret_cast<const fh8 *>(vt + vt_at(16 * b + c, g));
-                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[b], 0, 0, 0);
-                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[b], 0, 0, 0);
-            }
-        }
-        if (more) stage(step + 1);
-        if (tid < 8) slabs[step & 1][tid] = next;
-        __syncthreads();
-    }
-    float *sums = reinterpret_cast<float *>(kv);
-#pragma unroll
-    for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(sums + (wv * 16 + c) * HD + 16 * b + 4 * g) = o[b];
-    if (g == 0) sm[tile][par][c] = m, sl[tile][par][c] = l;
-    __syncthreads();
-    for (int i = 0; i < TILES; ++i)
-        meet<HD, 2>(sums + i * 32 * HD, sm[i], sl[i], TH, tid, first + 16 * i, nvec, G, kvh, heads, s.row0, out, nullptr, nullptr, 1, 0);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------
@@ -1116,47 +1119,50 @@ int launch_read4(const void *kc, const void *vc, float *k, float *v, const SegTa
     return status_of(hipGetLastError());
 }
 
-// Chunks for about a round or a few of the 512 workgroups that run at once (two per CU). `rounds` full rounds need chunks of at
-// least some length; among 1 to 4 rounds the least of rounds x (length + what a chunk costs besides its keys, in keys).
-int chunks_of(const SegTable &T, int i, long long len, int window) {
-    return static_cast<int>((T.s[i].pos0 + T.s[i].rows - first_key(T.s[i], window) + len - 1) / len);
-}
-Cuts make_cuts(const SegTable &T, int heads, int kv_heads, int window) {
-    #ifndef KFIX
-#define KFIX 160
-#endif
-    constexpr int kSlots = 512, kFixed = KFIX;
-    int groups = 1;
-    long long keys = 0;
+// Chunks for the 512 workgroups that run at once (two per CU): of the lengths that make one to four full rounds, and of whole
+// contexts, the one with the least rounds x (keys of a chunk + what a chunk costs besides, in keys: its start and end, 160 keys' time,
+// and with more than one chunk the partial results of a group, 100 for each tile).
+struct Shape {
+    int heads, kv_heads, tiles;
+    int groups(const Seg &s) const { return (s.rows * (heads / kv_heads) + 16 * tiles - 1) / (16 * tiles); }
+};
+int keys_of(const Seg &s, int window) { return s.pos0 + s.rows - first_key(s, window); }
+int chunks_of(const Seg &s, long long len, int window) { return static_cast<int>((keys_of(s, window) + len - 1) / len); }
+Cuts make_cuts(const SegTable &T, const Shape &P, int window, bool whole) {
+    constexpr long long kSlots = 512, kFixed = 160, kPart = 100;
+    long long most = 0, work = 0;
     for (int i = 0; i < T.n; ++i) {
-        groups = max(groups, (T.s[i].rows * (heads / kv_heads) + 15) / 16);
-        keys += T.s[i].pos0 + T.s[i].rows - first_key(T.s[i], window);
+        most = max(most, static_cast<long long>(keys_of(T.s[i], window)));
+        work += static_cast<long long>(keys_of(T.s[i], window)) * P.groups(T.s[i]) * P.kv_heads;
     }
+    most = (most + 127) / 128 * 128;
     auto count = [&](long long len) {
         long long n = 0;
-        for (int i = 0; i < T.n; ++i) n += chunks_of(T, i, len, window);
-        return n * kv_heads * groups;
+        for (int i = 0; i < T.n; ++i) n += static_cast<long long>(chunks_of(T.s[i], len, window)) * P.groups(T.s[i]);
+        return n * P.kv_heads;
     };
-    long long best = 0, cost = 0;
-    for (int rounds = 1; rounds <= 4; ++rounds) {
-        long long len = (keys * kv_heads * groups / (kSlots * rounds) + 127) / 128 * 128;
-        len = len < 128 ? 128 : len;
-        for (int i = 0; i < 64 && count(len) > static_cast<long long>(kSlots) * rounds; ++i) len += 128;
-        const long long c = rounds * (len + kFixed);
-        if (best == 0 || c < cost) best = len, cost = c;
+    auto cost = [&](long long len) { return (count(len) + kSlots - 1) / kSlots * (len + kFixed + (len < most ? kPart * P.tiles : 0)); };
+    long long best = most;
+    for (int rounds = 1; rounds <= 4 && !whole; ++rounds) {
+        long long lo = max(work / (kSlots * rounds) / 128, 1LL), hi = most / 128;  // the least length of at most that many rounds
+        while (lo < hi) {
+            const long long mid = (lo + hi) / 2;
+            if (count(128 * mid) > kSlots * rounds) lo = mid + 1;
+            else hi = mid;
+        }
+        if (128 * lo < most && cost(128 * lo) < cost(best)) best = 128 * lo;
     }
     Cuts C;
     C.len = static_cast<int>(best);
-    C.total = C.most = 0;
+    C.total = 0;
     int base = 0;
     for (int i = 0; i < VQ_MAX_SEGMENTS; ++i) {
         C.first[i] = C.total;
         C.base[i] = base;
         if (i >= T.n) continue;
-        const int n = chunks_of(T, i, C.len, window);
-        if (n > 1) base += n * T.s[i].rows * heads;
-        C.total += n;
-        C.most = max(C.most, n);
+        const int n = chunks_of(T.s[i], C.len, window);
+        if (n > 1) base += n * T.s[i].rows * P.heads;
+        C.total += n * P.groups(T.s[i]);
     }
     return C;
 }
@@ -1164,15 +1170,19 @@ Cuts make_cuts(const SegTable &T, int heads, int kv_heads, int window) {
 size_t parts_of(const SegTable &T, const Cuts &C, int heads, int window) {
     size_t n = 0;
     for (int i = 0; i < T.n; ++i) {
-        const size_t k = chunks_of(T, i, C.len, window);
+        const size_t k = chunks_of(T.s[i], C.len, window);
         if (k > 1) n += k * T.s[i].rows * heads;
     }
     return n;
 }
+// Two tiles to a group where a kv head has more than 16 query vectors in a segment; always without a workspace, so that a row's sums
+// are the same in every pass.
+Shape shape_of(const SegTable &T, int heads, int kv_heads, bool whole) {
+    return Shape{heads, kv_heads, whole || max_seg_rows(T) * (heads / kv_heads) > 16 ? 2 : 1};
+}
 size_t attention4_ws_bytes(const SegTable &T, int heads, int kv_heads, int hd, int window) {
-    if (max_seg_rows(T) > VQ_ATTN_ROW_MAX) return 0;
-    const size_t n = parts_of(T, make_cuts(T, heads, kv_heads, window), heads, window);
-    return n * (hd + 2) * 4 + 16;
+    const Cuts C = make_cuts(T, shape_of(T, heads, kv_heads, false), window, false);
+    return parts_of(T, C, heads, window) * (hd + 2) * 4 + 16;
 }
 
 template <typename F>
@@ -1193,43 +1203,38 @@ int launch_attention4(const float *q, const void *kc, const void *vc, float *out
                       int bidirectional, int window, void *ws, size_t ws_bytes, hipStream_t s) {
     if (!q || !out) return VQ_ERR_ARG;
     if (heads < M.kv_heads || heads % M.kv_heads || window < 0) return VQ_ERR_SHAPE;
-    const int G = heads / M.kv_heads;
+    if (static_cast<long long>(T.total) * heads > INT32_MAX / 2) return VQ_ERR_SHAPE;
+    const bool whole = ws == nullptr;
+    const Shape P = shape_of(T, heads, M.kv_heads, whole);
+    const Cuts C = make_cuts(T, P, window, whole);
+    const size_t parts = parts_of(T, C, heads, window);
+    if (!whole && ((reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < parts * (hd + 2) * 4 + 16)) return VQ_ERR_WORKSPACE;
+    const Starts R = starts_of(T, rows_of, 0);
     auto *kb = static_cast<const uint8_t *>(kc), *vb = static_cast<const uint8_t *>(vc);
-    if (ws != nullptr && max_seg_rows(T) <= VQ_ATTN_ROW_MAX) {
-        if ((reinterpret_cast<uintptr_t>(ws) & 15) || ws_bytes < attention4_ws_bytes(T, heads, M.kv_heads, hd, window))
-            return VQ_ERR_WORKSPACE;
-        const Cuts C = make_cuts(T, heads, M.kv_heads, window);
-        const Starts R = starts_of(T, rows_of, 0);
-        const size_t parts = parts_of(T, C, heads, window);
-        float *part = static_cast<float *>(ws), *pml = part + parts * hd;
-        const dim3 grid(C.total * M.kv_heads, (max_seg_rows(T) * G + 15) / 16);
-        for_hd(hd, [&](auto u) {
-            constexpr int U = decltype(u)::value;
-            auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window); };
-            if constexpr (U % 4 == 0) {
-                if (!M.pt) return go(attention4_stream_kernel<U, 0>);
-                if (M.spp % 4 == 0) return go(attention4_stream_kernel<U, 4>);
-                if (M.spp % 2 == 0) return go(attention4_stream_kernel<U, 2>);
-            }
-            if (M.pt) go(attention4_split_kernel<U, true>);
-            else if constexpr (U % 4 != 0) go(attention4_split_kernel<U, false>);
-        });
-        for_hd(hd, [&](auto u) {
-            constexpr int U = decltype(u)::value;
-            if (parts) attention4_merge_kernel<32 * U><<<dim3(T.total * heads, U % 2 == 0 ? U / 2 : U), 256, 0, s>>>(part, pml, out, T, C, R, heads);
-        });
-        return status_of(hipGetLastError());
-    }
-    constexpr int NW = 8, PER = 16 * (NW / 2);
-    long long vectors = 0;
-    for (int i = 0; i < T.n; ++i) vectors += static_cast<long long>(T.s[i].rows) * G + PER;
-    if (vectors / PER * M.kv_heads > INT32_MAX) return VQ_ERR_SHAPE;
-    const Starts R = starts_of(T, [](const Seg &x, int g) { return static_cast<int>((static_cast<long long>(x.rows) * g + PER - 1) / PER); }, G);
-    const dim3 grid(static_cast<unsigned>(R.total) * M.kv_heads);
+    float *part = static_cast<float *>(ws), *pml = part + parts * hd;
+    const dim3 grid(static_cast<unsigned>(C.total) * M.kv_heads);
+    auto pass = [&](auto u, auto tiles) {
+        constexpr int U = decltype(u)::value, NT = decltype(tiles)::value;
+        auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window); };
+        // hd 128 and 256 by DMA but for pages of odd numbers of slabs.
+        bool done = false;
+        if constexpr (U % 4 == 0) {
+            done = true;
+            if (!M.pt) go(attention4_kernel<U, NT, 0>);
+            else if (M.spp % 4 == 0) go(attention4_kernel<U, NT, 4>);
+            else if (M.spp % 2 == 0) go(attention4_kernel<U, NT, 2>);
+            else done = false;
+        }
+        if (!done && M.pt) go(attention4_kernel<U, NT, -1>);
+        if constexpr (U % 4 != 0)
+            if (!M.pt) go(attention4_kernel<U, NT, -2>);
+        if (parts)
+            attention4_merge_kernel<32 * U, NT><<<dim3(T.total * heads, U % 2 == 0 ? U / 2 : U), 256, 0, s>>>(part, pml, out, T, C, R, heads,
+                                                                                                          heads / M.kv_heads, bidirectional, window);
+    };
     for_hd(hd, [&](auto u) {
-        constexpr int U = decltype(u)::value;
-        if (M.pt) attention4_tiled_kernel<U, true, NW><<<grid, 64 * NW, 0, s>>>(q, kb, vb, out, T, R, M, heads, bidirectional, window);
-        else attention4_tiled_kernel<U, false, NW><<<grid, 64 * NW, 0, s>>>(q, kb, vb, out, T, R, M, heads, bidirectional, window);
+        if (P.tiles == 1) pass(u, std::integral_constant<int, 1>{});
+        else pass(u, std::integral_constant<int, 2>{});
     });
     return status_of(hipGetLastError());
 }
