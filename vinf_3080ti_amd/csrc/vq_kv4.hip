@@ -425,7 +425,7 @@ __device__ __forceinline__ void softmax_step(const fa4 (&s)[2], float unit, int 
 // key rounded down to 32; segment i's groups x chunks begin at first[i] of one list, its partial results at base[i] (where it has
 // more than one chunk).
 struct Cuts {
-    int len, total;
+    int len, total, most;  // most: of a segment's chunks
     int first[VQ_MAX_SEGMENTS], base[VQ_MAX_SEGMENTS];
 };
 // First key that any row of a segment sees, rounded down to a block.
@@ -530,7 +530,7 @@ __device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, const Sl
 
 // For hd 128 and 256, whose waves are few (hd 256: 2 per SIMD, for the registers of O and q): the blocks come to LDS by DMA, kSlots of
 // them for each wave, so that the loads of one are in flight while another is computed with, and no registers are spent on them. A
-// slot is K's words in the order of the loads, V's words, and 512 bytes each of K's and of V's headers, slab after slab. Page ids and
+// slot is K's words, slab after slab, V's words, and 512 bytes each of K's and of V's headers, slab after slab. Page ids and
 // addresses are wave-uniform and come by scalar loads: the only vector memory operations of the loop are the DMA's, which the waits
 // count.
 template <int U, int NT>
@@ -539,95 +539,86 @@ struct Ring {
     static constexpr int kWords = 512 * U, kBytes = 2 * kWords + 1024;
     static constexpr int kLoads = kSlots == 1 ? U / 2 + 1 : U + 1;  // of half a slot that is filled by halves, or of a slot
 };
-// Where a block's slabs are. MODE: how many of the four slabs one look at the page table gives (4: pages of whole blocks, 2: of
-// pairs of slabs), 0: a contiguous cache.
+// Where a block's four slabs are. MODE: how many of them one look at the page table gives (4: pages of whole blocks, 2: of pairs of
+// slabs), 0: a contiguous cache.
 struct Slab4 {
-    size_t block0, block1;  // first byte of the cache block of the first slab and (MODE 2) of the third
-    uint32_t slab0, slab1;
-    uint32_t bad;  // a bit for each slab whose page is none
+    size_t words0, words1, heads0, heads1;  // in the cache: of the first slab and (MODE 2) of the third
+    int rest;                               // MODE 0: slabs behind the first
+    uint32_t bad;                           // a bit for each slab whose page is none
 };
-// Slabs past the last key's: that one's page is read instead (their keys are masked).
-template <int MODE>
-__device__ __forceinline__ uint32_t look_up_page(const Map4 &M, int slot, int kvh, int slab, int last, size_t &block, uint32_t &at) {
+// Slabs past the last key's: that one's page (a contiguous cache: that one) is read instead; their keys are masked.
+template <int U, int MODE>
+__device__ __forceinline__ uint32_t look_up_page(const Map4 &M, int slot, int kvh, int slab, int last, size_t &words, size_t &heads) {
     const auto *pt = (const __attribute__((address_space(4))) int32_t *)(M.pt) + static_cast<size_t>(slot) * M.pps;
     const uint32_t want = min(slab, last & ~(MODE - 1)), p = static_cast<uint32_t>((static_cast<uint64_t>(want) * M.mul) >> M.shift);
     const int pg = pt[p];
     const bool none = static_cast<uint32_t>(pg) >= static_cast<uint32_t>(M.pages);
-    block = (static_cast<size_t>(none ? 0 : pg) * M.kv_heads + kvh) * M.bytes;
-    at = want - p * M.spp;
+    const size_t block = (static_cast<size_t>(none ? 0 : pg) * M.kv_heads + kvh) * M.bytes;
+    const uint32_t at = want - p * M.spp;
+    words = block + static_cast<size_t>(at) * (128 * U), heads = block + static_cast<size_t>(M.spp) * (128 * U) + static_cast<size_t>(at) * (16 * U);
     return none ? (1u << MODE) - 1 : 0u;
 }
-template <int MODE>
+template <int U, int MODE>
 __device__ __forceinline__ Slab4 look_up(const Map4 &M, int slot, int kvh, int kb, int last) {
     Slab4 r{};
+    const int slab = kb / kSlab;
     if constexpr (MODE == 0) {
-        r.block0 = static_cast<size_t>(kvh) * M.bytes;
-        r.slab0 = kb / kSlab;
+        const size_t block = static_cast<size_t>(kvh) * M.bytes;
+        r.words0 = block + static_cast<size_t>(slab) * (128 * U);
+        r.heads0 = block + static_cast<size_t>(M.spp) * (128 * U) + static_cast<size_t>(slab) * (16 * U);
+        r.rest = last - slab;
     } else {
-        r.bad = look_up_page<MODE>(M, slot, kvh, kb / kSlab, last, r.block0, r.slab0);
-        if constexpr (MODE == 2) {
-            r.bad |= look_up_page<MODE>(M, slot, kvh, kb / kSlab + 2, last, r.block1, r.slab1) << 2;
-        }
+        r.bad = look_up_page<U, MODE>(M, slot, kvh, slab, last, r.words0, r.heads0);
+        if constexpr (MODE == 2) r.bad |= look_up_page<U, MODE>(M, slot, kvh, slab + 2, last, r.words1, r.heads1) << 2;
     }
     return r;
 }
-// Slab i of the block, as a lane's own choice: (first byte of its block, slab in it).
-template <int MODE>
-__device__ __forceinline__ void choose(const Slab4 &s, int i, int last, size_t &block, uint32_t &slab) {
-    if constexpr (MODE == 0) {
-        block = s.block0, slab = min(s.slab0 + i, static_cast<uint32_t>(last));
-    } else if constexpr (MODE == 4) {
-        block = s.block0, slab = s.slab0 + i;
-    } else {
-        // Both are read, or the choice becomes one between their addresses, which puts them in memory.
-        const size_t b0 = s.block0, b1 = s.block1;
-        const uint32_t s0 = s.slab0, s1 = s.slab1;
-        block = i & 2 ? b1 : b0, slab = (i & 2 ? s1 : s0) + (i & 1);
+// The active lanes x 16 bytes from each lane's own address to LDS at (wave-uniform) dst + 16 lane. The second form: from a uniform
+// base and the lane's offset, which costs no vector instruction.
+__device__ __forceinline__ uint32_t lds_at(uint8_t *dst) {
+    return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(vq::lds_addr(dst))));
+}
+__device__ __forceinline__ void dma16(const uint8_t *from, uint8_t *dst) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds_at(dst)), "s"(dst) : "memory", "m0");
+}
+__device__ __forceinline__ void dma16(const uint8_t *base, uint32_t off, uint8_t *dst) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_at(dst)), "s"(dst) : "memory", "m0");
+}
+// Slab n's words begin at `key` 8 n. Its eight rows of 16 U bytes keep their order, but a row's pieces of 16 bytes (U / 2 for each of
+// a word's four g) change places by this, so that rows 8 a + 4 h + r (a, r < 4) and rows 16 a + r (r < 16) spread over the banks.
+template <int U>
+__device__ __forceinline__ int swizzle(int key) {
+    const int a = key >> 3 & 1, b = (key >> 2 ^ key >> 4) & 1;
+    return U == 8 ? (key >> 1 & 1) | a << 1 | b << 2 : a | b << 1;
+}
+// A DMA load brings 1024 bytes: a slab of hd 256, two of hd 128.
+template <int U, int MODE, bool K>
+__device__ __forceinline__ void dma_words(const uint8_t *cache, const Slab4 &at, uint8_t *words) {
+    const int lane = threadIdx.x & 63, slabs = 8 / U, sub = lane / (8 * U), piece = lane & (8 * U - 1);
+#pragma unroll
+    for (int x = 0; x < U / 2; ++x) {
+        const int n = x * slabs;
+        const int first = MODE == 0 ? min(n, at.rest) : n, step = MODE == 0 ? min(n + 1, at.rest) - first : 1;
+        const uint8_t *base = cache + (MODE == 2 && n >= 2 ? at.words1 + (n - 2) * (128 * U) : at.words0 + static_cast<size_t>(first) * (128 * U));
+        uint32_t off = 16 * piece;
+        if (K) {
+            const int row = piece / U, s = piece % U;
+            off = row * (16 * U) + 16 * (s ^ swizzle<U>(8 * (n + sub) + row));
+        }
+        dma16(base, off + sub * step * (128 * U), words + 1024 * x);
     }
 }
-// The active lanes x 16 bytes from each lane's own address to LDS at (wave-uniform) dst + 16 lane.
-__device__ __forceinline__ void dma16(const uint8_t *from, uint8_t *dst) {
-    const uint32_t at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(vq::lds_addr(dst))));
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at), "v"(dst) : "memory", "m0");
-}
-// Operand row c's pieces (eight of 16 bytes, two rows to the 64 banks) change places by this.
-__device__ __forceinline__ int k_swizzle(int c) { return c >> 1 & 7; }
 // The headers by lanes 0 to 31 (K's) and 32 to 63 (V's), or one of the two.
 template <int U, int MODE>
-__device__ __forceinline__ void dma_heads(const uint8_t *kc, const uint8_t *vc, const Map4 &M, const Slab4 &at, int last, uint8_t *to,
-                                          bool k, bool v) {
-    const int lane = threadIdx.x & 63, piece = min(lane & 31, 4 * U - 1);
-    size_t block;
-    uint32_t slab;
-    choose<MODE>(at, piece / U, last, block, slab);
-    if (k && v || (lane < 32) == k)
-        dma16((lane < 32 ? kc : vc) + block + static_cast<size_t>(M.spp) * (128 * U) + static_cast<size_t>(slab) * (16 * U) + piece % U * 16, to);
-}
-template <int U, int MODE>
-__device__ __forceinline__ void dma_k(const uint8_t *kc, const Map4 &M, const Slab4 &at, int last, uint8_t *part) {
-    const int lane = threadIdx.x & 63;
-    // hd 256: a load brings eight rows of 128 bytes whole, operand rows 8 x + r (x: the load's half of them), pieces swizzled so that
-    // the operand's reads spread over the banks. hd 128: a load brings the half's 16 rows of 64 bytes in operand order.
-    const int r = U == 8 ? lane >> 3 : lane & 15, s = U == 8 ? lane & 7 : lane >> 4;
-#pragma unroll
-    for (int x = 0; x < U / 4; ++x) {
-        size_t block;
-        uint32_t slab;
-        choose<MODE>(at, U == 8 ? 2 * x + (r >> 2) : r >> 2, last, block, slab);
-        const uint8_t *k = kc + block + static_cast<size_t>(slab) * (128 * U) + ((r & 3) * (16 * U) + (U == 8 ? s ^ k_swizzle(8 * x + r) : s) * 16);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) dma16(k + half * (64 * U), part + 1024 * (half * (U / 4) + x));
-    }
-}
-template <int U, int MODE>
-__device__ __forceinline__ void dma_v(const uint8_t *vc, const Map4 &M, const Slab4 &at, int last, uint8_t *part) {
-    const int lane = threadIdx.x & 63;
-    size_t block;
-    uint32_t slab;
-    choose<MODE>(at, lane >> 4, last, block, slab);
-    const uint8_t *v = vc + block + static_cast<size_t>(slab) * (128 * U) + (lane & 15) * 16;
-#pragma unroll
-    for (int i = 0; i < U / 2; ++i) dma16(v + 256 * i, part + 1024 * i);
+__device__ __forceinline__ void dma_heads(const uint8_t *kc, const uint8_t *vc, const Slab4 &at, uint8_t *to, bool k, bool v) {
+    const int lane = threadIdx.x & 63, piece = min(lane & 31, 4 * U - 1), n = piece / U;
+    const uint8_t *from = (lane < 32 ? kc : vc) + piece % U * 16;
+    // (Both are read, or the choice becomes one between their addresses, which puts them in memory.)
+    const size_t h0 = at.heads0, h1 = at.heads1;
+    if (MODE == 0) from += h0 + static_cast<size_t>(min(n, at.rest) * (16 * U));
+    if (MODE == 4) from += h0 + n * (16 * U);
+    if (MODE == 2) from += (n & 2 ? h1 : h0) + (n & 1) * (16 * U);
+    if ((k && v) || (lane < 32) == k) dma16(from, to);
 }
 template <int U>
 __device__ __forceinline__ void read_k(const uint8_t *words, const uint8_t *heads, Raw4<U> &r) {
@@ -636,8 +627,8 @@ __device__ __forceinline__ void read_k(const uint8_t *words, const uint8_t *head
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int i = 0; i < U / 4; ++i) {
-            const int at = U == 8 ? 128 * c + 16 * ((2 * g + i) ^ k_swizzle(c)) : 16 * lane;
-            const uint4 w = *reinterpret_cast<const uint4 *>(words + 256 * U * half + at);
+            const int key = 8 * (c >> 2) + 4 * half + (c & 3);
+            const uint4 w = *reinterpret_cast<const uint4 *>(words + (16 * U) * key + 16 * ((U / 4 * g + i) ^ swizzle<U>(key)));
             r.k[half][4 * i] = w.x, r.k[half][4 * i + 1] = w.y, r.k[half][4 * i + 2] = w.z, r.k[half][4 * i + 3] = w.w;
         }
         ld_words<U / 2>(heads + (8 * (c >> 2) + 4 * half + (c & 3)) * (2 * U), r.kh[half]);
@@ -648,7 +639,7 @@ __device__ __forceinline__ void read_v(const uint8_t *words, const uint8_t *head
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int i = 0; i < U / 2; ++i) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(words + 1024 * i + 16 * lane);
+        const uint4 w = *reinterpret_cast<const uint4 *>(words + (128 * U) * g + 256 * i + 16 * c);
         r.v[4 * i] = w.x, r.v[4 * i + 1] = w.y, r.v[4 * i + 2] = w.z, r.v[4 * i + 3] = w.w;
     }
     r.vh = *reinterpret_cast<const uint4 *>(heads + 16 * (g * U + min(c, U - 1)));
@@ -672,40 +663,43 @@ struct Query {
     fh8 h[kLds ? 1 : NT][kLds ? 1 : U], l[kLds ? 1 : NT][kLds ? 1 : U];
 };
 
-// The NT tiles' products of a block: K decoded once for all of them.
+// The NT tiles' products of a block: K decoded once for all of them. In steps of one word, each of which decodes the next one's while
+// the matrix unit works, and reads its queries ahead; left to itself the compiler waits for each.
 template <int U, int NT>
 __device__ __forceinline__ void scores(const Raw4<U> &r, const Query<U, NT> &q, const uint8_t *qlds, fa4 (&s)[NT][2]) {
     const int lane = threadIdx.x & 63;
-    fa4 a[2][NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = fa4{0.f, 0.f, 0.f, 0.f};
+    fh8 qb[2][NT][2], kb[2];
+    auto query = [&](int u) {
+        if constexpr (Query<U, NT>::kLds) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) a[h][n][0] = a[h][n][1] = fa4{0.f, 0.f, 0.f, 0.f};
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        fh8 qh[NT], ql[NT];
+                for (int x = 0; x < 2; ++x) qb[u & 1][n][x] = *reinterpret_cast<const fh8 *>(qlds + ((u * NT + n) * 2 + x) * 1024 + 16 * lane);
+        } else {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if constexpr (Query<U, NT>::kLds) {
-                qh[n] = *reinterpret_cast<const fh8 *>(qlds + ((u * NT + n) * 2) * 1024 + 16 * lane);
-                ql[n] = *reinterpret_cast<const fh8 *>(qlds + ((u * NT + n) * 2 + 1) * 1024 + 16 * lane);
-            } else {
-                qh[n] = q.h[n][u], ql[n] = q.l[n][u];
-            }
+            for (int n = 0; n < NT; ++n) qb[u & 1][n][0] = q.h[n][u], qb[u & 1][n][1] = q.l[n][u];
         }
+    };
+    auto key = [&](int i) {
+        const int u = i >> 1, h = i & 1;
+        kb[i & 1] = u % 2 == 0 ? decode8_one<false>(r.k[h][u], r.kh[h][u / 2]) : decode8_one<true>(r.k[h][u], r.kh[h][u / 2]);
+    };
+    query(0);
+    key(0);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const fh8 k = u % 2 == 0 ? decode8_one<false>(r.k[h][u], r.kh[h][u / 2]) : decode8_one<true>(r.k[h][u], r.kh[h][u / 2]);
+    for (int i = 0; i < 2 * U; ++i) {
+        const int u = i >> 1, h = i & 1;
+        if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
+        if (h == 0 && u + 1 < U) query(u + 1);
+        if (i + 1 < 2 * U) key(i + 1);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) a[h][n][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[n], a[h][n][0], 0, 0, 0);
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) a[h][n][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[n], a[h][n][1], 0, 0, 0);
-        }
+            for (int n = 0; n < NT; ++n) s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[i & 1], qb[u & 1][n][x], s[n][h], 0, 0, 0);
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[n][h] = a[h][n][0] + a[h][n][1];
+    if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
 }
 // O^T += V^T P^T. Every lane of a row of 16 needs the headers of all groups of its slab: lane c takes group c's apart and the others
 // read them from LDS (`hl`, the wave's own: [slab][group] scales, zero points; moving them by DPP costs 64 instructions a block of
@@ -727,20 +721,30 @@ __device__ __forceinline__ void add_values(const Raw4<U> &r, const fh8 (&ph)[NT]
     // A wave's LDS operations complete in order; the fence keeps the compiler from moving the reads above the writes.
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    uint4 dw[2], zw[2];
+    fh8 vb[2];
+    auto heads = [&](int u) {
+        dw[u & 1] = *reinterpret_cast<const uint4 *>(mine + 8 * u), zw[u & 1] = *reinterpret_cast<const uint4 *>(mine + 8 * u + 4);
+    };
+    auto value = [&](int b) {
+        const uint4 &x = dw[b >> 1 & 1], &y = zw[b >> 1 & 1];
+        const fh2 d[4] = {__builtin_bit_cast(fh2, x.x), __builtin_bit_cast(fh2, x.y), __builtin_bit_cast(fh2, x.z), __builtin_bit_cast(fh2, x.w)};
+        const fh2 z[4] = {__builtin_bit_cast(fh2, y.x), __builtin_bit_cast(fh2, y.y), __builtin_bit_cast(fh2, y.z), __builtin_bit_cast(fh2, y.w)};
+        vb[b & 1] = decode8(r.v[b], d, z);
+    };
+    heads(0);
+    value(0);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint4 dw = *reinterpret_cast<const uint4 *>(mine + 8 * u), zw = *reinterpret_cast<const uint4 *>(mine + 8 * u + 4);
-        const fh2 d[4] = {__builtin_bit_cast(fh2, dw.x), __builtin_bit_cast(fh2, dw.y), __builtin_bit_cast(fh2, dw.z), __builtin_bit_cast(fh2, dw.w)};
-        const fh2 z[4] = {__builtin_bit_cast(fh2, zw.x), __builtin_bit_cast(fh2, zw.y), __builtin_bit_cast(fh2, zw.z), __builtin_bit_cast(fh2, zw.w)};
+    for (int b = 0; b < 2 * U; ++b) {
+        if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
+        if (b % 2 == 0 && b + 2 < 2 * U) heads(b / 2 + 1);
+        if (b + 1 < 2 * U) value(b + 1);
 #pragma unroll
-        for (int b = 2 * u; b < 2 * u + 2; ++b) {
-            const fh8 a = decode8(r.v[b], d, z);
+        for (int n = 0; n < NT; ++n) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[b & 1], ph[n], o[n][b], 0, 0, 0);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[n], o[n][b], 0, 0, 0);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[n], o[n][b], 0, 0, 0);
-        }
+        for (int n = 0; n < NT; ++n) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[b & 1], pl[n], o[n][b], 0, 0, 0);
     }
+    if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");  // every lane has read before the next block's writes
     __builtin_amdgcn_wave_barrier();
 }
@@ -769,14 +773,26 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
     __shared__ float sm[4][2][16], sl[4][2][16];
     __shared__ __align__(16) uint32_t vheads[4][head_words<U>];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x % M.kv_heads, list = blockIdx.x / M.kv_heads;
     const int bases = C.base[lane];
-    const Found found = find_segment(T, C.first, C.total, list);
+    const Found found = find_segment(T, C.first, C.total, blockIdx.x / M.kv_heads);
     const Seg s = found.s;
-    const int G = heads / M.kv_heads, nvec = s.rows * G, units = found.next - found.first, at = list - found.first;
-    // One tile holds a segment's vectors whole. Of several groups the last rows, which see the most keys, come first.
+    const int G = heads / M.kv_heads, nvec = s.rows * G, units = found.next - found.first;
+    // A segment's kv heads x chunks x groups. One tile holds its vectors whole; of several groups (the last rows, which see the most
+    // keys, first) those of a head and chunk go to one XCD, for its L2: eight heads and chunks at a time, then the rest.
+    const int at = blockIdx.x - found.first * M.kv_heads;
     const int groups = NT == 1 ? 1 : (nvec + 16 * NT - 1) / (16 * NT), n = NT == 1 ? units : units / groups;
-    const int ci = NT == 1 ? at : at % n, j0 = NT == 1 ? 0 : (groups - 1 - at / n) * 16 * NT;
+    int stream = at, group = 0;
+    if (NT != 1) {
+        const int streams = n * M.kv_heads, rest = streams & 7, eights = (streams - rest) * groups;
+        if (at < eights) {
+            const int block = at / (8 * groups), x = at - block * 8 * groups;
+            group = x >> 3, stream = 8 * block + (x & 7);
+        } else {
+            group = (at - eights) / rest, stream = streams - rest + (at - eights) - group * rest;
+        }
+        group = groups - 1 - group;
+    }
+    const int ci = stream / M.kv_heads, kvh = stream - ci * M.kv_heads, j0 = group * 16 * NT;
     const Sees lo = sees(s, NT == 1 ? 0 : j0 / G, bidirectional, window);
     const Sees hi = sees(s, NT == 1 ? s.rows - 1 : min(j0 + 16 * NT - 1, nvec - 1) / G, bidirectional, window);
     const int c_lo = first_key(s, window) + ci * C.len;
@@ -794,12 +810,12 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
     };
     auto fetch = [&](int block, int slot) {
         if constexpr (DMA) {
-            const Slab4 where = look_up<MODE>(M, s.slot, kvh, block, last);
+            const Slab4 where = look_up<U, MODE>(M, s.slot, kvh, block, last);
             uint8_t *const to = ring + slot * BYTES;
-            dma_k<U, MODE>(kc, M, where, last, to);
-            if constexpr (SPLIT) dma_heads<U, MODE>(kc, vc, M, where, last, to + 2 * WORDS, true, false);
-            dma_v<U, MODE>(vc, M, where, last, to + WORDS);
-            dma_heads<U, MODE>(kc, vc, M, where, last, to + 2 * WORDS, !SPLIT, true);
+            dma_words<U, MODE, true>(kc, where, to);
+            if constexpr (SPLIT) dma_heads<U, MODE>(kc, vc, where, to + 2 * WORDS, true, false);
+            dma_words<U, MODE, false>(vc, where, to + WORDS);
+            dma_heads<U, MODE>(kc, vc, where, to + 2 * WORDS, !SPLIT, true);
             bad = (bad & ~(15u << 4 * slot)) | where.bad << 4 * slot;
         } else {
             places(block);
@@ -869,7 +885,7 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
             if constexpr (DMA) {
                 // Landed: all but this block's V and the blocks behind it. The page of the block that comes into the slot meanwhile.
                 wait_loads(SPLIT ? LD : LD * min(left, S - 1));
-                if (SPLIT && more) where = look_up<MODE>(M, s.slot, kvh, kb + 128 * S, last);
+                if (SPLIT && more) where = look_up<U, MODE>(M, s.slot, kvh, kb + 128 * S, last);
                 read_k<U>(from, from + 2 * WORDS, r);
                 if (MODE != 0 && bad != 0 && (bad >> (4 * slot + (c >> 2)) & 1)) no_page<U>(r);
             } else {
@@ -880,8 +896,8 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
             if (more) {
                 if constexpr (SPLIT) {
                     vq::wait_lgkm0();  // the part has been read
-                    dma_k<U, MODE>(kc, M, where, last, from);
-                    dma_heads<U, MODE>(kc, vc, M, where, last, from + 2 * WORDS, true, false);
+                    dma_words<U, MODE, true>(kc, where, from);
+                    dma_heads<U, MODE>(kc, vc, where, from + 2 * WORDS, true, false);
                     bad = (bad & ~(15u << 4 * slot)) | where.bad << 4 * slot;
                 } else if constexpr (!DMA) {
                     issue_k<U>(kc, ks, r);
@@ -899,8 +915,8 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
                 if constexpr (DMA) {
                     vq::wait_lgkm0();
                     if constexpr (SPLIT) {
-                        dma_v<U, MODE>(vc, M, where, last, from + WORDS);
-                        dma_heads<U, MODE>(kc, vc, M, where, last, from + 2 * WORDS, false, true);
+                        dma_words<U, MODE, false>(vc, where, from + WORDS);
+                        dma_heads<U, MODE>(kc, vc, where, from + 2 * WORDS, false, true);
                     } else {
                         fetch(kb + 128 * S, slot);
                     }
@@ -965,10 +981,69 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
     }
 }
 
+// A row's chunks: [lo, hi) of n hold its keys; the part of (row, head, chunk) is at `at` + head n + chunk.
+struct RowChunks {
+    int t, n, lo, hi;
+    size_t at;
+};
+template <int NT>
+__device__ __forceinline__ RowChunks row_chunks(const Found &found, const SegTable &T, const Cuts &C, int chunks, int bases, int row, int heads, int G,
+                                                int bidirectional, int window) {
+    const Seg s = found.s;
+    const int i = found.index, t = row - found.first;
+    const int units = (i + 1 < T.n ? from_lane(chunks, i + 1 < 64 ? i + 1 : 63) : C.total) - from_lane(chunks, i);
+    RowChunks r{t, NT == 1 ? units : units / ((s.rows * G + 16 * NT - 1) / (16 * NT)), 0, 0, 0};
+    r.hi = r.n;
+    if (NT != 1) {  // (one tile: every chunk has been written)
+        const Sees see = sees(s, t, bidirectional, window);
+        const int k0 = first_key(s, window);
+        r.lo = (see.from - k0) / C.len, r.hi = min((see.to - 1 - k0) / C.len + 1, r.n);
+    }
+    r.at = static_cast<size_t>(from_lane(bases, i)) + static_cast<size_t>(t) * heads * r.n;
+    return r;
+}
+// sum_c 2^(m_c - m) o_c and sum_c 2^(m_c - m) l_c over chunks lo, lo + step, ..: four of them in flight, under a running maximum.
+// `o`: these dims of chunk 0's part, `ml`: its maximum and sum.
+template <int HD>
+__device__ __forceinline__ float4 merge_parts(const float *o, const float *ml, int lo, int hi, int step, float &m, float &L) {
+    m = -INFINITY, L = 0.0f;
+    float4 acc{0.f, 0.f, 0.f, 0.f};
+    for (int c0 = lo; c0 < hi; c0 += 4 * step) {
+        float4 p[4];
+        float mc[4], lc[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int c = c0 + step * k < hi ? c0 + step * k : c0;
+            p[k] = *reinterpret_cast<const float4 *>(o + static_cast<size_t>(c) * HD);
+            mc[k] = c0 + step * k < hi ? ml[2 * c] : -INFINITY;
+            lc[k] = ml[2 * c + 1];
+        }
+        const float mn = fmaxf(fmaxf(m, fmaxf(mc[0], mc[1])), fmaxf(mc[2], mc[3])), f0 = share(m, mn);
+        m = mn;
+        L *= f0;
+        acc = float4{acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (c0 + step * k >= hi) break;
+            const float f = share(mc[k], mn);
+            L = fmaf(lc[k], f, L);
+            acc.x = fmaf(p[k].x, f, acc.x);
+            acc.y = fmaf(p[k].y, f, acc.y);
+            acc.z = fmaf(p[k].z, f, acc.z);
+            acc.w = fmaf(p[k].w, f, acc.w);
+        }
+    }
+    return acc;
+}
+__device__ __forceinline__ void put_merged(float *to, const float4 &acc, float L) {
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    const float4 r{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+    __builtin_memcpy(to, &r, 16);
+}
+
 // out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, for segments of more than one. It is latency that this
 // kernel spends, so a workgroup takes 64 dims of a (row, head) (32 where hd is no multiple of 64), a thread four dims of every 16th
-// (32nd) chunk, four of them in flight, under a running maximum; the 16 (32) sums meet in order. 24 rows of 128 chunks, hd 256: 4 us;
-// one workgroup of four waves for a row took 11.
+// (32nd) chunk; the 16 (32) sums meet in order. 24 rows of 128 chunks, hd 256: 4 us; one workgroup of four waves for a row took 11.
 template <int HD, int NT>
 __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
                                                                float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads,
@@ -980,48 +1055,11 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
     const int row = blockIdx.x / heads, h = blockIdx.x - row * heads, d = 4 * (Q * blockIdx.y + quad);
     const int chunks = C.first[lane], bases = C.base[lane];
     const Found found = find_segment(T, R.first, R.total, row);
-    const Seg s = found.s;
-    const int t = row - found.first, i = found.index;
-    const int units = (i + 1 < T.n ? from_lane(chunks, i + 1 < 64 ? i + 1 : 63) : C.total) - from_lane(chunks, i);
-    const int n = NT == 1 ? units : units / ((s.rows * G + 16 * NT - 1) / (16 * NT));
-    if (n == 1) return;
-    // One tile: every chunk has been written. Several groups: those that hold keys of this row.
-    int c_lo = 0, c_hi = n;
-    if (NT != 1) {
-        const Sees see = sees(s, t, bidirectional, window);
-        const int k0 = first_key(s, window);
-        c_lo = (see.from - k0) / C.len, c_hi = min((see.to - 1 - k0) / C.len + 1, n);
-    }
-    const size_t at = static_cast<size_t>(from_lane(bases, i)) + (static_cast<size_t>(t) * heads + h) * n;
-    const float *ml = pml + 2 * at;
-    float m = -INFINITY, L = 0.0f;
-    float4 acc{0.f, 0.f, 0.f, 0.f};
-    auto scale = [](float x, float to) { return x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x - to); };
-    for (int c0 = c_lo + grp; c0 < c_hi; c0 += 4 * GROUPS) {
-        float4 p[4];
-        float mc[4], lc[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int c = c0 + GROUPS * k < c_hi ? c0 + GROUPS * k : c0;
-            p[k] = *reinterpret_cast<const float4 *>(part + (at + c) * HD + d);
-            mc[k] = c0 + GROUPS * k < c_hi ? ml[2 * c] : -INFINITY;
-            lc[k] = ml[2 * c + 1];
-        }
-        const float mn = fmaxf(fmaxf(m, fmaxf(mc[0], mc[1])), fmaxf(mc[2], mc[3])), f0 = scale(m, mn);
-        m = mn;
-        L *= f0;
-        acc = float4{acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (c0 + GROUPS * k >= c_hi) break;
-            const float f = scale(mc[k], mn);
-            L = fmaf(lc[k], f, L);
-            acc.x = fmaf(p[k].x, f, acc.x);
-            acc.y = fmaf(p[k].y, f, acc.y);
-            acc.z = fmaf(p[k].z, f, acc.z);
-            acc.w = fmaf(p[k].w, f, acc.w);
-        }
-    }
+    const RowChunks r = row_chunks<NT>(found, T, C, chunks, bases, row, heads, G, bidirectional, window);
+    if (r.n == 1) return;
+    const size_t at = r.at + static_cast<size_t>(h) * r.n;
+    float m, L;
+    float4 acc = merge_parts<HD>(part + at * HD + d, pml + 2 * at, r.lo + grp, r.hi, GROUPS, m, L);
     sacc[grp][quad] = acc;
     if (quad == 0) sm[grp] = m, sl[grp] = L;
     __syncthreads();
@@ -1034,16 +1072,31 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
 #pragma unroll
     for (int w = 0; w < GROUPS; ++w) {
         const float4 a = sacc[w][quad];
-        const float f = scale(sm[w], m);
+        const float f = share(sm[w], m);
         L = fmaf(sl[w], f, L);
         acc.x = fmaf(a.x, f, acc.x);
         acc.y = fmaf(a.y, f, acc.y);
         acc.z = fmaf(a.z, f, acc.z);
         acc.w = fmaf(a.w, f, acc.w);
     }
-    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    const float4 r{acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-    __builtin_memcpy(out + (static_cast<size_t>(s.row0 + t) * heads + h) * HD + d, &r, 16);
+    put_merged(out + (static_cast<size_t>(found.s.row0 + r.t) * heads + h) * HD + d, acc, L);
+}
+// The same for up to kFewChunks chunks: a thread takes four dims of a head, workgroups (row, 1024 values of it).
+constexpr int kFewChunks = 8;
+template <int HD, int NT>
+__global__ __launch_bounds__(256) void attention4_merge_few_kernel(const float *__restrict__ part, const float *__restrict__ pml,
+                                                                   float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads,
+                                                                   int G, int bidirectional, int window) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x;
+    const int chunks = C.first[lane], bases = C.base[lane];
+    const Found found = find_segment(T, R.first, R.total, row);
+    const RowChunks r = row_chunks<NT>(found, T, C, chunks, bases, row, heads, G, bidirectional, window);
+    const int e = blockIdx.y * 256 + threadIdx.x, h = e / (HD / 4), d = 4 * (e - h * (HD / 4));
+    if (r.n == 1 || h >= heads) return;
+    const size_t at = r.at + static_cast<size_t>(h) * r.n;
+    float m, L;
+    const float4 acc = merge_parts<HD>(part + at * HD + d, pml + 2 * at, r.lo, r.hi, 1, m, L);
+    put_merged(out + (static_cast<size_t>(found.s.row0 + r.t) * heads + h) * HD + d, acc, L);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------
@@ -1154,7 +1207,7 @@ Cuts make_cuts(const SegTable &T, const Shape &P, int window, bool whole) {
     }
     Cuts C;
     C.len = static_cast<int>(best);
-    C.total = 0;
+    C.total = C.most = 0;
     int base = 0;
     for (int i = 0; i < VQ_MAX_SEGMENTS; ++i) {
         C.first[i] = C.total;
@@ -1163,6 +1216,7 @@ Cuts make_cuts(const SegTable &T, const Shape &P, int window, bool whole) {
         const int n = chunks_of(T.s[i], C.len, window);
         if (n > 1) base += n * T.s[i].rows * P.heads;
         C.total += n * P.groups(T.s[i]);
+        C.most = max(C.most, n);
     }
     return C;
 }
@@ -1228,9 +1282,11 @@ int launch_attention4(const float *q, const void *kc, const void *vc, float *out
         if (!done && M.pt) go(attention4_kernel<U, NT, -1>);
         if constexpr (U % 4 != 0)
             if (!M.pt) go(attention4_kernel<U, NT, -2>);
-        if (parts)
-            attention4_merge_kernel<32 * U, NT><<<dim3(T.total * heads, U % 2 == 0 ? U / 2 : U), 256, 0, s>>>(part, pml, out, T, C, R, heads,
-                                                                                                          heads / M.kv_heads, bidirectional, window);
+        auto merge = [&](auto kernel, const dim3 &rows) {
+            kernel<<<rows, 256, 0, s>>>(part, pml, out, T, C, R, heads, heads / M.kv_heads, bidirectional, window);
+        };
+        if (parts && C.most > kFewChunks) merge(attention4_merge_kernel<32 * U, NT>, dim3(T.total * heads, U % 2 == 0 ? U / 2 : U));
+        else if (parts) merge(attention4_merge_few_kernel<32 * U, NT>, dim3(T.total, (heads * 8 * U + 255) / 256));
     };
     for_hd(hd, [&](auto u) {
         if (P.tiles == 1) pass(u, std::integral_constant<int, 1>{});
