@@ -339,89 +339,58 @@ __device__ __forceinline__ SlabAt slab_at(const Map4 &M, int slot, int kvh, int 
                   p.bad};
 }
 
-// Operand layout of v_mfma_f32_16x16x32_f16: lane l = (c = l & 15, g = l >> 4) gives row c of A and column c of B at the same eight
-// k slots (g, j); the result has rows 4 g + r, column c. Over a block of 32 keys:
-//  - S^T of key half h: A row c is key 8 (c >> 2) + 4 h + (c & 3), dims 32 u + 8 g + j (one K word); lane (c, g) ends with the
-//    scores of keys 8 g + 4 h + r of query vector c.
-//  - O^T += V^T P^T: k slot (g, j) is key 8 g + j, so B is the lane's own eight weights in order and A, dims 16 b + c of V^T at
-//    positions 8 g .. 8 g + 7, is one V word of slab g.
-
-// The lane's query vector (column c, dims 32 u + 8 g + j) as B operands: times a power of two that brings its largest element near
-// 2^14, as f16 pairs hi + lo (22 significant bits). Returns the factor that takes a product back and into base-2 units of the
-// softmax, log2(e) / sqrt(hd) over that power. 230 instructions: a short context's workgroup runs this once for a block or two.
 __device__ __forceinline__ float max3_abs(float m, float a, float b) {
     asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(m) : "v"(m), "v"(a), "v"(b));
     return m;
 }
+// A query vector goes in as f16 pairs hi + lo (22 significant bits) of its elements times a power of two that brings the largest,
+// `amax`, near 2^14. Returns that power; `unit` takes a product back and into base-2 units of the softmax, log2(e) / sqrt(hd) over it.
 template <int U>
-__device__ __forceinline__ float load_query(const float *qrow, fh8 (&qh)[U], fh8 (&ql)[U]) {
-    const int g = (threadIdx.x & 63) >> 4;
-    float x[U][8], amax = 0.0f;
-#pragma unroll
-    for (int u = 0; u < U; ++u) __builtin_memcpy(x[u], qrow + 32 * u + 8 * g, 32);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) amax = max3_abs(amax, x[u][j], x[u][j + 1]);
-    amax = xor32_max(xor16_max(amax));
+__device__ __forceinline__ float query_scale(float amax, float &unit) {
     // amax = f 2^ex, f in [0.5, 1). Capped at 2^126, so that the power and its inverse are finite for the smallest queries.
     const int ex = amax > 0.0f && amax <= 3.0e38f ? __builtin_amdgcn_frexp_expf(amax) : 0, e2 = 14 - ex < 126 ? 14 - ex : 126;
-    const float up = ldexpf(1.0f, e2);
+    unit = ldexpf(1.44269504088896341f / sqrtf(32.0f * U), -e2);
+    return ldexpf(1.0f, e2);
+}
+__device__ __forceinline__ void split_query(const float (&x)[8], float up, fh8 &h, fh8 &l) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            _Float16 hi, lo;
-            split_h(x[u][j] * up, hi, lo);
-            qh[u][j] = hi;
-            ql[u][j] = lo;
-        }
-    return ldexpf(1.44269504088896341f / sqrtf(32.0f * U), -e2);
+    for (int j = 0; j < 8; ++j) {
+        _Float16 hi, lo;
+        split_h(x[j] * up, hi, lo);
+        h[j] = hi;
+        l[j] = lo;
+    }
 }
 
-// Softmax step over a block's products s[h][r] (key kb + 8 g + 4 h + r; keys outside [qs, qe) are masked), which times `unit` are
-// scores in base-2 units: new running maximum and sum, O rescaled where the maximum moved, the weights as an f16 pair (the first
-// half rounded towards zero, the second the rest: 22 significant bits). The sum is of the weights before they are split.
-template <int U>
-__device__ __forceinline__ void softmax_step(const fa4 (&s)[2], float unit, int kb, int qs, int qe, float &m, float &l, fa4 (&o)[2 * U],
-                                             fh8 &ph, fh8 &pl) {
-    const int g = (threadIdx.x & 63) >> 4;
-    float v[8], bm = -INFINITY;
+// Softmax step over a lane's N products s of a block (masked ones are -inf), which times `unit` are scores in base-2 units: new
+// running maximum and sum, the factor for what was summed before, the weights as f16 pairs (the first half rounded towards zero, the
+// second the rest: 22 significant bits). The sum is of the weights before they are split. `across`: over the lanes of a vector.
+template <int N, typename Max, typename Add>
+__device__ __forceinline__ float softmax_step(const float (&v)[N], float unit, float &m, float &l, fh8 (&ph)[N / 8], fh8 (&pl)[N / 8], Max max_across,
+                                              Add add_across) {
+    float bm = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = s[j >> 2][j & 3];
-    if (__any(kb < qs || kb + 32 > qe)) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int p = kb + 8 * g + j;
-            v[j] = p >= qs && p < qe ? v[j] : -INFINITY;
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) bm = fmaxf(bm, v[j]);
-    bm = xor32_max(xor16_max(bm)) * unit;
+    for (int j = 0; j < N; ++j) bm = fmaxf(bm, v[j]);
+    bm = max_across(bm) * unit;
     const float mn = fmaxf(m, bm), ms = mn == -INFINITY ? 0.0f : mn;  // ms: exp2(-inf - ms) is 0 also before any key
     const float alpha = __builtin_amdgcn_exp2f(m - ms);
     float ps = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
+    for (int j = 0; j < N; j += 2) {
         const float a = __builtin_amdgcn_exp2f(fmaf(v[j], unit, -ms)), b = __builtin_amdgcn_exp2f(fmaf(v[j + 1], unit, -ms));
         ps += a;
         ps += b;
         const fh2 hi = __builtin_bit_cast(fh2, __builtin_amdgcn_cvt_pkrtz(a, b));
         const fh2 lo = __builtin_bit_cast(fh2, __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(hi[0]), b - static_cast<float>(hi[1])));
-        ph[j] = hi[0], ph[j + 1] = hi[1];
-        pl[j] = lo[0], pl[j + 1] = lo[1];
+        ph[j / 8][j % 8] = hi[0], ph[j / 8][j % 8 + 1] = hi[1];
+        pl[j / 8][j % 8] = lo[0], pl[j / 8][j % 8 + 1] = lo[1];
     }
-    ps = xor32_add(xor16_add(ps));
-    l = l * alpha + ps;
+    l = l * alpha + add_across(ps);
     m = mn;
-    if (__any(alpha != 1.0f)) {
-#pragma unroll
-        for (int b = 0; b < 2 * U; ++b) o[b] *= alpha;
-    }
+    return alpha;
 }
 
-// How a pass is cut: each segment's query vectors in groups of 16 NT, its keys in chunks of `len` (a multiple of 128) from its first
+// How a pass is cut: each segment's query vectors in groups of 16 or 32, its keys in chunks of `len` (a multiple of 128) from its first
 // key rounded down to 32; segment i's groups x chunks begin at first[i] of one list, its partial results at base[i] (where it has
 // more than one chunk).
 struct Cuts {
@@ -464,68 +433,6 @@ struct Dest {
 // A sum's share against maximum m where it was kept against `own`.
 __device__ __forceinline__ float share(float own, float m) { return own == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(own - m); }
 
-// Four waves' sums of 16 vectors (each wave's [16][HD], maxima and totals) meet in wave order.
-template <int HD>
-__device__ __forceinline__ void meet4(const float *sums, const float (&sm)[4][2][16], const float (&sl)[4][2][16], int j0, const Dest &to) {
-    for (int e = threadIdx.x; e < 16 * (HD / 4); e += 256) {
-        const int c = e / (HD / 4), d4 = 4 * (e - c * (HD / 4));
-        if (j0 + c >= to.nvec) continue;
-        const float mx = fmaxf(fmaxf(sm[0][0][c], sm[1][0][c]), fmaxf(sm[2][0][c], sm[3][0][c]));
-        float L = 0.0f;
-        float4 acc{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = share(sm[w][0][c], mx);
-            L = fmaf(sl[w][0][c], f, L);
-            const float4 p = *reinterpret_cast<const float4 *>(sums + (w * 16 + c) * HD + d4);
-            acc.x = fmaf(p.x, f, acc.x);
-            acc.y = fmaf(p.y, f, acc.y);
-            acc.z = fmaf(p.z, f, acc.z);
-            acc.w = fmaf(p.w, f, acc.w);
-        }
-        to.put<HD>(j0 + c, d4, acc, mx, L);
-    }
-}
-
-// A block's codes and headers in registers. Lane (c, g) has K rows 8 (c >> 2) + 4 h + (c & 3) at its dims, the V words of its dims in
-// slab g, and of slab g the headers of group c.
-template <int U>
-struct Raw4 {
-    uint32_t k[2][U], kh[2][(U + 1) / 2], v[2 * U];
-    uint4 vh;
-};
-template <int U>
-__device__ __forceinline__ void no_page(Raw4<U> &r) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < (U + 1) / 2; ++i) r.kh[h][i] = kNanHeader | kNanHeader << 16;
-}
-template <int U>
-__device__ __forceinline__ void issue_k(const uint8_t *__restrict__ kc, const SlabAt &at, Raw4<U> &r) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int row = 4 * h + (c & 3);
-        ld_words<U>(kc + at.words + row * (16 * U) + g * (4 * U), r.k[h]);
-        ld_heads<U>(kc + at.heads + row * (2 * U), r.kh[h]);
-    }
-    if (at.bad) no_page<U>(r);
-}
-template <int U>
-__device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, const SlabAt &at, Raw4<U> &r) {
-    const int c = threadIdx.x & 15;
-    constexpr int W = U % 2 == 0 ? 4 : 2;
-#pragma unroll
-    for (int i = 0; i < 2 * U / W; ++i) {
-        uint32_t w[W];
-        ld_words<W>(vc + at.words + (16 * i + c) * (4 * W), w);
-#pragma unroll
-        for (int k = 0; k < W; ++k) r.v[W * i + k] = w[k];
-    }
-    r.vh = *reinterpret_cast<const uint4 *>(vc + at.heads + 16 * min(c, U - 1));
-}
-
 // ---- blocks by DMA ----
 
 // For hd 128 and 256, whose waves are few (hd 256: 2 per SIMD, for the registers of O and q): the blocks come to LDS by DMA, kSlots of
@@ -533,9 +440,9 @@ __device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, const Sl
 // slot is K's words, slab after slab, V's words, and 512 bytes each of K's and of V's headers, slab after slab. Page ids and
 // addresses are wave-uniform and come by scalar loads: the only vector memory operations of the loop are the DMA's, which the waits
 // count.
-template <int U, int NT>
+template <int U, int VECS>
 struct Ring {
-    static constexpr int kSlots = U == 8 ? (NT == 1 ? 2 : 1) : (NT == 1 ? 3 : 2);
+    static constexpr int kSlots = (U == 8 ? 2 : 3) - (VECS == 32);
     static constexpr int kWords = 512 * U, kBytes = 2 * kWords + 1024;
     static constexpr int kLoads = kSlots == 1 ? U / 2 + 1 : U + 1;  // of half a slot that is filled by halves, or of a slot
 };
@@ -620,30 +527,6 @@ __device__ __forceinline__ void dma_heads(const uint8_t *kc, const uint8_t *vc, 
     if (MODE == 2) from += (n & 2 ? h1 : h0) + (n & 1) * (16 * U);
     if ((k && v) || (lane < 32) == k) dma16(from, to);
 }
-template <int U>
-__device__ __forceinline__ void read_k(const uint8_t *words, const uint8_t *heads, Raw4<U> &r) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int i = 0; i < U / 4; ++i) {
-            const int key = 8 * (c >> 2) + 4 * half + (c & 3);
-            const uint4 w = *reinterpret_cast<const uint4 *>(words + (16 * U) * key + 16 * ((U / 4 * g + i) ^ swizzle<U>(key)));
-            r.k[half][4 * i] = w.x, r.k[half][4 * i + 1] = w.y, r.k[half][4 * i + 2] = w.z, r.k[half][4 * i + 3] = w.w;
-        }
-        ld_words<U / 2>(heads + (8 * (c >> 2) + 4 * half + (c & 3)) * (2 * U), r.kh[half]);
-    }
-}
-template <int U>
-__device__ __forceinline__ void read_v(const uint8_t *words, const uint8_t *heads, Raw4<U> &r) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int i = 0; i < U / 2; ++i) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(words + (128 * U) * g + 256 * i + 16 * c);
-        r.v[4 * i] = w.x, r.v[4 * i + 1] = w.y, r.v[4 * i + 2] = w.z, r.v[4 * i + 3] = w.w;
-    }
-    r.vh = *reinterpret_cast<const uint4 *>(heads + 16 * (g * U + min(c, U - 1)));
-}
 // At most N loads outstanding, for the few N that occur.
 __device__ __forceinline__ void wait_loads(int n) {
     switch (n) {
@@ -654,135 +537,505 @@ __device__ __forceinline__ void wait_loads(int n) {
     }
 }
 
-// ---- the products ----
+// ---- a wave's tile of query vectors: 16 or 32 ----
 
-// Query operands of NT tiles: in registers, or (more than 8 operand steps) in LDS, [u][tile][hi, lo][lane].
-template <int U, int NT>
-struct Query {
-    static constexpr bool kLds = NT * U > 8;
-    fh8 h[kLds ? 1 : NT][kLds ? 1 : U], l[kLds ? 1 : NT][kLds ? 1 : U];
+// Every lane needs the headers of all groups of its V slabs: 4 U lanes take a slab's group apart each and the others read them from
+// LDS ([slab][group] scales, zero points, the wave's own; moving them by DPP costs 64 instructions a block of the kind that bounds
+// this kernel).
+template <int U>
+constexpr int head_words = 4 * (8 * U + 8);
+struct Heads2 {
+    fh2 d[4], z[4];
+};
+__device__ __forceinline__ void put_heads(const uint4 &raw, uint32_t *to) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t d[4], z[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = w[i] & 0xFFF0FFF0u, z[i] = __builtin_bit_cast(uint32_t, zeros2(w[i], i % 2 != 0));
+    *reinterpret_cast<uint4 *>(to) = uint4{d[0], d[1], d[2], d[3]};
+    *reinterpret_cast<uint4 *>(to + 4) = uint4{z[0], z[1], z[2], z[3]};
+}
+__device__ __forceinline__ Heads2 get_heads(const uint32_t *from) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(from), y = *reinterpret_cast<const uint4 *>(from + 4);
+    return Heads2{{__builtin_bit_cast(fh2, x.x), __builtin_bit_cast(fh2, x.y), __builtin_bit_cast(fh2, x.z), __builtin_bit_cast(fh2, x.w)},
+                  {__builtin_bit_cast(fh2, y.x), __builtin_bit_cast(fh2, y.y), __builtin_bit_cast(fh2, y.z), __builtin_bit_cast(fh2, y.w)}};
+}
+// A wave's LDS operations complete in order; the fence keeps the compiler from moving them over each other.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// 16 vectors by v_mfma_f32_16x16x32_f16: lane l = (c = l & 15, g = l >> 4) gives row c of A and column c of B at the same eight k
+// slots (g, j); the result has rows 4 g + r, column c. Over a block of 32 keys:
+//  - S^T of key half h: A row c is key 8 (c >> 2) + 4 h + (c & 3), dims 32 u + 8 g + j (one K word); lane (c, g) ends with the
+//    scores of keys 8 g + 4 h + r of query vector c.
+//  - O^T += V^T P^T: k slot (g, j) is key 8 g + j, so B is the lane's own eight weights in order and A, dims 16 b + c of V^T at
+//    positions 8 g .. 8 g + 7, is one V word of slab g.
+template <int U>
+struct Tile16 {
+    static constexpr int kVecs = 16, kQueryLds = 0;
+    uint32_t k[2][U], kh[2][(U + 1) / 2], v[2 * U];
+    uint4 vh;
+    fh8 qh[U], ql[U];
+    float unit, m, l;
+    fa4 o[2 * U];
+
+    static __device__ __forceinline__ int lane() { return threadIdx.x & 63; }
+    static __device__ __forceinline__ int vec() { return lane() & 15; }
+    static __device__ __forceinline__ int key(int h) { return 8 * (vec() >> 2) + 4 * h + (vec() & 3); }
+    static __device__ __forceinline__ int kslab() { return vec() >> 2; }
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int b = 0; b < 2 * U; ++b) o[b] = fa4{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void no_page() {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < (U + 1) / 2; ++i) kh[h][i] = kNanHeader | kNanHeader << 16;
+    }
+    // 230 instructions at hd 256: a short context's workgroup runs this once for a block or two.
+    __device__ __forceinline__ void load_query(const float *qrow, uint8_t *) {
+        const int g = lane() >> 4;
+        float x[U][8], amax = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) __builtin_memcpy(x[u], qrow + 32 * u + 8 * g, 32);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) amax = max3_abs(amax, x[u][j], x[u][j + 1]);
+        const float up = query_scale<U>(xor32_max(xor16_max(amax)), unit);
+#pragma unroll
+        for (int u = 0; u < U; ++u) split_query(x[u], up, qh[u], ql[u]);
+    }
+    // From the cache: `at(slab)` is the place of a slab of the block.
+    template <typename At>
+    __device__ __forceinline__ void issue_k(const uint8_t *__restrict__ kc, At at) {
+        const SlabAt p = at(kslab());
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = key(h) & 7;
+            ld_words<U>(kc + p.words + row * (16 * U) + (lane() >> 4) * (4 * U), k[h]);
+            ld_heads<U>(kc + p.heads + row * (2 * U), kh[h]);
+        }
+        if (p.bad) no_page();
+    }
+    template <typename At>
+    __device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, At at) {
+        constexpr int W = U % 2 == 0 ? 4 : 2;
+        const SlabAt p = at(lane() >> 4);
+#pragma unroll
+        for (int i = 0; i < 2 * U / W; ++i) {
+            uint32_t w[W];
+            ld_words<W>(vc + p.words + (16 * i + vec()) * (4 * W), w);
+#pragma unroll
+            for (int x = 0; x < W; ++x) v[W * i + x] = w[x];
+        }
+        vh = *reinterpret_cast<const uint4 *>(vc + p.heads + 16 * min(vec(), U - 1));
+    }
+    // From a slot.
+    __device__ __forceinline__ void read_k(const uint8_t *words, const uint8_t *heads) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < U / 4; ++i) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(words + (16 * U) * key(h) + 16 * ((U / 4 * (lane() >> 4) + i) ^ swizzle<U>(key(h))));
+                k[h][4 * i] = w.x, k[h][4 * i + 1] = w.y, k[h][4 * i + 2] = w.z, k[h][4 * i + 3] = w.w;
+            }
+            ld_words<U / 2>(heads + key(h) * (2 * U), kh[h]);
+        }
+    }
+    __device__ __forceinline__ void read_v(const uint8_t *words, const uint8_t *heads) {
+        const int g = lane() >> 4;
+#pragma unroll
+        for (int i = 0; i < U / 2; ++i) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(words + (128 * U) * g + 256 * i + 16 * vec());
+            v[4 * i] = w.x, v[4 * i + 1] = w.y, v[4 * i + 2] = w.z, v[4 * i + 3] = w.w;
+        }
+        vh = *reinterpret_cast<const uint4 *>(heads + 16 * (g * U + min(vec(), U - 1)));
+    }
+    // A block's scores and its share of the sums; `between`: what is done when K's registers are free, `values`: before V's are used.
+    template <typename Between, typename Values>
+    __device__ __forceinline__ void block(int kb, const Sees &see, const uint8_t *, uint32_t *heads, Between between, Values values) {
+        const int g = lane() >> 4;
+        fa4 s[2] = {fa4{0.f, 0.f, 0.f, 0.f}, fa4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const fh8 a = u % 2 == 0 ? decode8_one<false>(k[h][u], kh[h][u / 2]) : decode8_one<true>(k[h][u], kh[h][u / 2]);
+                s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[u], s[h], 0, 0, 0);
+                s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[u], s[h], 0, 0, 0);
+            }
+        between();
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3];
+        if (__any(kb < see.from || kb + 32 > see.to)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int p = kb + 8 * g + j;
+                x[j] = p >= see.from && p < see.to ? x[j] : -INFINITY;
+            }
+        }
+        fh8 ph[1], pl[1];
+        const float alpha = softmax_step<8>(x, unit, m, l, ph, pl, [](float y) { return xor32_max(xor16_max(y)); },
+                                            [](float y) { return xor32_add(xor16_add(y)); });
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int b = 0; b < 2 * U; ++b) o[b] *= alpha;
+        }
+        values();
+        uint32_t *mine = heads + g * (8 * U + 8);
+        if (vec() < U) put_heads(vh, mine + 8 * vec());
+        wave_lds_fence();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const Heads2 z = get_heads(mine + 8 * u);
+#pragma unroll
+            for (int b = 2 * u; b < 2 * u + 2; ++b) {
+                const fh8 a = decode8(v[b], z.d, z.z);
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[0], o[b], 0, 0, 0);
+                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[0], o[b], 0, 0, 0);
+            }
+        }
+        wave_lds_fence();  // every lane has read before the next block's writes
+    }
+    // The waves' sums ([wave][16][HD] in `sums`) meet in wave order.
+    __device__ __forceinline__ void finish(float *sums, float (*sm)[32], float (*sl)[32], int j0, const Dest &to) {
+        constexpr int HD = 32 * U;
+        const int wv = threadIdx.x >> 6, c = vec(), g = lane() >> 4;
+        if (j0 + c < to.nvec) {
+#pragma unroll
+            for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(sums + (wv * 16 + c) * HD + 16 * b + 4 * g) = o[b];
+            if (g == 0) sm[wv][c] = m, sl[wv][c] = l;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < 16 * (HD / 4); e += 256) {
+            const int x = e / (HD / 4), d4 = 4 * (e - x * (HD / 4));
+            if (j0 + x >= to.nvec) continue;
+            const float mx = fmaxf(fmaxf(sm[0][x], sm[1][x]), fmaxf(sm[2][x], sm[3][x]));
+            float L = 0.0f;
+            float4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = share(sm[w][x], mx);
+                L = fmaf(sl[w][x], f, L);
+                const float4 p = *reinterpret_cast<const float4 *>(sums + (w * 16 + x) * HD + d4);
+                acc.x = fmaf(p.x, f, acc.x);
+                acc.y = fmaf(p.y, f, acc.y);
+                acc.z = fmaf(p.z, f, acc.z);
+                acc.w = fmaf(p.w, f, acc.w);
+            }
+            to.template put<HD>(j0 + x, d4, acc, mx, L);
+        }
+    }
 };
 
-// The NT tiles' products of a block: K decoded once for all of them. In steps of one word, each of which decodes the next one's while
-// the matrix unit works, and reads its queries ahead; left to itself the compiler waits for each.
-template <int U, int NT>
-__device__ __forceinline__ void scores(const Raw4<U> &r, const Query<U, NT> &q, const uint8_t *qlds, fa4 (&s)[NT][2]) {
-    const int lane = threadIdx.x & 63;
+// 32 vectors by v_mfma_f32_32x32x16_f16: lane l = (c = l & 31, g = l >> 5) gives row c of A and column c of B at the eight k slots
+// (g, j); the result has rows 8 (e >> 2) + 4 g + (e & 3), e < 16, column c. Over a block of 32 keys:
+//  - S^T: A row c = 8 a + 4 h + r is key 16 (a >> 1) + 8 h + 4 (a & 1) + r, dims 32 u + 16 w + 8 g + j (the K word of 2 w + g); lane
+//    (c, g) ends with the scores of keys 16 x + 8 g + j at e = 8 x + j.
+//  - O^T += V^T P^T of keys 16 x + 8 g + j: B is the lane's own eight weights in order, A a V word of slab 2 x + g; row c of row
+//    block b is dim 16 (U (c >> 4) + b) + (c & 15), so that a lane's words are whole pieces.
+// A step decodes the next one's operand while the matrix unit works (and reads its queries ahead, for hd above 128 from LDS: O is
+// half of the registers of two waves per SIMD); left to itself the compiler waits for each.
+typedef float fa16 __attribute__((ext_vector_type(16)));
+template <int U>
+struct Tile32 {
+    static constexpr int kVecs = 32;
+    static constexpr bool kLds = U > 4;
+    static constexpr int kQueryLds = kLds ? 4096 * U : 0;  // [step][hi, lo][lane]
+    uint32_t k[2][U], kh[(U + 1) / 2], v[2][U];
+    uint4 vh;
+    fh8 qh[kLds ? 1 : 2 * U], ql[kLds ? 1 : 2 * U];
+    float unit, m, l;
+    fa16 o[U];
+
+    static __device__ __forceinline__ int lane() { return threadIdx.x & 63; }
+    static __device__ __forceinline__ int vec() { return lane() & 31; }
+    static __device__ __forceinline__ int half() { return lane() >> 5; }
+    static __device__ __forceinline__ int key() {
+        const int c = vec(), a = c >> 3;
+        return 16 * (a >> 1) + 8 * (c >> 2 & 1) + 4 * (a & 1) + (c & 3);
+    }
+    static __device__ __forceinline__ int kslab() { return key() >> 3; }
+    static __device__ __forceinline__ int hslab() { return 2 * (lane() >> 4 & 1) + half(); }  // whose headers the lane takes apart
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = fa4{0.f, 0.f, 0.f, 0.f};
-    fh8 qb[2][NT][2], kb[2];
-    auto query = [&](int u) {
-        if constexpr (Query<U, NT>::kLds) {
+        for (int b = 0; b < U; ++b)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
+    }
+    __device__ __forceinline__ void no_page() {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) qb[u & 1][n][x] = *reinterpret_cast<const fh8 *>(qlds + ((u * NT + n) * 2 + x) * 1024 + 16 * lane);
+        for (int i = 0; i < (U + 1) / 2; ++i) kh[i] = kNanHeader | kNanHeader << 16;
+    }
+    static __device__ __forceinline__ int dim(int step) { return 16 * step + 8 * half(); }
+    // In LDS a wave makes every fourth step's operands; the maxima meet there first.
+    __device__ __forceinline__ void load_query(const float *qrow, uint8_t *qlds) {
+        if constexpr (kLds) {
+            constexpr int N = (2 * U + 3) / 4;
+            __shared__ float part[4][32];
+            const int wv = threadIdx.x >> 6;
+            float x[N][8], amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) __builtin_memcpy(x[i], qrow + dim(min(4 * i + wv, 2 * U - 1)), 32);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) amax = max3_abs(amax, x[i][j], x[i][j + 1]);
+            amax = xor32_max(amax);
+            if (half() == 0) part[wv][vec()] = amax;
+            __syncthreads();
+            amax = fmaxf(fmaxf(part[0][vec()], part[1][vec()]), fmaxf(part[2][vec()], part[3][vec()]));
+            const float up = query_scale<U>(amax, unit);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int step = 4 * i + wv;
+                if (step >= 2 * U) continue;
+                fh8 h, lo;
+                split_query(x[i], up, h, lo);
+                *reinterpret_cast<fh8 *>(qlds + 2048 * step + 16 * lane()) = h;
+                *reinterpret_cast<fh8 *>(qlds + 2048 * step + 1024 + 16 * lane()) = lo;
+            }
+            __syncthreads();
         } else {
+            float x[2 * U][8], amax = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) qb[u & 1][n][0] = q.h[n][u], qb[u & 1][n][1] = q.l[n][u];
+            for (int i = 0; i < 2 * U; ++i) __builtin_memcpy(x[i], qrow + dim(i), 32);
+#pragma unroll
+            for (int i = 0; i < 2 * U; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) amax = max3_abs(amax, x[i][j], x[i][j + 1]);
+            const float up = query_scale<U>(xor32_max(amax), unit);
+#pragma unroll
+            for (int i = 0; i < 2 * U; ++i) split_query(x[i], up, qh[i], ql[i]);
         }
-    };
-    auto key = [&](int i) {
-        const int u = i >> 1, h = i & 1;
-        kb[i & 1] = u % 2 == 0 ? decode8_one<false>(r.k[h][u], r.kh[h][u / 2]) : decode8_one<true>(r.k[h][u], r.kh[h][u / 2]);
-    };
-    query(0);
-    key(0);
+    }
+    template <typename At>
+    __device__ __forceinline__ void issue_k(const uint8_t *__restrict__ kc, At at) {
+        const SlabAt p = at(kslab());
+        const int row = key() & 7;
 #pragma unroll
-    for (int i = 0; i < 2 * U; ++i) {
-        const int u = i >> 1, h = i & 1;
-        if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
-        if (h == 0 && u + 1 < U) query(u + 1);
-        if (i + 1 < 2 * U) key(i + 1);
+        for (int w = 0; w < 2; ++w) ld_words<U>(kc + p.words + row * (16 * U) + (2 * w + half()) * (4 * U), k[w]);
+        ld_heads<U>(kc + p.heads + row * (2 * U), kh);
+        if (p.bad) no_page();
+    }
+    template <typename At>
+    __device__ __forceinline__ void issue_v(const uint8_t *__restrict__ vc, At at) {
+        constexpr int W = U % 2 == 0 ? 4 : 2, L = U % 4 == 0 ? 4 : U % 2 == 0 ? 2 : 1;  // words of a piece, of a load
+        const int c = vec();
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const SlabAt p = at(2 * x + half());
+#pragma unroll
+            for (int i = 0; i < U / L; ++i) {
+                const int f = U * (c >> 4) + L * i;
+                uint32_t w[L];
+                ld_words<L>(vc + p.words + (16 * (f / W) + (c & 15)) * (4 * W) + f % W * 4, w);
+#pragma unroll
+                for (int y = 0; y < L; ++y) v[x][L * i + y] = w[y];
+            }
+        }
+        vh = *reinterpret_cast<const uint4 *>(vc + at(hslab()).heads + 16 * min(c & 15, U - 1));
+    }
+    __device__ __forceinline__ void read_k(const uint8_t *words, const uint8_t *heads) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < U / 4; ++i) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(words + (16 * U) * key() + 16 * ((U / 4 * (2 * w + half()) + i) ^ swizzle<U>(key())));
+                k[w][4 * i] = x.x, k[w][4 * i + 1] = x.y, k[w][4 * i + 2] = x.z, k[w][4 * i + 3] = x.w;
+            }
+        ld_words<U / 2>(heads + key() * (2 * U), kh);
+    }
+    __device__ __forceinline__ void read_v(const uint8_t *words, const uint8_t *heads) {
+        const int c = vec();
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb[i & 1], qb[u & 1][n][x], s[n][h], 0, 0, 0);
+            for (int i = 0; i < U / 4; ++i) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(words + (128 * U) * (2 * x + half()) + 256 * (U / 4 * (c >> 4) + i) + 16 * (c & 15));
+                v[x][4 * i] = w.x, v[x][4 * i + 1] = w.y, v[x][4 * i + 2] = w.z, v[x][4 * i + 3] = w.w;
+            }
+        vh = *reinterpret_cast<const uint4 *>(heads + 16 * (hslab() * U + min(c & 15, U - 1)));
     }
-    if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
-}
-// O^T += V^T P^T. Every lane of a row of 16 needs the headers of all groups of its slab: lane c takes group c's apart and the others
-// read them from LDS (`hl`, the wave's own: [slab][group] scales, zero points; moving them by DPP costs 64 instructions a block of
-// the kind that bounds this kernel).
-template <int U>
-constexpr int head_words = 4 * (8 * U + 8);
-template <int U, int NT>
-__device__ __forceinline__ void add_values(const Raw4<U> &r, const fh8 (&ph)[NT], const fh8 (&pl)[NT], uint32_t *hl, fa4 (&o)[NT][2 * U]) {
-    const int lane = threadIdx.x & 63, c = lane & 15;
-    uint32_t *mine = hl + (lane >> 4) * (8 * U + 8);
-    if (c < U) {
-        const uint32_t raw[4] = {r.vh.x, r.vh.y, r.vh.z, r.vh.w};
-        uint32_t d[4], z[4];
+    template <typename Between, typename Values>
+    __device__ __forceinline__ void block(int kb, const Sees &see, const uint8_t *qlds, uint32_t *heads, Between between, Values values) {
+        fa16 s;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = raw[i] & 0xFFF0FFF0u, z[i] = __builtin_bit_cast(uint32_t, zeros2(raw[i], i % 2 != 0));
-        *reinterpret_cast<uint4 *>(mine + 8 * c) = uint4{d[0], d[1], d[2], d[3]};
-        *reinterpret_cast<uint4 *>(mine + 8 * c + 4) = uint4{z[0], z[1], z[2], z[3]};
+        for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+        fh8 q[2][2], a[2];
+        auto query = [&](int i) {
+            if constexpr (kLds) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) q[i & 1][x] = *reinterpret_cast<const fh8 *>(qlds + 2048 * i + 1024 * x + 16 * lane());
+            } else {
+                q[i & 1][0] = qh[i], q[i & 1][1] = ql[i];
+            }
+        };
+        auto keys = [&](int i) {
+            const int u = i >> 1, w = i & 1;
+            a[i & 1] = u % 2 == 0 ? decode8_one<false>(k[w][u], kh[u / 2]) : decode8_one<true>(k[w][u], kh[u / 2]);
+        };
+        query(0);
+        keys(0);
+#pragma unroll
+        for (int i = 0; i < 2 * U; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + 1 < 2 * U) query(i + 1), keys(i + 1);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i & 1], q[i & 1][0], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i & 1], q[i & 1][1], s, 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        between();
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = s[e];
+        if (__any(kb < see.from || kb + 32 > see.to)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int p = kb + 16 * (e >> 3) + 8 * half() + (e & 7);
+                x[e] = p >= see.from && p < see.to ? x[e] : -INFINITY;
+            }
+        }
+        fh8 ph[2], pl[2];
+        const float alpha = softmax_step<16>(x, unit, m, l, ph, pl, [](float y) { return xor32_max(y); }, [](float y) { return xor32_add(y); });
+        if (__any(alpha != 1.0f)) {
+#pragma unroll
+            for (int b = 0; b < U; ++b) o[b] *= alpha;
+        }
+        values();
+        if ((lane() & 15) < U) put_heads(vh, heads + hslab() * (8 * U + 8) + 8 * (lane() & 15));
+        wave_lds_fence();
+        // Step i: row block i % U of keys 16 (i / U).
+        Heads2 z;
+        auto value = [&](int i) {
+            const int xx = i / U, b = i % U;
+            if (U % 2 != 0 || b % 2 == 0) z = get_heads(heads + (2 * xx + half()) * (8 * U + 8) + 8 * ((U * (vec() >> 4) + b) >> 1));
+            a[i & 1] = decode8(v[xx][b], z.d, z.z);
+        };
+        value(0);
+#pragma unroll
+        for (int i = 0; i < 2 * U; ++i) {
+            const int xx = i / U, b = i % U;
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + 1 < 2 * U) value(i + 1);
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i & 1], ph[xx], o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i & 1], pl[xx], o[b], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        wave_lds_fence();
     }
-    // A wave's LDS operations complete in order; the fence keeps the compiler from moving the reads above the writes.
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    uint4 dw[2], zw[2];
-    fh8 vb[2];
-    auto heads = [&](int u) {
-        dw[u & 1] = *reinterpret_cast<const uint4 *>(mine + 8 * u), zw[u & 1] = *reinterpret_cast<const uint4 *>(mine + 8 * u + 4);
-    };
-    auto value = [&](int b) {
-        const uint4 &x = dw[b >> 1 & 1], &y = zw[b >> 1 & 1];
-        const fh2 d[4] = {__builtin_bit_cast(fh2, x.x), __builtin_bit_cast(fh2, x.y), __builtin_bit_cast(fh2, x.z), __builtin_bit_cast(fh2, x.w)};
-        const fh2 z[4] = {__builtin_bit_cast(fh2, y.x), __builtin_bit_cast(fh2, y.y), __builtin_bit_cast(fh2, y.z), __builtin_bit_cast(fh2, y.w)};
-        vb[b & 1] = decode8(r.v[b], d, z);
-    };
-    heads(0);
-    value(0);
+    // Waves 2 and 3 hand their sums to waves 0 and 1, then those two exchange half of the dims each: result rows 16 i .. of every row
+    // block, e = 8 i .. 8 i + 7. A lane reads what the same lane of the other wave wrote.
+    __device__ __forceinline__ void finish(float *sums, float (*sm)[32], float (*sl)[32], int j0, const Dest &to) {
+        constexpr int HD = 32 * U;
+        const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = vec();
+        auto give = [&](float *box, int i) {
 #pragma unroll
-    for (int b = 0; b < 2 * U; ++b) {
-        if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
-        if (b % 2 == 0 && b + 2 < 2 * U) heads(b / 2 + 1);
-        if (b + 1 < 2 * U) value(b + 1);
+            for (int b = 0; b < U; ++b)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[b & 1], ph[n], o[n][b], 0, 0, 0);
+                for (int y = 0; y < 2; ++y) {
+                    const int e = 8 * i + 4 * y;
+                    *reinterpret_cast<fa4 *>(box + 512 * b + 256 * y + 4 * lane()) = fa4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]};
+                }
+        };
+        // o and the other wave's sums under their shares; `first`: the other's count as the left operand.
+        auto take = [&](const float *box, int i, float own, float other, bool first) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) o[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[b & 1], pl[n], o[n][b], 0, 0, 0);
+            for (int b = 0; b < U; ++b)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const fa4 x = *reinterpret_cast<const fa4 *>(box + 512 * b + 256 * y + 4 * lane());
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float mine = o[b][8 * i + 4 * y + e];
+                        o[b][8 * i + 4 * y + e] = first ? fmaf(mine, own, x[e] * other) : fmaf(x[e], other, mine * own);
+                    }
+                }
+        };
+        auto stats = [&](int from, bool first, float &own, float &other) {
+            const float om = sm[from][c], ol = sl[from][c], mx = fmaxf(m, om);
+            own = share(m, mx), other = share(om, mx);
+            l = first ? fmaf(l, own, ol * other) : fmaf(ol, other, l * own);
+            m = mx;
+        };
+        float *const box = sums + (wv & 1) * 32 * HD;  // of waves wv and wv ^ 2
+        float own, other;
+        if (wv >= 2) {
+            give(box, 0), give(box + 16 * HD, 1);
+            if (half() == 0) sm[wv][c] = m, sl[wv][c] = l;
+        }
+        __syncthreads();
+        if (wv < 2) {
+            stats(wv + 2, false, own, other);
+            take(box, 0, own, other, false), take(box + 16 * HD, 1, own, other, false);
+            give(box, 1 - wv);
+            if (half() == 0) sm[wv][c] = m, sl[wv][c] = l;
+        }
+        __syncthreads();
+        if (wv >= 2) return;
+        const float *theirs = sums + (1 - wv) * 32 * HD;
+        stats(1 - wv, wv == 1, own, other);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (wv != i) continue;
+            take(theirs, i, own, other, i == 1);
+            if (j0 + c >= to.nvec) continue;
+#pragma unroll
+            for (int b = 0; b < U; ++b)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const int e = 8 * i + 4 * y;
+                    to.template put<HD>(j0 + c, 16 * (U * i + b) + 8 * y + 4 * half(), float4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]}, m, l);
+                }
+        }
     }
-    if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");  // every lane has read before the next block's writes
-    __builtin_amdgcn_wave_barrier();
-}
+};
+template <int U, int VECS>
+using Tile = std::conditional_t<VECS == 16, Tile16<U>, Tile32<U>>;
 
-// One workgroup of four waves per (chunk of keys, kv head, group of 16 NT query vectors); vector j of a segment is (row j / G, head
+// One workgroup of four waves per (chunk of keys, kv head, group of VECS query vectors); vector j of a segment is (row j / G, head
 // j % G of the kv head's group). The waves take the 32-key blocks in turn (wave w those whose index is w modulo 4, whatever the
 // chunk: with one chunk a row's sums do not depend on the other rows of its pass), decode them once into MFMA operands for all of
-// the group's tiles, with an online softmax each, and meet at the end.
+// the group's vectors, with an online softmax, and meet at the end.
 //
-// Bound by vector instructions: 640 a block and wave at hd 256 for one tile, 500 of them for the 16384 values decoded, 64 MFMAs
-// beside them; a second tile adds 140 and 64. So groups of more than 16 vectors take two tiles (q in LDS then, for hd 256: O alone
-// is half of the registers of two waves per SIMD). Keys by LDS tiles decoded once for 64 vectors (8 waves, a barrier per 64 keys)
-// took 94 us for 512 rows over 2048 keys, its two waves per SIMD in step; this takes 74.
+// Bound by vector instructions: at hd 256 500 a block and wave for the 16384 values decoded, 140 more for 16 vectors, beside 64 MFMAs
+// of 16 cycles. So groups of more than 16 vectors take 32, by the larger MFMA, which halves the issue slots of the products and the
+// keys' header work. Keys by LDS tiles decoded once for 64 vectors (8 waves, a barrier per 64 keys) took 94 us for 512 rows over
+// 2048 keys, its two waves per SIMD in step; 32 vectors as two tiles of 16 70, this XX.
 // MODE: see Slab4; -1 and -2: blocks by vector loads, in pages and contiguous.
-template <int U, int NT, int MODE>
+template <int U, int VECS, int MODE>
 __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
                                                             const uint8_t *__restrict__ vc, float *__restrict__ part,
                                                             float *__restrict__ pml, float *__restrict__ out, SegTable T, Map4 M, Cuts C,
                                                             int heads, int bidirectional, int window) {
-    constexpr bool DMA = MODE >= 0, QLDS = Query<U, NT>::kLds;
-    constexpr int HD = 32 * U, S = DMA ? Ring<U, NT>::kSlots : 1, LD = Ring<U, NT>::kLoads, WORDS = Ring<U, NT>::kWords;
+    using Tile = Tile<U, VECS>;
+    using Ring = Ring<U, VECS>;
+    constexpr bool DMA = MODE >= 0;
+    constexpr int HD = 32 * U, S = DMA ? Ring::kSlots : 1, LD = Ring::kLoads, WORDS = Ring::kWords;
     // One slot only: its K part and its V part are filled again each as soon as it has been read.
     constexpr bool SPLIT = DMA && S == 1;
-    constexpr int BYTES = Ring<U, NT>::kBytes, RING = DMA ? S * BYTES : 0, QB = QLDS ? U * NT * 2048 : 0, SUMS = 256 * HD;
+    constexpr int BYTES = Ring::kBytes, RING = DMA ? S * BYTES : 0, QB = Tile::kQueryLds, SUMS = 256 * HD;
     __shared__ __align__(16) uint8_t lds[4 * RING + QB > SUMS ? 4 * RING + QB : SUMS];
-    __shared__ float sm[4][2][16], sl[4][2][16];
+    __shared__ float sm[4][32], sl[4][32];
     __shared__ __align__(16) uint32_t vheads[4][head_words<U>];
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int bases = C.base[lane];
     const Found found = find_segment(T, C.first, C.total, blockIdx.x / M.kv_heads);
     const Seg s = found.s;
     const int G = heads / M.kv_heads, nvec = s.rows * G, units = found.next - found.first;
-    // A segment's kv heads x chunks x groups. One tile holds its vectors whole; of several groups (the last rows, which see the most
-    // keys, first) those of a head and chunk go to one XCD, for its L2: eight heads and chunks at a time, then the rest.
+    // A segment's kv heads x chunks x groups. One tile of 16 holds its vectors whole; of several groups (the last rows, which see the
+    // most keys, first) those of a head and chunk go to one XCD, for its L2: eight heads and chunks at a time, then the rest.
     const int at = blockIdx.x - found.first * M.kv_heads;
-    const int groups = NT == 1 ? 1 : (nvec + 16 * NT - 1) / (16 * NT), n = NT == 1 ? units : units / groups;
+    const int groups = VECS == 16 ? 1 : (nvec + VECS - 1) / VECS, n = VECS == 16 ? units : units / groups;
     int stream = at, group = 0;
-    if (NT != 1) {
+    if (VECS != 16) {
         const int streams = n * M.kv_heads, rest = streams & 7, eights = (streams - rest) * groups;
         if (at < eights) {
             const int block = at / (8 * groups), x = at - block * 8 * groups;
@@ -792,22 +1045,18 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
         }
         group = groups - 1 - group;
     }
-    const int ci = stream / M.kv_heads, kvh = stream - ci * M.kv_heads, j0 = group * 16 * NT;
-    const Sees lo = sees(s, NT == 1 ? 0 : j0 / G, bidirectional, window);
-    const Sees hi = sees(s, NT == 1 ? s.rows - 1 : min(j0 + 16 * NT - 1, nvec - 1) / G, bidirectional, window);
+    const int ci = stream / M.kv_heads, kvh = stream - ci * M.kv_heads, j0 = group * VECS;
+    const Sees lo = sees(s, VECS == 16 ? 0 : j0 / G, bidirectional, window);
+    const Sees hi = sees(s, VECS == 16 ? s.rows - 1 : min(j0 + VECS - 1, nvec - 1) / G, bidirectional, window);
     const int c_lo = first_key(s, window) + ci * C.len;
     const int k_lo = max(c_lo, lo.from & ~31), k_hi = n == 1 ? hi.to : min(c_lo + C.len, hi.to), last = (k_hi - 1) / kSlab;
     if (k_lo >= k_hi) return;
     int kb = k_lo + 32 * ((wv - (k_lo >> 5)) & 3);
     uint8_t *const ring = lds + wv * RING, *const qlds = lds + 4 * RING;
-    Raw4<U> r;
-    SlabAt ks, vs;
+    Tile tile;
     uint32_t bad = 0;  // four bits a slot
-    // Lane (c, g) takes K rows of slab c >> 2 and V words of slab g of a block; slabs past the last key's read that one's (masked).
-    auto places = [&](int block) {
-        ks = slab_at<U, MODE == -1>(M, s.slot, kvh, min(block / kSlab + (c >> 2), last));
-        vs = slab_at<U, MODE == -1>(M, s.slot, kvh, min(block / kSlab + g, last));
-    };
+    // Slabs past the last key's: that one is read (their keys are masked).
+    auto place_in = [&](int block) { return [&, block](int slab) { return slab_at<U, MODE == -1>(M, s.slot, kvh, min(block / kSlab + slab, last)); }; };
     auto fetch = [&](int block, int slot) {
         if constexpr (DMA) {
             const Slab4 where = look_up<U, MODE>(M, s.slot, kvh, block, last);
@@ -818,53 +1067,17 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
             dma_heads<U, MODE>(kc, vc, where, to + 2 * WORDS, !SPLIT, true);
             bad = (bad & ~(15u << 4 * slot)) | where.bad << 4 * slot;
         } else {
-            places(block);
-            issue_k<U>(kc, ks, r);
-            issue_v<U>(vc, vs, r);
+            tile.issue_k(kc, place_in(block));
+            tile.issue_v(vc, place_in(block));
         }
     };
     if (kb < k_hi) fetch(kb, 0);
     // Vectors past the last one repeat it; they are not written.
-    auto vector = [&](int tile) { return min(j0 + 16 * tile + c, nvec - 1); };
-    auto qrow = [&](int j) {
-        const int t = j / G;
-        return q + (static_cast<size_t>(s.row0 + t) * heads + kvh * G + j - t * G) * HD;
-    };
-    Query<U, NT> qr;
-    float unit[NT];
-    Sees see[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        see[i] = sees(s, vector(i) / G, bidirectional, window);
-        see[i].to = min(see[i].to, k_hi);
-    }
-    if constexpr (QLDS) {  // a wave makes every second step's operands of a tile
-        __shared__ float units[NT][16];
-        const int tile = wv % NT;
-        fh8 h[U], l[U];
-        const float x = load_query<U>(qrow(vector(tile)), h, l);
-        if (wv < NT && g == 0) units[tile][c] = x;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (u % (4 / NT) != wv / NT) continue;
-            *reinterpret_cast<fh8 *>(qlds + ((u * NT + tile) * 2) * 1024 + 16 * lane) = h[u];
-            *reinterpret_cast<fh8 *>(qlds + ((u * NT + tile) * 2 + 1) * 1024 + 16 * lane) = l[u];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NT; ++i) unit[i] = units[i][c];
-    } else {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) unit[i] = load_query<U>(qrow(vector(i)), qr.h[i], qr.l[i]);
-    }
-    float m[NT], l[NT];
-    fa4 o[NT][2 * U];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        m[i] = -INFINITY, l[i] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < 2 * U; ++b) o[i][b] = fa4{0.f, 0.f, 0.f, 0.f};
-    }
+    const int j = min(j0 + Tile::vec(), nvec - 1), t = j / G;
+    Sees see = sees(s, t, bidirectional, window);
+    see.to = min(see.to, k_hi);
+    tile.load_query(q + (static_cast<size_t>(s.row0 + t) * heads + kvh * G + j - t * G) * HD, qlds);
+    tile.clear();
 #pragma unroll
     for (int i = 1; i < S; ++i)
         if (kb + 128 * i < k_hi) fetch(kb + 128 * i, i);
@@ -883,45 +1096,40 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
             uint8_t *const from = ring + slot * BYTES;
             Slab4 where;
             if constexpr (DMA) {
-                // Landed: all but this block's V and the blocks behind it. The page of the block that comes into the slot meanwhile.
+                // Landed: all but the blocks behind this one (one slot: this one's V). One slot: the page of the block that comes into
+                // it meanwhile.
                 wait_loads(SPLIT ? LD : LD * min(left, S - 1));
                 if (SPLIT && more) where = look_up<U, MODE>(M, s.slot, kvh, kb + 128 * S, last);
-                read_k<U>(from, from + 2 * WORDS, r);
-                if (MODE != 0 && bad != 0 && (bad >> (4 * slot + (c >> 2)) & 1)) no_page<U>(r);
-            } else {
-                if (more) places(kb + 128);
+                tile.read_k(from, from + 2 * WORDS);
+                if (MODE != 0 && bad != 0 && (bad >> (4 * slot + Tile::kslab()) & 1)) tile.no_page();
             }
-            fa4 sc[NT][2];
-            scores<U, NT>(r, qr, qlds, sc);
+            tile.block(
+                kb, see, qlds, vheads[wv],
+                [&] {
+                    if (!more) return;
+                    if constexpr (SPLIT) {
+                        vq::wait_lgkm0();  // the part has been read
+                        dma_words<U, MODE, true>(kc, where, from);
+                        dma_heads<U, MODE>(kc, vc, where, from + 2 * WORDS, true, false);
+                        bad = (bad & ~(15u << 4 * slot)) | where.bad << 4 * slot;
+                    } else if constexpr (!DMA) {
+                        tile.issue_k(kc, place_in(kb + 128));
+                    }
+                },
+                [&] {
+                    if constexpr (SPLIT) wait_loads(more ? LD : 0);
+                    if constexpr (DMA) tile.read_v(from + WORDS, from + 2 * WORDS + 512);
+                });
             if (more) {
                 if constexpr (SPLIT) {
-                    vq::wait_lgkm0();  // the part has been read
-                    dma_words<U, MODE, true>(kc, where, from);
-                    dma_heads<U, MODE>(kc, vc, where, from + 2 * WORDS, true, false);
-                    bad = (bad & ~(15u << 4 * slot)) | where.bad << 4 * slot;
-                } else if constexpr (!DMA) {
-                    issue_k<U>(kc, ks, r);
-                }
-            }
-            fh8 ph[NT], pl[NT];
-#pragma unroll
-            for (int i = 0; i < NT; ++i) softmax_step<U>(sc[i], unit[i], kb, see[i].from, see[i].to, m[i], l[i], o[i], ph[i], pl[i]);
-            if constexpr (DMA) {
-                if (SPLIT) wait_loads(more ? LD : 0);
-                read_v<U>(from + WORDS, from + 2 * WORDS + 512, r);
-            }
-            add_values<U, NT>(r, ph, pl, vheads[wv], o);
-            if (more) {
-                if constexpr (DMA) {
                     vq::wait_lgkm0();
-                    if constexpr (SPLIT) {
-                        dma_words<U, MODE, false>(vc, where, from + WORDS);
-                        dma_heads<U, MODE>(kc, vc, where, from + 2 * WORDS, false, true);
-                    } else {
-                        fetch(kb + 128 * S, slot);
-                    }
+                    dma_words<U, MODE, false>(vc, where, from + WORDS);
+                    dma_heads<U, MODE>(kc, vc, where, from + 2 * WORDS, false, true);
+                } else if constexpr (DMA) {
+                    vq::wait_lgkm0();
+                    fetch(kb + 128 * S, slot);
                 } else {
-                    issue_v<U>(vc, vs, r);
+                    tile.issue_v(vc, place_in(kb + 128));
                 }
             }
             kb += 128;
@@ -929,56 +1137,8 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
     }
     __builtin_amdgcn_s_setprio(0);
     __syncthreads();  // every slot of every wave, and the queries, have been read
-    float *sums = reinterpret_cast<float *>(lds);
-    const Dest to{out, part, pml, static_cast<size_t>(from_lane(bases, found.index)), heads, G, kvh, s.row0, nvec, n, ci};
-    if constexpr (NT == 1) {
-        if (j0 + c < nvec) {
-#pragma unroll
-            for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(sums + (wv * 16 + c) * HD + 16 * b + 4 * g) = o[0][b];
-            if (g == 0) sm[wv][0][c] = m[0], sl[wv][0][c] = l[0];
-        }
-        __syncthreads();
-        meet4<HD>(sums, sm, sl, j0, to);
-    } else {
-        // Waves 2 and 3 hand their sums to waves 0 and 1, then those two exchange a tile each. [wave or its partner][tile][lane's
-        // values]: a lane reads what the same lane of the other wave wrote.
-        auto give = [&](int box, int i) {
-            float *to_box = sums + (box * 2 + i) * 16 * HD;
-#pragma unroll
-            for (int b = 0; b < 2 * U; ++b) *reinterpret_cast<fa4 *>(to_box + 256 * b + 4 * lane) = o[i][b];
-            if (g == 0) sm[wv][i][c] = m[i], sl[wv][i][c] = l[i];
-        };
-        auto take = [&](int box, int i, int from, bool first) {  // `first`: the other wave's sums count as the left operand
-            const float *box_at = sums + (box * 2 + i) * 16 * HD;
-            const float om = sm[from][i][c], ol = sl[from][i][c], mx = fmaxf(m[i], om);
-            const float own = share(m[i], mx), other = share(om, mx), fl = first ? other : own, fr = first ? own : other;
-            l[i] = fmaf(first ? l[i] : ol, fr, (first ? ol : l[i]) * fl);
-#pragma unroll
-            for (int b = 0; b < 2 * U; ++b) {
-                const fa4 x = *reinterpret_cast<const fa4 *>(box_at + 256 * b + 4 * lane);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[i][b][e] = first ? fmaf(o[i][b][e], fr, x[e] * fl) : fmaf(x[e], fr, o[i][b][e] * fl);
-            }
-            m[i] = mx;
-        };
-        if (wv >= 2) give(wv - 2, 0), give(wv - 2, 1);
-        __syncthreads();
-        if (wv < 2) take(wv, 0, wv + 2, false), take(wv, 1, wv + 2, false);
-        __syncthreads();
-        if (wv == 0) give(0, 1);
-        if (wv == 1) give(1, 0);
-        __syncthreads();
-        if (wv >= 2) return;
-        if (wv == 0) take(1, 0, 1, false);
-        else take(0, 1, 0, true);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int j = j0 + 16 * i + c;
-            if (wv != i || j >= nvec) continue;
-#pragma unroll
-            for (int b = 0; b < 2 * U; ++b) to.put<HD>(j, 16 * b + 4 * g, float4{o[i][b][0], o[i][b][1], o[i][b][2], o[i][b][3]}, m[i], l[i]);
-        }
-    }
+    tile.finish(reinterpret_cast<float *>(lds), sm, sl, j0,
+                Dest{out, part, pml, static_cast<size_t>(from_lane(bases, found.index)), heads, G, kvh, s.row0, nvec, n, ci});
 }
 
 // A row's chunks: [lo, hi) of n hold its keys; the part of (row, head, chunk) is at `at` + head n + chunk.
@@ -986,15 +1146,15 @@ struct RowChunks {
     int t, n, lo, hi;
     size_t at;
 };
-template <int NT>
+template <int VECS>
 __device__ __forceinline__ RowChunks row_chunks(const Found &found, const SegTable &T, const Cuts &C, int chunks, int bases, int row, int heads, int G,
                                                 int bidirectional, int window) {
     const Seg s = found.s;
     const int i = found.index, t = row - found.first;
     const int units = (i + 1 < T.n ? from_lane(chunks, i + 1 < 64 ? i + 1 : 63) : C.total) - from_lane(chunks, i);
-    RowChunks r{t, NT == 1 ? units : units / ((s.rows * G + 16 * NT - 1) / (16 * NT)), 0, 0, 0};
+    RowChunks r{t, VECS == 16 ? units : units / ((s.rows * G + VECS - 1) / VECS), 0, 0, 0};
     r.hi = r.n;
-    if (NT != 1) {  // (one tile: every chunk has been written)
+    if (VECS != 16) {  // (one tile of 16: every chunk has been written)
         const Sees see = sees(s, t, bidirectional, window);
         const int k0 = first_key(s, window);
         r.lo = (see.from - k0) / C.len, r.hi = min((see.to - 1 - k0) / C.len + 1, r.n);
@@ -1044,7 +1204,7 @@ __device__ __forceinline__ void put_merged(float *to, const float4 &acc, float L
 // out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, for segments of more than one. It is latency that this
 // kernel spends, so a workgroup takes 64 dims of a (row, head) (32 where hd is no multiple of 64), a thread four dims of every 16th
 // (32nd) chunk; the 16 (32) sums meet in order. 24 rows of 128 chunks, hd 256: 4 us; one workgroup of four waves for a row took 11.
-template <int HD, int NT>
+template <int HD, int VECS>
 __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
                                                                float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads,
                                                                int G, int bidirectional, int window) {
@@ -1055,7 +1215,7 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
     const int row = blockIdx.x / heads, h = blockIdx.x - row * heads, d = 4 * (Q * blockIdx.y + quad);
     const int chunks = C.first[lane], bases = C.base[lane];
     const Found found = find_segment(T, R.first, R.total, row);
-    const RowChunks r = row_chunks<NT>(found, T, C, chunks, bases, row, heads, G, bidirectional, window);
+    const RowChunks r = row_chunks<VECS>(found, T, C, chunks, bases, row, heads, G, bidirectional, window);
     if (r.n == 1) return;
     const size_t at = r.at + static_cast<size_t>(h) * r.n;
     float m, L;
@@ -1083,14 +1243,14 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
 }
 // The same for up to kFewChunks chunks: a thread takes four dims of a head, workgroups (row, 1024 values of it).
 constexpr int kFewChunks = 8;
-template <int HD, int NT>
+template <int HD, int VECS>
 __global__ __launch_bounds__(256) void attention4_merge_few_kernel(const float *__restrict__ part, const float *__restrict__ pml,
                                                                    float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads,
                                                                    int G, int bidirectional, int window) {
     const int lane = threadIdx.x & 63, row = blockIdx.x;
     const int chunks = C.first[lane], bases = C.base[lane];
     const Found found = find_segment(T, R.first, R.total, row);
-    const RowChunks r = row_chunks<NT>(found, T, C, chunks, bases, row, heads, G, bidirectional, window);
+    const RowChunks r = row_chunks<VECS>(found, T, C, chunks, bases, row, heads, G, bidirectional, window);
     const int e = blockIdx.y * 256 + threadIdx.x, h = e / (HD / 4), d = 4 * (e - h * (HD / 4));
     if (r.n == 1 || h >= heads) return;
     const size_t at = r.at + static_cast<size_t>(h) * r.n;
@@ -1176,8 +1336,8 @@ int launch_read4(const void *kc, const void *vc, float *k, float *v, const SegTa
 // contexts, the one with the least rounds x (keys of a chunk + what a chunk costs besides, in keys: its start and end, 160 keys' time,
 // and with more than one chunk the partial results of a group, 100 for each tile).
 struct Shape {
-    int heads, kv_heads, tiles;
-    int groups(const Seg &s) const { return (s.rows * (heads / kv_heads) + 16 * tiles - 1) / (16 * tiles); }
+    int heads, kv_heads, vecs;
+    int groups(const Seg &s) const { return (s.rows * (heads / kv_heads) + vecs - 1) / vecs; }
 };
 int keys_of(const Seg &s, int window) { return s.pos0 + s.rows - first_key(s, window); }
 int chunks_of(const Seg &s, long long len, int window) { return static_cast<int>((keys_of(s, window) + len - 1) / len); }
@@ -1194,7 +1354,7 @@ Cuts make_cuts(const SegTable &T, const Shape &P, int window, bool whole) {
         for (int i = 0; i < T.n; ++i) n += static_cast<long long>(chunks_of(T.s[i], len, window)) * P.groups(T.s[i]);
         return n * P.kv_heads;
     };
-    auto cost = [&](long long len) { return (count(len) + kSlots - 1) / kSlots * (len + kFixed + (len < most ? kPart * P.tiles : 0)); };
+    auto cost = [&](long long len) { return (count(len) + kSlots - 1) / kSlots * (len + kFixed + (len < most ? kPart * P.vecs / 16 : 0)); };
     long long best = most;
     for (int rounds = 1; rounds <= 4 && !whole; ++rounds) {
         long long lo = max(work / (kSlots * rounds) / 128, 1LL), hi = most / 128;  // the least length of at most that many rounds
@@ -1229,10 +1389,10 @@ size_t parts_of(const SegTable &T, const Cuts &C, int heads, int window) {
     }
     return n;
 }
-// Two tiles to a group where a kv head has more than 16 query vectors in a segment; always without a workspace, so that a row's sums
+// 32 vectors to a group where a kv head has more than 16 in a segment; always without a workspace, so that a row's sums
 // are the same in every pass.
 Shape shape_of(const SegTable &T, int heads, int kv_heads, bool whole) {
-    return Shape{heads, kv_heads, whole || max_seg_rows(T) * (heads / kv_heads) > 16 ? 2 : 1};
+    return Shape{heads, kv_heads, whole || max_seg_rows(T) * (heads / kv_heads) > 16 ? 32 : 16};
 }
 size_t attention4_ws_bytes(const SegTable &T, int heads, int kv_heads, int hd, int window) {
     const Cuts C = make_cuts(T, shape_of(T, heads, kv_heads, false), window, false);
@@ -1267,30 +1427,30 @@ int launch_attention4(const float *q, const void *kc, const void *vc, float *out
     auto *kb = static_cast<const uint8_t *>(kc), *vb = static_cast<const uint8_t *>(vc);
     float *part = static_cast<float *>(ws), *pml = part + parts * hd;
     const dim3 grid(static_cast<unsigned>(C.total) * M.kv_heads);
-    auto pass = [&](auto u, auto tiles) {
-        constexpr int U = decltype(u)::value, NT = decltype(tiles)::value;
+    auto pass = [&](auto u, auto vecs) {
+        constexpr int U = decltype(u)::value, VECS = decltype(vecs)::value;
         auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window); };
         // hd 128 and 256 by DMA but for pages of odd numbers of slabs.
         bool done = false;
         if constexpr (U % 4 == 0) {
             done = true;
-            if (!M.pt) go(attention4_kernel<U, NT, 0>);
-            else if (M.spp % 4 == 0) go(attention4_kernel<U, NT, 4>);
-            else if (M.spp % 2 == 0) go(attention4_kernel<U, NT, 2>);
+            if (!M.pt) go(attention4_kernel<U, VECS, 0>);
+            else if (M.spp % 4 == 0) go(attention4_kernel<U, VECS, 4>);
+            else if (M.spp % 2 == 0) go(attention4_kernel<U, VECS, 2>);
             else done = false;
         }
-        if (!done && M.pt) go(attention4_kernel<U, NT, -1>);
+        if (!done && M.pt) go(attention4_kernel<U, VECS, -1>);
         if constexpr (U % 4 != 0)
-            if (!M.pt) go(attention4_kernel<U, NT, -2>);
+            if (!M.pt) go(attention4_kernel<U, VECS, -2>);
         auto merge = [&](auto kernel, const dim3 &rows) {
             kernel<<<rows, 256, 0, s>>>(part, pml, out, T, C, R, heads, heads / M.kv_heads, bidirectional, window);
         };
-        if (parts && C.most > kFewChunks) merge(attention4_merge_kernel<32 * U, NT>, dim3(T.total * heads, U % 2 == 0 ? U / 2 : U));
-        else if (parts) merge(attention4_merge_few_kernel<32 * U, NT>, dim3(T.total, (heads * 8 * U + 255) / 256));
+        if (parts && C.most > kFewChunks) merge(attention4_merge_kernel<32 * U, VECS>, dim3(T.total * heads, U % 2 == 0 ? U / 2 : U));
+        else if (parts) merge(attention4_merge_few_kernel<32 * U, VECS>, dim3(T.total, (heads * 8 * U + 255) / 256));
     };
     for_hd(hd, [&](auto u) {
-        if (P.tiles == 1) pass(u, std::integral_constant<int, 1>{});
-        else pass(u, std::integral_constant<int, 2>{});
+        if (P.vecs == 16) pass(u, std::integral_constant<int, 16>{});
+        else pass(u, std::integral_constant<int, 32>{});
     });
     return status_of(hipGetLastError());
 }
