@@ -363,8 +363,10 @@ __device__ __forceinline__ void split_query(const float (&x)[8], float up, fh8 &
 }
 
 // Softmax step over a lane's N products s of a block (masked ones are -inf), which times `unit` are scores in base-2 units: new
-// running maximum and sum, the factor for what was summed before, the weights as f16 pairs (the first half rounded towards zero, the
+// running maximum and sum, the factor for what was summed before (the maximum follows only by steps above kMaxStep, since the sums'
+// rescaling costs as much as the step: weights are then up to 2^kMaxStep, which takes nothing from them), the weights as f16 pairs (the first half rounded towards zero, the
 // second the rest: 22 significant bits). The sum is of the weights before they are split. `across`: over the lanes of a vector.
+constexpr float kMaxStep = 8.0f;
 template <int N, typename Max, typename Add>
 __device__ __forceinline__ float softmax_step(const float (&v)[N], float unit, float &m, float &l, fh8 (&ph)[N / 8], fh8 (&pl)[N / 8], Max max_across,
                                               Add add_across) {
@@ -372,7 +374,7 @@ __device__ __forceinline__ float softmax_step(const float (&v)[N], float unit, f
 #pragma unroll
     for (int j = 0; j < N; ++j) bm = fmaxf(bm, v[j]);
     bm = max_across(bm) * unit;
-    const float mn = fmaxf(m, bm), ms = mn == -INFINITY ? 0.0f : mn;  // ms: exp2(-inf - ms) is 0 also before any key
+    const float mn = bm > m + kMaxStep ? bm : m, ms = mn == -INFINITY ? 0.0f : mn;  // ms: exp2(-inf - ms) is 0 also before any key
     const float alpha = __builtin_amdgcn_exp2f(m - ms);
     float ps = 0.0f;
 #pragma unroll
@@ -1094,12 +1096,13 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
             else __builtin_amdgcn_s_setprio(0);
             const bool more = left >= S;
             uint8_t *const from = ring + slot * BYTES;
-            Slab4 where;
+            Slab4 where{};
             if constexpr (DMA) {
                 // Landed: all but the blocks behind this one (one slot: this one's V). One slot: the page of the block that comes into
                 // it meanwhile.
-                wait_loads(SPLIT ? LD : LD * min(left, S - 1));
                 if (SPLIT && more) where = look_up<U, MODE>(M, s.slot, kvh, kb + 128 * S, last);
+                if (SPLIT) asm volatile("" : "+s"(where.words0), "+s"(where.heads0));  // (before K's reads, which would wait for it)
+                wait_loads(SPLIT ? LD : LD * min(left, S - 1));
                 tile.read_k(from, from + 2 * WORDS);
                 if (MODE != 0 && bad != 0 && (bad >> (4 * slot + Tile::kslab()) & 1)) tile.no_page();
             }
