@@ -48,8 +48,8 @@ struct Starts {
 };
 
 // A segment as a workgroup finds it: the last one whose beginning is <= x. Lane i loads segment i and what goes with it, all at
-// once, and the found one's values come from its lane. Kernel arguments lie in host memory, 2 us away at the first touch, and one
-// load after the other (a walk over the segments, then their rows, then their bases) made up a third of a decode step's time.
+// once, and the found one's values come from its lane: kernel arguments lie in host memory, and loads that wait for each other (a walk
+// over the segments, then their rows, then their bases) would each pay that way.
 struct Found {
     Seg s;
     int index, first, next;  // beginning of the segment, and of the next one
@@ -914,18 +914,25 @@ struct Tile32 {
         values();
         if ((lane() & 15) < U) put_heads(vh, heads + hslab() * (8 * U + 8) + 8 * (lane() & 15));
         wave_lds_fence();
-        // Step i: row block i % U of keys 16 (i / U).
-        Heads2 z;
-        auto value = [&](int i) {
+        // Step i: row block i % U of keys 16 (i / U). Headers are read two steps ahead.
+        Heads2 z[2];
+        auto header = [&](int i) {
             const int xx = i / U, b = i % U;
-            if (U % 2 != 0 || b % 2 == 0) z = get_heads(heads + (2 * xx + half()) * (8 * U + 8) + 8 * ((U * (vec() >> 4) + b) >> 1));
-            a[i & 1] = decode8(v[xx][b], z.d, z.z);
+            if (U % 2 != 0 || b % 2 == 0)
+                z[U % 2 != 0 ? i & 1 : i >> 1 & 1] = get_heads(heads + (2 * xx + half()) * (8 * U + 8) + 8 * ((U * (vec() >> 4) + b) >> 1));
         };
+        auto value = [&](int i) {
+            const Heads2 &y = z[U % 2 != 0 ? i & 1 : i >> 1 & 1];
+            a[i & 1] = decode8(v[i / U][i % U], y.d, y.z);
+        };
+        header(0);
+        if (U % 2 != 0) header(1);
         value(0);
 #pragma unroll
         for (int i = 0; i < 2 * U; ++i) {
             const int xx = i / U, b = i % U;
             __builtin_amdgcn_sched_barrier(0);
+            if (i + 2 < 2 * U) header(i + 2);
             if (i + 1 < 2 * U) value(i + 1);
             o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i & 1], ph[xx], o[b], 0, 0, 0);
             o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i & 1], pl[xx], o[b], 0, 0, 0);
@@ -1010,7 +1017,7 @@ using Tile = std::conditional_t<VECS == 16, Tile16<U>, Tile32<U>>;
 // Bound by vector instructions: at hd 256 500 a block and wave for the 16384 values decoded, 140 more for 16 vectors, beside 64 MFMAs
 // of 16 cycles. So groups of more than 16 vectors take 32, by the larger MFMA, which halves the issue slots of the products and the
 // keys' header work. Keys by LDS tiles decoded once for 64 vectors (8 waves, a barrier per 64 keys) took 94 us for 512 rows over
-// 2048 keys, its two waves per SIMD in step; 32 vectors as two tiles of 16 70, this XX.
+// 2048 keys, its two waves per SIMD in step; 32 vectors as two tiles of 16 70, this 63.
 // MODE: see Slab4; -1 and -2: blocks by vector loads, in pages and contiguous.
 template <int U, int VECS, int MODE>
 __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
@@ -1244,8 +1251,8 @@ __global__ __launch_bounds__(256) void attention4_merge_kernel(const float *__re
     }
     put_merged(out + (static_cast<size_t>(found.s.row0 + r.t) * heads + h) * HD + d, acc, L);
 }
-// The same for up to kFewChunks chunks: a thread takes four dims of a head, workgroups (row, 1024 values of it).
-constexpr int kFewChunks = 8;
+// The same where chunks are few or rows many: a thread takes four dims of a head over all chunks, a workgroup 1024 values of a row.
+// 64 rows of 9 chunks, 24 heads, hd 256: 5.1 us, the kernel above 10.7; 8 rows of 128 chunks: 14.3, and 4.9.
 template <int HD, int VECS>
 __global__ __launch_bounds__(256) void attention4_merge_few_kernel(const float *__restrict__ part, const float *__restrict__ pml,
                                                                    float *__restrict__ out, SegTable T, Cuts C, Starts R, int heads,
@@ -1430,6 +1437,8 @@ int launch_attention4(const float *q, const void *kc, const void *vc, float *out
     auto *kb = static_cast<const uint8_t *>(kc), *vb = static_cast<const uint8_t *>(vc);
     float *part = static_cast<float *>(ws), *pml = part + parts * hd;
     const dim3 grid(static_cast<unsigned>(C.total) * M.kv_heads);
+    // Which merge: by rows where no thread has more than two batches of chunks, or 256 workgroups' worth of rows with up to 32 chunks.
+    const bool few = C.most <= 8 || (C.most <= 32 && static_cast<long long>(T.total) * heads * hd >= 1 << 18);
     auto pass = [&](auto u, auto vecs) {
         constexpr int U = decltype(u)::value, VECS = decltype(vecs)::value;
         auto go = [&](auto kernel) { kernel<<<grid, 256, 0, s>>>(q, kb, vb, part, pml, out, T, M, C, heads, bidirectional, window); };
@@ -1448,7 +1457,7 @@ int launch_attention4(const float *q, const void *kc, const void *vc, float *out
         auto merge = [&](auto kernel, const dim3 &rows) {
             kernel<<<rows, 256, 0, s>>>(part, pml, out, T, C, R, heads, heads / M.kv_heads, bidirectional, window);
         };
-        if (parts && C.most > kFewChunks) merge(attention4_merge_kernel<32 * U, VECS>, dim3(T.total * heads, U % 2 == 0 ? U / 2 : U));
+        if (parts && !few) merge(attention4_merge_kernel<32 * U, VECS>, dim3(T.total * heads, U % 2 == 0 ? U / 2 : U));
         else if (parts) merge(attention4_merge_few_kernel<32 * U, VECS>, dim3(T.total, (heads * 8 * U + 255) / 256));
     };
     for_hd(hd, [&](auto u) {
