@@ -21,6 +21,7 @@
 
 namespace {
 
+// Logits of a thread: 4 or 16 take longer (64 rows sampled: 24.4 us with 8, 28.7 and 25.0; one sequence of 4 rows: 17.5, 17.7, 21.1).
 constexpr int kThreads = 256, kEach = 8, kChunk = kThreads * kEach;
 
 struct VerSeq {
@@ -46,30 +47,34 @@ struct VerArgs {
 
 // A logit as it counts: NaN never wins, like -inf.
 __device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY; }
-// e^x for x <= 0: x = n ln 2 + r with |r| <= ln 2 / 2, the Taylor polynomial of degree 12 in r (the rest is below 2^-53), times 2^n.
-// Below -1100 the result is 0 anyway. Half the instructions of the math library's, which also serves x > 0 and NaN: the statistics
-// of 64 rows of 248320 take 17 us instead of 24.
-__device__ __forceinline__ double exp_neg(double x) {
+// 2^x for x <= 0: x = n + f with |f| <= 1/2, the Taylor polynomial of degree 12 in f ln 2 (the rest is below 2^-53), times 2^n. Below
+// -1100 the result is 0 anyway. The math library's exp, which also serves x > 0 and NaN, takes twice the instructions, and they are
+// as many as hide behind the logits' loads: see verify_stats_kernel.
+__device__ __forceinline__ double exp2_neg(double x) {
+    constexpr double L = 0.6931471805599453;
     x = fmax(x, -1100.0);
-    const double n = rint(x * 1.4426950408889634);
-    const double r = fma(-n, 2.3190468138462996e-17, fma(-n, 0.6931471805599453, x));
-    double p = 1.0 / 479001600.0;
-    p = fma(p, r, 1.0 / 39916800.0);
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
+    const double n = rint(x), f = x - n;
+    double p = L * L * L * L * L * L * L * L * L * L * L * L / 479001600.0;
+    p = fma(p, f, L * L * L * L * L * L * L * L * L * L * L / 39916800.0);
+    p = fma(p, f, L * L * L * L * L * L * L * L * L * L / 3628800.0);
+    p = fma(p, f, L * L * L * L * L * L * L * L * L / 362880.0);
+    p = fma(p, f, L * L * L * L * L * L * L * L / 40320.0);
+    p = fma(p, f, L * L * L * L * L * L * L / 5040.0);
+    p = fma(p, f, L * L * L * L * L * L / 720.0);
+    p = fma(p, f, L * L * L * L * L / 120.0);
+    p = fma(p, f, L * L * L * L / 24.0);
+    p = fma(p, f, L * L * L / 6.0);
+    p = fma(p, f, L * L / 2.0);
+    p = fma(p, f, L);
+    p = fma(p, f, 1.0);
     return ldexp(p, static_cast<int>(n));
 }
-// exp((x - m) / T), 1 at the maximum whatever it is (all of the mass is at +inf where that is the maximum).
-__device__ __forceinline__ double weight(double x, double m, double inv_t) { return x == m ? 1.0 : exp_neg((x - m) * inv_t); }
+// exp((x - m) / T), `per` being log2(e) / T; 1 at the maximum whatever it is (all of the mass is at +inf where that is the maximum).
+__device__ __forceinline__ double weight(double x, double m, double per) {
+    if (m == INFINITY) return x == m ? 1.0 : 0.0;
+    return x == m ? 1.0 : exp2_neg((x - m) * per);
+}
+constexpr double kLog2e = 1.4426950408889634;
 
 // A thread's kEach neighbouring values from i on, `fill` past n.
 __device__ __forceinline__ void load_each(const float *p, int i, int n, float fill, float (&x)[kEach]) {
@@ -125,6 +130,9 @@ __device__ __forceinline__ int2 group_span(int lo, int hi, int2 *lds) {
 }
 
 // Workgroup (chunk, row of a sequence, sequence): (maximum, sum of weights against it), for a greedy row (maximum, its lowest index).
+// Bound by the logits' bytes and by the weights' 22 instructions of 64 bits a logit, nearly equally: 64 rows of 248320 are 64 MB, 12.5
+// us at the rate of a copy, and 9 us of instructions; this takes 19 (22 with an exp of 27 instructions). Workgroups of several chunks that load one while they compute
+// with the one before take longer (4 chunks: 24 us): many workgroups at different points overlap the two better.
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerArgs a, VerTable T) {
     __shared__ float smax[4];
     __shared__ double ssum[4];
@@ -152,10 +160,15 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerArgs a, VerTa
         if (threadIdx.x == 0) *out = double2{m, static_cast<double>(first)};
         return;
     }
-    const double inv_t = 1.0 / t;
+    const double per = kLog2e / t;
     double s = 0.0;
+    if (m < INFINITY) {
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) s += weight(x[e], m, inv_t);
+        for (int e = 0; e < kEach; ++e) s += exp2_neg((static_cast<double>(x[e]) - m) * per);  // (1 at the maximum)
+    } else {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) s += x[e] == m ? 1.0 : 0.0;
+    }
     s = group_sum(m > -INFINITY ? s : 0.0, ssum);
     if (threadIdx.x == 0) *out = double2{m, s};
 }
@@ -169,7 +182,7 @@ struct Decision {
 __device__ void decide(const VerArgs &a, const VerSeq &s, Decision &d) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const bool greedy = s.t == 0.0;
-    const double inv_t = greedy ? 0.0 : 1.0 / s.t;
+    const double per = greedy ? 0.0 : kLog2e / s.t;
     if (threadIdx.x == 0) d.stop = s.k;
     __syncthreads();
     for (int j = wv; j <= s.k; j += kThreads / 64) {
@@ -201,7 +214,7 @@ __device__ void decide(const VerArgs &a, const VerSeq &s, Decision &d) {
         for (int o = 32; o > 0; o >>= 1) m = fmax(m, __shfl_xor(m, o, 64));
         double z = greedy ? static_cast<double>(INT_MAX) : 0.0;
         auto add = [&](const double2 &v) {
-            if (!greedy) z += v.y * weight(v.x, m, inv_t);
+            if (!greedy) z += v.y * weight(v.x, m, per);
             else if (v.x == m) z = fmin(z, v.y);
         };
 #pragma unroll
@@ -217,7 +230,7 @@ __device__ void decide(const VerArgs &a, const VerSeq &s, Decision &d) {
             d.m[j] = m;
             d.z[j] = z;
             const double given = q > 0.0f ? q : 0.0;
-            const bool ok = greedy ? static_cast<double>(x) == z : z > 0.0 && static_cast<double>(u) * given * z < weight(l, m, inv_t);
+            const bool ok = greedy ? static_cast<double>(x) == z : z > 0.0 && static_cast<double>(u) * given * z < weight(l, m, per);
             if (j < s.k && (x < 0 || !ok)) atomicMin(&d.stop, j);
         }
     }
@@ -229,14 +242,14 @@ __device__ void decide(const VerArgs &a, const VerSeq &s, Decision &d) {
 struct Source {
     const float *l, *q;  // q null: no draft's probabilities are taken off
     int without;         // a token left out
-    double m, inv_t, inv_z;
+    double m, per, inv_z;
     __device__ __forceinline__ void each(int i, int n, double (&w)[kEach]) const {
         float x[kEach], y[kEach];
         load_each(l, i, n, -INFINITY, x);
         if (q) load_each(q, i, n, 0.0f, y);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            const double p = weight(logit(x[e]), m, inv_t) * inv_z;
+            const double p = weight(logit(x[e]), m, per) * inv_z;
             w[e] = p;
             if (q) w[e] = fmax(p - (y[e] > 0.0f ? static_cast<double>(y[e]) : 0.0), 0.0);
             if (i + e >= n || i + e == without) w[e] = 0.0;
@@ -245,7 +258,7 @@ struct Source {
 };
 __device__ __forceinline__ Source source_of(const VerArgs &a, const VerSeq &s, const Decision &d, bool refused) {
     const int j = d.stop;
-    Source r{a.logits + static_cast<size_t>(s.row0 + j) * a.vocab, nullptr, -1, d.m[j], 1.0 / s.t, 1.0 / d.z[j]};
+    Source r{a.logits + static_cast<size_t>(s.row0 + j) * a.vocab, nullptr, -1, d.m[j], kLog2e / s.t, 1.0 / d.z[j]};
     if (refused) {
         if (a.probs) r.q = a.probs + static_cast<size_t>(s.draft0 + j) * a.vocab;
         else r.without = a.draft[s.draft0 + j];
@@ -288,7 +301,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerArgs a, VerTab
         const double v = a.u[2 * static_cast<size_t>(s.row0 + j) + 1], inv_z = 1.0 / d.z[j];
         const int per = (a.chunks + kThreads - 1) / kThreads, c0 = tid * per, c1 = min(c0 + per, a.chunks);
         bool refused = j < s.k;
-        auto of_chunk = [&](int c) { return refused ? left[c] : st[c].y * weight(st[c].x, d.m[j], inv_t) * inv_z; };
+        auto of_chunk = [&](int c) { return refused ? left[c] : st[c].y * weight(st[c].x, d.m[j], kLog2e / s.t) * inv_z; };
         for (;;) {
             double mine = 0.0;
             for (int c = c0; c < c1; ++c) mine += of_chunk(c);
