@@ -562,6 +562,14 @@ __device__ __forceinline__ Heads2 get_heads(const uint32_t *from) {
     return Heads2{{__builtin_bit_cast(fh2, x.x), __builtin_bit_cast(fh2, x.y), __builtin_bit_cast(fh2, x.z), __builtin_bit_cast(fh2, x.w)},
                   {__builtin_bit_cast(fh2, y.x), __builtin_bit_cast(fh2, y.y), __builtin_bit_cast(fh2, y.z), __builtin_bit_cast(fh2, y.w)}};
 }
+// Of a slab's V headers those of positions below `to`: what lies behind the last key may never have been written, and a weight of zero
+// does not take away a scale that is no number.
+__device__ __forceinline__ uint4 heads_below(const uint4 &raw, int pos, int to) {
+    uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] &= (pos + 2 * i < to ? 0xFFFFu : 0u) | (pos + 2 * i + 1 < to ? 0xFFFF0000u : 0u);
+    return uint4{w[0], w[1], w[2], w[3]};
+}
 // A wave's LDS operations complete in order; the fence keeps the compiler from moving them over each other.
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
@@ -660,7 +668,7 @@ struct Tile16 {
     }
     // A block's scores and its share of the sums; `between`: what is done when K's registers are free, `values`: before V's are used.
     template <typename Between, typename Values>
-    __device__ __forceinline__ void block(int kb, const Sees &see, const uint8_t *, uint32_t *heads, Between between, Values values) {
+    __device__ __forceinline__ void block(int kb, int k_hi, const Sees &see, const uint8_t *, uint32_t *heads, Between between, Values values) {
         const int g = lane() >> 4;
         fa4 s[2] = {fa4{0.f, 0.f, 0.f, 0.f}, fa4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -691,6 +699,7 @@ struct Tile16 {
         }
         values();
         uint32_t *mine = heads + g * (8 * U + 8);
+        if (kb + 32 > k_hi) vh = heads_below(vh, kb + 8 * g, k_hi);
         if (vec() < U) put_heads(vh, mine + 8 * vec());
         wave_lds_fence();
 #pragma unroll
@@ -867,7 +876,7 @@ struct Tile32 {
         vh = *reinterpret_cast<const uint4 *>(heads + 16 * (hslab() * U + min(c & 15, U - 1)));
     }
     template <typename Between, typename Values>
-    __device__ __forceinline__ void block(int kb, const Sees &see, const uint8_t *qlds, uint32_t *heads, Between between, Values values) {
+    __device__ __forceinline__ void block(int kb, int k_hi, const Sees &see, const uint8_t *qlds, uint32_t *heads, Between between, Values values) {
         fa16 s;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = 0.0f;
@@ -912,6 +921,7 @@ struct Tile32 {
             for (int b = 0; b < U; ++b) o[b] *= alpha;
         }
         values();
+        if (kb + 32 > k_hi) vh = heads_below(vh, kb + 8 * hslab(), k_hi);
         if ((lane() & 15) < U) put_heads(vh, heads + hslab() * (8 * U + 8) + 8 * (lane() & 15));
         wave_lds_fence();
         // Step i: row block i % U of keys 16 (i / U). Headers are read two steps ahead.
@@ -1114,7 +1124,7 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
                 if (MODE != 0 && bad != 0 && (bad >> (4 * slot + Tile::kslab()) & 1)) tile.no_page();
             }
             tile.block(
-                kb, see, qlds, vheads[wv],
+                kb, k_hi, see, qlds, vheads[wv],
                 [&] {
                     if (!more) return;
                     if constexpr (SPLIT) {

@@ -1,5 +1,5 @@
-// vq_seq.h -- what the sequence ops' translation units share: segment tables, cache addressing, cross-lane exchanges, the
-// query operand of the f16 attention products and the merge of a split context's chunks.
+// vq_seq.h -- what the sequence ops' translation units share: segment tables, cache addressing, cross-lane exchanges, operand
+// types of the f16 products.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -108,7 +108,7 @@ inline SegTable one_segment(int pos0, int rows) {
     return T;
 }
 
-// ---- attention: the query operand and the merge of chunks ---------------------------------------------------
+// ---- operands of the f16 products -----------------------------------------------------------------------
 
 typedef float fa4 __attribute__((ext_vector_type(4)));
 typedef _Float16 fh8 __attribute__((ext_vector_type(8)));
@@ -122,117 +122,6 @@ __device__ __forceinline__ void split_h(float x, _Float16 &hi, _Float16 &lo) {
     hi = static_cast<_Float16>(x);
     lo = static_cast<_Float16>(x - static_cast<float>(hi));
 }
-// The query vector of lane column c (dims 32 u + 8 g .. + 7), loaded raw; fa16_q_split turns it into the B
-// operands, times 1/sqrt(hd) * 2^s, and returns 2^-s log2(e): scores leave the S product in base-2 units, so
-// the softmax weights are exp2 (v_exp_f32) of their differences, and maxima are converted back (times ln 2) only
-// where they leave the kernel. Split in two so that a block's K/V loads can be issued
-// between them.
-template <int HD>
-__device__ __forceinline__ void fa16_q_load(const float *qrow, float4 (&qr)[HD / 16]) {
-    const int g = (threadIdx.x & 63) >> 4;
-#pragma unroll
-    for (int u = 0; u < HD / 32; ++u) {
-        qr[2 * u] = *reinterpret_cast<const float4 *>(qrow + 32 * u + 8 * g);
-        qr[2 * u + 1] = *reinterpret_cast<const float4 *>(qrow + 32 * u + 8 * g + 4);
-    }
-}
-template <int HD>
-__device__ __forceinline__ float fa16_q_split(const float4 (&qr)[HD / 16], float scale, fh8 (&qh)[HD / 32],
-                                              fh8 (&ql)[HD / 32]) {
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < HD / 16; ++i)
-        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(qr[i].x), fabsf(qr[i].y))), fmaxf(fabsf(qr[i].z), fabsf(qr[i].w)));
-    amax *= scale;
-    amax = xor16_max(amax);
-    amax = xor32_max(amax);
-    int ex = 0;
-    if (amax > 0.0f && amax <= 3.0e38f) frexpf(amax, &ex);  // amax = f 2^ex, f in [0.5, 1)
-    // Capped at 2^126 so that the scale and its inverse stay finite for queries below ~1e-34 (their scores are
-    // then tiny, as they should be, instead of NaN).
-    const int e2 = 14 - ex < 126 ? 14 - ex : 126;
-    const float up = ldexpf(1.0f, e2);
-#pragma unroll
-    for (int u = 0; u < HD / 32; ++u) {
-        const float v[8] = {qr[2 * u].x, qr[2 * u].y, qr[2 * u].z, qr[2 * u].w,
-                            qr[2 * u + 1].x, qr[2 * u + 1].y, qr[2 * u + 1].z, qr[2 * u + 1].w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            _Float16 h, l;
-            split_h(v[j] * scale * up, h, l);
-            qh[u][j] = h;
-            ql[u][j] = l;
-        }
-    }
-    return ldexpf(1.0f, -e2) * 1.44269504088896341f;  // S in base-2 units: the softmax uses exp2
-}
-
-// out = sum_c e^(m_c - M) o_c / sum_c e^(m_c - M) l_c, M = max_c m_c; one workgroup of four waves per (row of the
-// pass, head): the chunks' maxima through LDS, then wave w adds chunks w, w + 4, ... (lane = four head dims, one
-// 16-byte load per chunk) and the four waves' sums are added in wave order (deterministic).
-template <int HD>
-__global__ __launch_bounds__(256) void attention_merge_kernel(const float *__restrict__ part, const float *__restrict__ pml,
-                                                              float *__restrict__ out, SegTable T, int heads, int hd,
-                                                              int nch) {
-    __shared__ float smx[4];
-    __shared__ float4 sacc[4][HD / 4];
-    __shared__ float sl[4];
-    int t;
-    const Seg &s = seg_of_row(T, blockIdx.x / heads, t);
-    const int h = blockIdx.x % heads;
-    const size_t qv = static_cast<size_t>(s.row0 + t) * heads + h;
-    const float *ml = pml + qv * nch * 2;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    float mx = -INFINITY;
-    for (int c = tid; c < nch; c += 256) mx = fmaxf(mx, ml[2 * c]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-    if (lane == 0) smx[wv] = mx;
-    __syncthreads();
-    const float M = fmaxf(fmaxf(smx[0], smx[1]), fmaxf(smx[2], smx[3]));
-    float4 acc{0.f, 0.f, 0.f, 0.f};
-    float L = 0.0f;
-    if (4 * lane < HD) {
-        // Chunks wv, wv + 4, ... in order, four at a time with all their loads in flight.
-        for (int c0 = wv; c0 < nch; c0 += 16) {
-            float4 p4[4];
-            float mc[4], lc[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int c = c0 + 4 * k < nch ? c0 + 4 * k : c0;
-                p4[k] = *reinterpret_cast<const float4 *>(part + (qv * nch + c) * HD + 4 * lane);
-                mc[k] = ml[2 * c];
-                lc[k] = ml[2 * c + 1];
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (c0 + 4 * k >= nch) break;
-                const float f = mc[k] == -INFINITY ? 0.0f : expf(mc[k] - M);
-                L = fmaf(lc[k], f, L);
-                acc.x = fmaf(p4[k].x, f, acc.x);
-                acc.y = fmaf(p4[k].y, f, acc.y);
-                acc.z = fmaf(p4[k].z, f, acc.z);
-                acc.w = fmaf(p4[k].w, f, acc.w);
-            }
-        }
-        sacc[wv][lane] = acc;
-    }
-    if (lane == 0) sl[wv] = L;
-    __syncthreads();
-    if (wv == 0 && 4 * lane < HD) {
-        const float Lt = ((sl[0] + sl[1]) + sl[2]) + sl[3];
-        const float inv = Lt > 0.0f ? 1.0f / Lt : 0.0f;
-        const float4 a = sacc[0][lane], b = sacc[1][lane], c = sacc[2][lane], d = sacc[3][lane];
-        const float r[4] = {((a.x + b.x) + c.x) + d.x, ((a.y + b.y) + c.y) + d.y, ((a.z + b.z) + c.z) + d.z,
-                            ((a.w + b.w) + c.w) + d.w};
-        float *o = out + qv * hd;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (4 * lane + k < hd) o[4 * lane + k] = r[k] * inv;
-    }
-}
-
-inline int fa_hd(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 inline int max_seg_rows(const SegTable &T) {
     int r = 0;
     for (int i = 0; i < T.n; ++i) r = T.s[i].rows > r ? T.s[i].rows : r;
