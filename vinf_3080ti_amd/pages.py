@@ -82,9 +82,8 @@ class PageBook:
 
     def apply(self, pools: Sequence[int], page_bytes: Sequence[int], table: int, stream: int) -> None:
         """Carry the plan out: pools at these addresses with pages of these sizes, the page table at `table`."""
-        n = len(pools)
-        _lib.check(self._lib.vq_book_apply(self._book, (ctypes.c_void_p * n)(*pools), (ctypes.c_size_t * n)(*page_bytes), n, table,
-                                           stream), "pages")
+        at, sizes = array.array("Q", pools), array.array("Q", page_bytes)
+        _lib.check(self._lib.vq_book_apply(self._book, at.buffer_info()[0], sizes.buffer_info()[0], len(at), table, stream), "pages")
 
     def row(self, slot: int) -> list[int]:
         """The pages that a slot holds, in the order of its positions."""

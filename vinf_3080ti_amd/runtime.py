@@ -775,48 +775,59 @@ class Runtime:
         _, page, per_slot, slots = self._paging
         self._pages = (PageBook(int(pages), page, per_slot, slots), dict(zip(names, sizes)))
 
-    def _page_work(self, what: str, plan, *args) -> int:
-        """PageBook's call plan(*args), then what it decided on the device; returns the pages copied."""
+    def _page_work(self, what: str, plan, *args) -> None:
+        """PageBook's call plan(*args), then what it decided on the device. Called under the pages' lock."""
         if self._pages is None or self._paging is None:
             raise RuntimeError("set_page_pools first")
-        with self._pages_lock:
-            book, pools = self._pages
-            ptrs = []
-            for name, size in pools.items():
+        book, pools = self._pages
+        ptrs = []
+        for name, size in pools.items():
+            b = self.buffers.get(name)
+            if b is None or b.lent:
                 b = self._any_buffer(name)
-                if b.n * b.elem < size * book.pages:
-                    raise ValueError(f"device buffer {name} has {b.n * b.elem} bytes, need {size * book.pages}")
-                ptrs.append(b.ptr)
-            table, _, _ = self._page_table()
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"{what}: page work cannot be captured")
-            plan(book, *args)
-            copied = book.copies()
-            book.apply(ptrs, pools.values(), table, self._stream())
-            return copied
+            if b.n * b.elem < size * book.pages:
+                raise ValueError(f"device buffer {name} has {b.n * b.elem} bytes, need {size * book.pages}")
+            ptrs.append(b.ptr)
+        table, _, _ = self._page_table()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what}: page work cannot be captured")
+        plan(book, *args)
+        book.apply(ptrs, pools.values(), table, self._stream())
 
     def pages_reserve(self, segments) -> None:
         """Make the rows that a pass is about to write ((slot, pos0, rows, ...) as in set_segments) the slot's own: pages that it
         lacks are taken, pages that it shares replaced by copies. ValueError when the pool has too few, and nothing changes."""
-        self._page_work("pages_reserve", PageBook.reserve, segments)
+        with self._pages_lock:
+            self._page_work("pages_reserve", PageBook.reserve, segments)
 
     def pages_fork(self, src: int, dst: Sequence[int], length: int) -> None:
         """Empty slots dst begin as src's first `length` positions, in the same pages (pages_reserve parts them where one is
         written)."""
-        self._page_work("pages_fork", PageBook.fork, src, dst, length)
+        with self._pages_lock:
+            self._page_work("pages_fork", PageBook.fork, src, dst, length)
 
     def pages_copy(self, pairs) -> None:
         """(src, dst, length) each: empty slot dst gets a copy of src's first `length` positions in pages of its own."""
-        self._page_work("pages_copy", PageBook.copy, pairs)
+        with self._pages_lock:
+            self._page_work("pages_copy", PageBook.copy, pairs)
 
     def pages_free(self, slots: Sequence[int], length: int = 0) -> None:
         """The slots give back the pages behind their first `length` positions (all of them by default; after a verification that
         refused drafts, those behind what was accepted). Table entries are left as they are."""
-        self._page_work("pages_free", PageBook.free, slots, length)
+        with self._pages_lock:
+            self._page_work("pages_free", PageBook.free, slots, length)
 
     def pages_compact(self) -> int:
         """Move pages so that those in use are the lowest ids; returns how many moved."""
-        return self._page_work("pages_compact", PageBook.compact)
+        def compact(book: PageBook) -> None:
+            nonlocal moved
+            book.compact()
+            moved = book.copies()
+
+        moved = 0
+        with self._pages_lock:
+            self._page_work("pages_compact", compact)
+        return moved
 
     def pages_of(self, slot: int) -> list[int]:
         """The pages that a slot holds, in the order of its positions."""
