@@ -266,7 +266,7 @@ int vq_kv4_read(const void *kc, const void *vc, float *k, float *v, int ntok, in
 int vq_kv4_read_seg(const void *kc, const void *vc, float *k, float *v, const int32_t *segs, int nseg, int kv_heads, int hd,
                     const int32_t *page_table, int page_size, int pages_per_seq, int pages, void *stream);
 
-/* Workspace bytes of vq_attention4_ws / vq_attention4_seg_ws for these shapes; 0 for passes that take none, and for invalid
+/* Workspace bytes of vq_attention4_ws / vq_attention4_seg_ws for these shapes (a few for passes that are not cut); 0 for invalid
  * arguments. */
 size_t vq_attention4_workspace_bytes(int heads, int kv_heads, int hd, int seq_len, int ntok, int window);
 size_t vq_attention4_seg_workspace_bytes(const int32_t *segs, int nseg, int heads, int kv_heads, int hd);
@@ -274,7 +274,8 @@ size_t vq_attention4_seg_workspace_bytes(const int32_t *segs, int nseg, int head
 /* vq_attention / vq_attention_seg over 4-bit caches: the products are exact f16 products of the cache's values with the query
  * and the softmax weights as f16 pairs (22 significant bits), sums in fp32. With a workspace (16-byte aligned, >= the matching
  * query, else VQ_ERR_WORKSPACE) a context may be cut into chunks that are merged in chunk order (deterministic); with NULL each
- * row's keys are walked in one order, which does not depend on the other rows of the pass (the batch-invariant mode). No
+ * row's keys are walked in one order, which does not depend on the other rows of the pass (the batch-invariant mode). Positions
+ * behind a pass's last key are not used, whatever their memory holds; q and out need float alignment only. No
  * counterpart in the reference (its attention reads fp32 and fp16 caches, qwen_runtime.cu:128-162, 2449-2478). */
 int vq_attention4_ws(const float *q, const void *kc, const void *vc, float *out, int heads, int kv_heads, int hd, int max_seq,
                      int seq_len, int ntok, int bidirectional, int window, void *workspace, size_t workspace_bytes,

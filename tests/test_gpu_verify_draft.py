@@ -130,6 +130,18 @@ def test_values_at_the_edges(rt, oracle_mod):
     check(oracle_mod, run(rt, *args), args)
 
 
+def test_temperatures_at_the_ends(rt, oracle_mod):
+    """The smallest positive temperatures leave the largest logit (ties share), the largest one makes all tokens alike."""
+    rng = np.random.default_rng(6)
+    drafted, temps = [2, 0, 1, 2, 0], [5e-324, 1e-310, 1e-300, 1.7e308, 1e-308]
+    l, draft, probs, u = case(rng, 3000, drafted, temps, True)
+    l[3, [5, 90]] = 50.0
+    l[0, draft[0]] = 60.0
+    for p in (probs, None):
+        args = (l, draft, p, u, drafted, temps)
+        check(oracle_mod, run(rt, *args), args)
+
+
 def test_a_sequence_does_not_depend_on_the_others(rt):
     """The bits of a sequence's results alone, in a batch, and behind a capture that is replayed."""
     import torch

@@ -142,3 +142,11 @@ def test_attention_refusals(lib):
     if need:
         big = dict(heads=24, kvh=4, hd=256, max_seq=100000, seq_len=100000, ntok=1)
         assert call(**big, ws=FAKE, nws=need - 1) == call(**big, ws=ODD, nws=need) == _lib.VQ_ERR_WORKSPACE
+
+
+def test_attention_ends_inside_32_bits(lib):
+    """Contexts so near the end of 32 bits that a wave's step past the last key would leave them: no workspace size, and a refusal."""
+    end = 2 ** 31 - 1
+    assert lib.vq_attention4_workspace_bytes(8, 2, 64, end - 1024, 1, 0) > 0
+    assert lib.vq_attention4_workspace_bytes(8, 2, 64, end - 1022, 1, 0) == 0
+    assert lib.vq_attention4_ws(FAKE, FAKE, FAKE, FAKE, 8, 2, 64, end - 8, end - 1022, 1, 0, 0, None, 0, None) == _lib.VQ_ERR_SHAPE

@@ -74,7 +74,8 @@ __device__ __forceinline__ double weight(double x, double m, double per) {
     if (m == INFINITY) return x == m ? 1.0 : 0.0;
     return x == m ? 1.0 : exp2_neg((x - m) * per);
 }
-constexpr double kLog2e = 1.4426950408889634;
+// log2(e) / T, finite for the smallest T too: a zero difference times it stays zero.
+__device__ __forceinline__ double per_of(double t) { return fmin(1.4426950408889634 / t, 1e300); }
 
 // A thread's kEach neighbouring values from i on, `fill` past n.
 __device__ __forceinline__ void load_each(const float *p, int i, int n, float fill, float (&x)[kEach]) {
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerArgs a, VerTa
         if (threadIdx.x == 0) *out = double2{m, static_cast<double>(first)};
         return;
     }
-    const double per = kLog2e / t;
+    const double per = per_of(t);
     double s = 0.0;
     if (m < INFINITY) {
 #pragma unroll
@@ -182,7 +183,7 @@ struct Decision {
 __device__ void decide(const VerArgs &a, const VerSeq &s, Decision &d) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const bool greedy = s.t == 0.0;
-    const double per = greedy ? 0.0 : kLog2e / s.t;
+    const double per = greedy ? 0.0 : per_of(s.t);
     if (threadIdx.x == 0) d.stop = s.k;
     __syncthreads();
     for (int j = wv; j <= s.k; j += kThreads / 64) {
@@ -258,7 +259,7 @@ struct Source {
 };
 __device__ __forceinline__ Source source_of(const VerArgs &a, const VerSeq &s, const Decision &d, bool refused) {
     const int j = d.stop;
-    Source r{a.logits + static_cast<size_t>(s.row0 + j) * a.vocab, nullptr, -1, d.m[j], kLog2e / s.t, 1.0 / d.z[j]};
+    Source r{a.logits + static_cast<size_t>(s.row0 + j) * a.vocab, nullptr, -1, d.m[j], per_of(s.t), 1.0 / d.z[j]};
     if (refused) {
         if (a.probs) r.q = a.probs + static_cast<size_t>(s.draft0 + j) * a.vocab;
         else r.without = a.draft[s.draft0 + j];
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerArgs a, VerTab
         const double v = a.u[2 * static_cast<size_t>(s.row0 + j) + 1], inv_z = 1.0 / d.z[j];
         const int per = (a.chunks + kThreads - 1) / kThreads, c0 = tid * per, c1 = min(c0 + per, a.chunks);
         bool refused = j < s.k;
-        auto of_chunk = [&](int c) { return refused ? left[c] : st[c].y * weight(st[c].x, d.m[j], kLog2e / s.t) * inv_z; };
+        auto of_chunk = [&](int c) { return refused ? left[c] : st[c].y * weight(st[c].x, d.m[j], per_of(s.t)) * inv_z; };
         for (;;) {
             double mine = 0.0;
             for (int c = c0; c < c1; ++c) mine += of_chunk(c);
