@@ -147,7 +147,8 @@ def _pack(x, values):
     else:
         words = _words(c.reshape(n, p, hd // 32, 4, 8)).transpose(2, 3)
         heads = _headers(d, z)
-    return torch.cat([words.contiguous().view(torch.uint8).reshape(n, -1), heads.contiguous().view(torch.uint8).reshape(n, -1)], 1)
+    # (As rows first: a last axis of one group, hd 32, may keep any stride, and a view as bytes needs one.)
+    return torch.cat([x.reshape(n, -1).contiguous().view(torch.uint8) for x in (words, heads)], 1)
 
 
 def _unpack(blocks, p, hd, values):
