@@ -145,8 +145,12 @@ def test_attention_refusals(lib):
 
 
 def test_attention_ends_inside_32_bits(lib):
-    """Contexts so near the end of 32 bits that a wave's step past the last key would leave them: no workspace size, and a refusal."""
+    """Contexts so near the end of 32 bits that a wave's step past the last key would leave them, and passes with more query vectors
+    than that: no workspace size, and a refusal."""
     end = 2 ** 31 - 1
     assert lib.vq_attention4_workspace_bytes(8, 2, 64, end - 1024, 1, 0) > 0
     assert lib.vq_attention4_workspace_bytes(8, 2, 64, end - 1022, 1, 0) == 0
     assert lib.vq_attention4_ws(FAKE, FAKE, FAKE, FAKE, 8, 2, 64, end - 8, end - 1022, 1, 0, 0, None, 0, None) == _lib.VQ_ERR_SHAPE
+    assert lib.vq_attention4_workspace_bytes(8, 2, 64, 5, 2 ** 27 + 1, 0) == 0
+    assert lib.vq_attention4_seg_workspace_bytes(segs((0, 0, 2 ** 26, 0), (1, 0, 2 ** 26 + 1, 0))[0], 2, 8, 2, 64) == 0
+    assert lib.vq_attention4_ws(FAKE, FAKE, FAKE, FAKE, 8, 2, 64, end - 8, 5, 2 ** 27 + 1, 0, 0, None, 0, None) == _lib.VQ_ERR_SHAPE

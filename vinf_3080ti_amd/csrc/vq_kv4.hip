@@ -1360,11 +1360,14 @@ int launch_read4(const void *kc, const void *vc, float *k, float *v, const SegTa
     return status_of(hipGetLastError());
 }
 
-// Positions that a wave may step past, and chunks be rounded up by, without leaving 32 bits.
-bool ends_ok(const SegTable &T) {
-    for (int i = 0; i < T.n; ++i)
+// Passes whose numbers stay inside 32 bits: query vectors, and the positions that a wave may step to or chunks be rounded up to.
+bool fits(const SegTable &T, int heads) {
+    long long rows = 0;
+    for (int i = 0; i < T.n; ++i) {
         if (T.s[i].pos0 > INT32_MAX - 1024 - T.s[i].rows) return false;
-    return true;
+        rows += T.s[i].rows;
+    }
+    return rows <= INT32_MAX / 2 / heads;
 }
 // Chunks for the 512 workgroups that run at once (two per CU): of the lengths that make one to four full rounds, and of whole
 // contexts, the one with the least rounds x (keys of a chunk + what a chunk costs besides, in keys: its start and end, 160 keys' time,
@@ -1451,7 +1454,7 @@ int launch_attention4(const float *q, const void *kc, const void *vc, float *out
                       int bidirectional, int window, void *ws, size_t ws_bytes, hipStream_t s) {
     if (!q || !out) return VQ_ERR_ARG;
     if (heads < M.kv_heads || heads % M.kv_heads || window < 0) return VQ_ERR_SHAPE;
-    if (static_cast<long long>(T.total) * heads > INT32_MAX / 2 || !ends_ok(T)) return VQ_ERR_SHAPE;
+    if (!fits(T, heads)) return VQ_ERR_SHAPE;
     const bool whole = ws == nullptr;
     const Shape P = shape_of(T, heads, M.kv_heads, whole);
     const Cuts C = make_cuts(T, P, window, whole);
@@ -1540,14 +1543,14 @@ int vq_kv4_read_seg(const void *kc, const void *vc, float *k, float *v, const in
 size_t vq_attention4_workspace_bytes(int heads, int kv_heads, int hd, int seq_len, int ntok, int window) {
     if (kv_heads < 1 || heads < kv_heads || heads % kv_heads || !hd_ok(hd) || ntok < 1 || seq_len < 1 || window < 0) return 0;
     const SegTable T = one_segment(seq_len - 1, ntok);
-    return ends_ok(T) ? attention4_ws_bytes(T, heads, kv_heads, hd, window) : 0;
+    return fits(T, heads) ? attention4_ws_bytes(T, heads, kv_heads, hd, window) : 0;
 }
 
 size_t vq_attention4_seg_workspace_bytes(const int32_t *segs, int nseg, int heads, int kv_heads, int hd) {
     SegTable T;
     if (make_table(segs, nseg, T, nullptr) != VQ_OK) return 0;
     if (kv_heads < 1 || heads < kv_heads || heads % kv_heads || !hd_ok(hd)) return 0;
-    return ends_ok(T) ? attention4_ws_bytes(T, heads, kv_heads, hd, 0) : 0;
+    return fits(T, heads) ? attention4_ws_bytes(T, heads, kv_heads, hd, 0) : 0;
 }
 
 int vq_attention4_ws(const float *q, const void *kc, const void *vc, float *out, int heads, int kv_heads, int hd, int max_seq,
