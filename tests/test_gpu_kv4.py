@@ -280,7 +280,8 @@ def test_attention(rt, oracle_mod, heads, kvh, hd, ntok, seq_len, bidirectional,
         check(got[: q.size].reshape(q.shape), q, k, v, heads, kvh, seq_len, oracle_mod, bidirectional, window)
 
 
-@pytest.mark.parametrize("heads,kvh,hd,page", [(24, 4, 256, 64), (32, 8, 128, 16), (64, 8, 64, 8), (6, 2, 96, 24), (5, 5, 32, 40)])
+@pytest.mark.parametrize("heads,kvh,hd,page", [(24, 4, 256, 64), (32, 8, 128, 16), (64, 8, 64, 8), (6, 2, 96, 24), (5, 5, 32, 40), (24, 4, 256, 24),
+                                                (32, 8, 128, 8), (16, 16, 128, 40), (12, 2, 256, 16), (8, 1, 160, 32), (14, 2, 224, 8)])
 def test_attention_seg(rt, oracle_mod, heads, kvh, hd, page):
     """A pass of decode, verify and prompt segments over pages in random order, one segment behind a gap whose rows stay as they
     are; each segment is also checked in passes of its own kind."""
