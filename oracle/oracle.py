@@ -351,7 +351,8 @@ def verify_draft(logits, draft, probs, u, drafted, temperature):
                 p = np.where(np.arange(l.size) == l.argmax(), 1.0, 0.0)
                 logp = np.zeros(l.size)
             else:
-                e = np.where(l == m, 1.0, np.exp((np.where(l == m, 0, l) - (m if np.isfinite(m) else 0)) / t) if m < np.inf else 0.0)
+                with np.errstate(over="ignore"):
+                    e = np.where(l == m, 1.0, np.exp((np.where(l == m, 0, l) - (m if np.isfinite(m) else 0)) / t) if m < np.inf else 0.0)
                 p = e / e.sum()
                 with np.errstate(divide="ignore"):
                     logp = np.log(p)
