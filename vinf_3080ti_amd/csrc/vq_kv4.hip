@@ -666,7 +666,8 @@ struct Tile16 {
         }
         vh = *reinterpret_cast<const uint4 *>(heads + 16 * (g * U + min(vec(), U - 1)));
     }
-    // A block's scores and its share of the sums; `between`: what is done when K's registers are free, `values`: before V's are used.
+    // A block's scores and its share of the sums; `between`: what is done when K's registers are free, `values`: V's come, under the
+    // softmax.
     template <typename Between, typename Values>
     __device__ __forceinline__ void block(int kb, int k_hi, const Sees &see, const uint8_t *, uint32_t *heads, Between between, Values values) {
         const int g = lane() >> 4;
@@ -680,6 +681,7 @@ struct Tile16 {
                 s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[u], s[h], 0, 0, 0);
             }
         between();
+        values();
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3];
@@ -697,7 +699,6 @@ struct Tile16 {
 #pragma unroll
             for (int b = 0; b < 2 * U; ++b) o[b] *= alpha;
         }
-        values();
         uint32_t *mine = heads + g * (8 * U + 8);
         if (kb + 32 > k_hi) vh = heads_below(vh, kb + 8 * g, k_hi);
         if (vec() < U) put_heads(vh, mine + 8 * vec());
@@ -904,6 +905,7 @@ struct Tile32 {
         }
         __builtin_amdgcn_sched_barrier(0);
         between();
+        values();
         float x[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = s[e];
@@ -920,7 +922,6 @@ struct Tile32 {
 #pragma unroll
             for (int b = 0; b < U; ++b) o[b] *= alpha;
         }
-        values();
         if (kb + 32 > k_hi) vh = heads_below(vh, kb + 8 * hslab(), k_hi);
         if ((lane() & 15) < U) put_heads(vh, heads + hslab() * (8 * U + 8) + 8 * (lane() & 15));
         wave_lds_fence();
