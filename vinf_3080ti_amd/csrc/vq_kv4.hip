@@ -1028,7 +1028,7 @@ using Tile = std::conditional_t<VECS == 16, Tile16<U>, Tile32<U>>;
 // Bound by vector instructions: at hd 256 500 a block and wave for the 16384 values decoded, 140 more for 16 vectors, beside 64 MFMAs
 // of 16 cycles. So groups of more than 16 vectors take 32, by the larger MFMA, which halves the issue slots of the products and the
 // keys' header work. Keys by LDS tiles decoded once for 64 vectors (8 waves, a barrier per 64 keys) took 94 us for 512 rows over
-// 2048 keys, its two waves per SIMD in step; 32 vectors as two tiles of 16 70, this 63.
+// 2048 keys, its two waves per SIMD in step; 32 vectors as two tiles of 16 70, this 61.
 // MODE: see Slab4; -1 and -2: blocks by vector loads, in pages and contiguous.
 template <int U, int VECS, int MODE>
 __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restrict__ q, const uint8_t *__restrict__ kc,
