@@ -147,8 +147,7 @@ def _pack(x, values):
     else:
         words = _words(c.reshape(n, p, hd // 32, 4, 8)).transpose(2, 3)
         heads = _headers(d, z)
-    # (As rows first: a last axis of one group, hd 32, may keep any stride, and a view as bytes needs one.)
-    return torch.cat([x.reshape(n, -1).contiguous().view(torch.uint8) for x in (words, heads)], 1)
+    return torch.cat([words.contiguous().view(torch.uint8).reshape(n, -1), heads.contiguous().view(torch.uint8).reshape(n, -1)], 1)
 
 
 def _unpack(blocks, p, hd, values):
@@ -413,7 +412,7 @@ def _plain_verify(s):
     # In 64 bits: of 248320 tokens many have less than 1e-8 of the mass, and a random number falls between their borders.
     top, best = logits.max(1)
     t = s["temp"][seq, None]
-    p = torch.exp((logits.double() - top[:, None]) / torch.where(t > 0, t, torch.ones_like(t)))
+    p = torch.exp((logits - top[:, None]).double() / torch.where(t > 0, t, torch.ones_like(t)))
     p /= p.sum(1, keepdim=True)
     one = torch.zeros_like(p).scatter_(1, best[:, None], 1.0)
     p = torch.where(t > 0, p, one)
