@@ -272,11 +272,12 @@ size_t vq_attention4_workspace_bytes(int heads, int kv_heads, int hd, int seq_le
 size_t vq_attention4_seg_workspace_bytes(const int32_t *segs, int nseg, int heads, int kv_heads, int hd);
 
 /* vq_attention / vq_attention_seg over 4-bit caches: the products are exact f16 products of the cache's values with the query
- * and the softmax weights as f16 pairs (22 significant bits), sums in fp32. With a workspace (16-byte aligned, >= the matching
- * query, else VQ_ERR_WORKSPACE) a context may be cut into chunks that are merged in chunk order (deterministic); with NULL each
- * row's keys are walked in one order, which does not depend on the other rows of the pass (the batch-invariant mode). Positions
- * behind a pass's last key are not used, whatever their memory holds; q and out need float alignment only. No
- * counterpart in the reference (its attention reads fp32 and fp16 caches, qwen_runtime.cu:128-162, 2449-2478). */
+ * and the softmax weights as f16 pairs (off by 2^-22 of themselves, or by 2^-38 of a query vector's largest element and 2^-36 of a
+ * row's largest weight), sums in fp32. With a workspace (16-byte aligned, >= the matching query, else VQ_ERR_WORKSPACE) a context
+ * may be cut into chunks that are merged in chunk order (deterministic); with NULL each row's keys are walked in one order, which
+ * does not depend on the other rows of the pass (the batch-invariant mode). Positions behind a pass's last key are not used,
+ * whatever their memory holds; q and out need float alignment only. No counterpart in the reference (its attention reads fp32 and
+ * fp16 caches, qwen_runtime.cu:128-162, 2449-2478). */
 int vq_attention4_ws(const float *q, const void *kc, const void *vc, float *out, int heads, int kv_heads, int hd, int max_seq,
                      int seq_len, int ntok, int bidirectional, int window, void *workspace, size_t workspace_bytes,
                      void *stream);

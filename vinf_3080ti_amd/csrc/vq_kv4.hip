@@ -256,6 +256,7 @@ __global__ __launch_bounds__(kMaxHd) void kv4_read_kernel(const uint8_t *__restr
 // ---- attention -----------------------------------------------------------------------------------------------
 
 typedef _Float16 fh2 __attribute__((ext_vector_type(2)));
+typedef float ff2 __attribute__((ext_vector_type(2)));
 
 // A 32-bit constant in a VGPR: a VOP3 instruction takes no literal and one SGPR at most, so (a & m) | b with two constants is one
 // instruction only where they are in VGPRs.
@@ -363,10 +364,15 @@ __device__ __forceinline__ void split_query(const float (&x)[8], float up, fh8 &
 }
 
 // Softmax step over a lane's N products s of a block (masked ones are -inf), which times `unit` are scores in base-2 units: new
-// running maximum and sum, the factor for what was summed before (the maximum follows only by steps above kMaxStep, since the sums'
-// rescaling costs as much as the step: weights are then up to 2^kMaxStep, which takes nothing from them), the weights as f16 pairs (the first half rounded towards zero, the
-// second the rest: 22 significant bits). The sum is of the weights before they are split. `across`: over the lanes of a vector.
-constexpr float kMaxStep = 8.0f;
+// reference m and sum, the factor for what was summed before, the weights 2^(score - m) as f16 pairs. m is the running maximum
+// less kLift and follows only when the maximum is past m + kMost, since the sums' rescaling costs as much as the step: a row's
+// largest weight lies between 2^kLift and 2^kMost, near the top of f16's range. So a weight is off by 2^-23 of itself or, where
+// its second half is an f16 below the normal ones, by 2^-25, at most 2^-(25 + kLift) of the largest. Both halves are rounded to
+// nearest: sums over thousands of keys would add up what rounding towards zero takes from each. 2048 keys, all but one of them
+// 14 nats below that one, whose value is zero: 2e-7 to 5e-7 of the result, with kLift 7 up to 4e-5, with weights up to 1 rounded
+// towards zero 1e-2. What kLift costs: 512 rows over 2048 keys take 62.8, 63.6, 65.5 us with 7, 11, 13. The sum is of the weights
+// before they are split. `across`: over the lanes of a vector.
+constexpr float kLift = 11.0f, kMost = 15.0f;
 template <int N, typename Max, typename Add>
 __device__ __forceinline__ float softmax_step(const float (&v)[N], float unit, float &m, float &l, fh8 (&ph)[N / 8], fh8 (&pl)[N / 8], Max max_across,
                                               Add add_across) {
@@ -374,16 +380,16 @@ __device__ __forceinline__ float softmax_step(const float (&v)[N], float unit, f
 #pragma unroll
     for (int j = 0; j < N; ++j) bm = fmaxf(bm, v[j]);
     bm = max_across(bm) * unit;
-    const float mn = bm > m + kMaxStep ? bm : m, ms = mn == -INFINITY ? 0.0f : mn;  // ms: exp2(-inf - ms) is 0 also before any key
+    const float mn = bm > m + kMost ? bm - kLift : m, ms = mn == -INFINITY ? 0.0f : mn;  // ms: exp2(-inf - ms) is 0 also before any key
     const float alpha = __builtin_amdgcn_exp2f(m - ms);
     float ps = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
-        const float a = __builtin_amdgcn_exp2f(fmaf(v[j], unit, -ms)), b = __builtin_amdgcn_exp2f(fmaf(v[j + 1], unit, -ms));
-        ps += a;
-        ps += b;
-        const fh2 hi = __builtin_bit_cast(fh2, __builtin_amdgcn_cvt_pkrtz(a, b));
-        const fh2 lo = __builtin_bit_cast(fh2, __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(hi[0]), b - static_cast<float>(hi[1])));
+        const ff2 w{__builtin_amdgcn_exp2f(fmaf(v[j], unit, -ms)), __builtin_amdgcn_exp2f(fmaf(v[j + 1], unit, -ms))};
+        ps += w[0];
+        ps += w[1];
+        const fh2 hi = __builtin_convertvector(w, fh2);
+        const fh2 lo = __builtin_convertvector((ff2{w[0] - static_cast<float>(hi[0]), w[1] - static_cast<float>(hi[1])}), fh2);
         ph[j / 8][j % 8] = hi[0], ph[j / 8][j % 8 + 1] = hi[1];
         pl[j / 8][j % 8] = lo[0], pl[j / 8][j % 8 + 1] = lo[1];
     }
