@@ -177,7 +177,7 @@ class Runtime:
         self._seg_tables: list[tuple[ctypes.Array, int]] = []  # as int32 tables of one launch each
         self._seg_span = self._seg_longest = 0
         self._pages: tuple[PageBook, dict[str, int]] | None = None  # the book, and bytes of a page of each pool
-        self._pages_lock = threading.Lock()
+        self._pages_lock = threading.RLock()  # (a call's arguments may be an iterator that asks pages_of)
         # Resident-weight memory: an optional arena and the executor's per-layer weight groups. Nothing streams
         # over PCIe here, so the stream order only records which uploads were requested as streamed.
         self._arena: _Region | None = None
@@ -747,33 +747,35 @@ class Runtime:
             raise ValueError("invalid paging shape")
         pt = self._f32_buffer(page_table, pages_per_seq * max_slots)
         paging = (pt, int(page_size), int(pages_per_seq), int(max_slots))
-        if self._paging is not None and (self._paging[0] is not pt or self._paging[1:] != paging[1:]):
-            self._pages = None  # another table: set_page_pools again
-        self._paging = paging
+        with self._pages_lock:
+            if self._paging is not None and (self._paging[0] is not pt or self._paging[1:] != paging[1:]):
+                self._pages = None  # another table: set_page_pools again
+            self._paging = paging
 
     # Pages of the caches as the runtime deals them: the pages_* calls keep the book of who holds which (pages.py) and write
     # the page table, in stream order with the passes on the current stream. They are a scheduler's calls between passes, not for
-    # a captured graph (what they decided would be replayed).
+    # a captured graph (what they decided would be replayed). The book takes one thread's call at a time, reading included.
     def set_page_pools(self, pools: Sequence[str], pages: int) -> None:
         """The runtime deals the pages from now on: `pools` are the caches (buffers of `pages` pages each, of any precision) that
         share set_paging's page table, page i of one belonging to page i of every other. Every slot is empty then. set_paging with
         another table or shape ends it. No counterpart in the reference, whose callers write the table."""
-        if self._paging is None:
-            raise RuntimeError("set_paging first")
-        names = list(pools)
-        if isinstance(pools, (str, bytes)) or len(set(names)) < len(names):
-            raise ValueError("pools are distinct buffer names")
-        if not 1 <= pages < 1 << 31:
-            raise ValueError("pages must be positive")
-        sizes = []
-        for name in names:
-            b = self._any_buffer(name)
-            n = b.kv4[3] if b.kv4 else b.n * b.elem
-            if n % pages:
-                raise ValueError(f"device buffer {name} is not {pages} pages of one size")
-            sizes.append(n // pages)
-        _, page, per_slot, slots = self._paging
-        self._pages = (PageBook(int(pages), page, per_slot, slots), dict(zip(names, sizes)))
+        with self._pages_lock:
+            if self._paging is None:
+                raise RuntimeError("set_paging first")
+            names = list(pools)
+            if isinstance(pools, (str, bytes)) or len(set(names)) < len(names):
+                raise ValueError("pools are distinct buffer names")
+            if not 1 <= pages < 1 << 31:
+                raise ValueError("pages must be positive")
+            sizes = []
+            for name in names:
+                b = self._any_buffer(name)
+                n = b.kv4[3] if b.kv4 else b.n * b.elem
+                if n % pages:
+                    raise ValueError(f"device buffer {name} is not {pages} pages of one size")
+                sizes.append(n // pages)
+            _, page, per_slot, slots = self._paging
+            self._pages = (PageBook(int(pages), page, per_slot, slots), dict(zip(names, sizes)))
 
     def _page_work(self, what: str, plan, *args) -> None:
         """PageBook's call plan(*args), then what it decided on the device. Called under the pages' lock."""
@@ -831,15 +833,17 @@ class Runtime:
 
     def pages_of(self, slot: int) -> list[int]:
         """The pages that a slot holds, in the order of its positions."""
-        if self._pages is None:
-            raise RuntimeError("set_page_pools first")
-        return self._pages[0].row(slot)
+        with self._pages_lock:
+            if self._pages is None:
+                raise RuntimeError("set_page_pools first")
+            return self._pages[0].row(slot)
 
     def pages_available(self) -> int:
         """Pages that no slot holds."""
-        if self._pages is None:
-            raise RuntimeError("set_page_pools first")
-        return self._pages[0].available()
+        with self._pages_lock:
+            if self._pages is None:
+                raise RuntimeError("set_page_pools first")
+            return self._pages[0].available()
 
     def set_segments(self, segments) -> int:
         """Row layout of the next *_seg ops: [(slot, pos0, rows[, row0]), ...], rows of a segment being
