@@ -89,6 +89,10 @@ class _Buffer:
     def look_again(self) -> None:
         self.ptr, self.n = self.address(), self.data.numel()
 
+    def made_as(self) -> tuple:
+        """What the places of its values follow from: a 4-bit cache's shape, else elements and their size."""
+        return self.kv4 or (self.n, self.elem)
+
 
 def _check_upload_args(name: str, nbytes_given: int, type_id: int, cols: int, rows: int) -> tuple[int, int]:
     """Validation of Runtime_upload (qwen_runtime.cu:1338-1357). Returns (row_bytes, nbytes)."""
@@ -176,7 +180,8 @@ class Runtime:
         self._segments: list[tuple[int, int, int, int]] = []
         self._seg_tables: list[tuple[ctypes.Array, int]] = []  # as int32 tables of one launch each
         self._seg_span = self._seg_longest = 0
-        self._pages: tuple[PageBook, dict[str, int]] | None = None  # the book, and bytes of a page of each pool
+        # The book, what each pool was when the book was made (_Buffer.made_as), and the bytes of a page of each.
+        self._pages: tuple[PageBook, dict[str, tuple], list[int]] | None = None
         self._pages_lock = threading.RLock()  # (a call's arguments may be an iterator that asks pages_of)
         # Resident-weight memory: an optional arena and the executor's per-layer weight groups. Nothing streams
         # over PCIe here, so the stream order only records which uploads were requested as streamed.
@@ -758,7 +763,7 @@ class Runtime:
     def set_page_pools(self, pools: Sequence[str], pages: int) -> None:
         """The runtime deals the pages from now on: `pools` are the caches (buffers of `pages` pages each, of any precision) that
         share set_paging's page table, page i of one belonging to page i of every other. Every slot is empty then. set_paging with
-        another table or shape ends it. No counterpart in the reference, whose callers write the table."""
+        another table or shape ends it, and a pool that is allocated anew keeps its size and precision. No counterpart in the reference, whose callers write the table."""
         with self._pages_lock:
             if self._paging is None:
                 raise RuntimeError("set_paging first")
@@ -767,34 +772,35 @@ class Runtime:
                 raise ValueError("pools are distinct buffer names")
             if not 1 <= pages < 1 << 31:
                 raise ValueError("pages must be positive")
-            sizes = []
+            sizes, made = [], {}
             for name in names:
                 b = self._any_buffer(name)
+                made[name] = b.made_as()
                 n = b.kv4[3] if b.kv4 else b.n * b.elem
                 if n % pages:
                     raise ValueError(f"device buffer {name} is not {pages} pages of one size")
                 sizes.append(n // pages)
             _, page, per_slot, slots = self._paging
-            self._pages = (PageBook(int(pages), page, per_slot, slots), dict(zip(names, sizes)))
+            self._pages = (PageBook(int(pages), page, per_slot, slots), made, sizes)
 
     def _page_work(self, what: str, plan, *args) -> None:
         """PageBook's call plan(*args), then what it decided on the device. Called under the pages' lock."""
         if self._pages is None or self._paging is None:
             raise RuntimeError("set_page_pools first")
-        book, pools = self._pages
+        book, pools, sizes = self._pages
         ptrs = []
-        for name, size in pools.items():
+        for name, made in pools.items():
             b = self.buffers.get(name)
             if b is None or b.lent:
                 b = self._any_buffer(name)
-            if b.n * b.elem < size * book.pages:
-                raise ValueError(f"device buffer {name} has {b.n * b.elem} bytes, need {size * book.pages}")
+            if b.made_as() != made or (b.kv4 and b.n < b.kv4[3]):
+                raise ValueError(f"device buffer {name} is another one than set_page_pools was given (set_page_pools again)")
             ptrs.append(b.ptr)
         table, _, _ = self._page_table()
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what}: page work cannot be captured")
         plan(book, *args)
-        book.apply(ptrs, pools.values(), table, self._stream())
+        book.apply(ptrs, sizes, table, self._stream())
 
     def pages_reserve(self, segments) -> None:
         """Make the rows that a pass is about to write ((slot, pos0, rows, ...) as in set_segments) the slot's own: pages that it
