@@ -69,3 +69,23 @@ def test_a_pool_in_another_storage_is_followed(rt, torch):
     with pytest.raises(ValueError):
         rt.pages_free([0])
     assert rt.pages_of(0) == [0, 1, 2]
+
+
+def test_a_table_in_a_smaller_storage_is_refused(rt, torch):
+    """A lent page table whose storage is exchanged for a smaller one: no entry is written or read behind it."""
+    for name in ("k", "v", "x", "o"):
+        rt.alloc(name, 2 * 2 * 32)
+    rt.set_segments([(0, 18, 2)])
+    t = rt.buffer_tensor("table")
+    held = t.data
+    t.data = torch.zeros(7, device="cuda")
+    for call in (lambda: rt.pages_fork(0, [1], 20), lambda: rt.pages_free([0]), lambda: rt.kv_append_seg("k", "v", "q", "q", 2, 32),
+                 lambda: rt.kv4_read_seg("q", "q", "k", "v", 2, 32), lambda: rt.attention_seg("x", "q", "q", "o", 2, 2, 32),
+                 lambda: rt.attention_seg("x", "h", "h", "o", 2, 2, 32)):
+        for _ in range(2):
+            with pytest.raises(ValueError):
+                call()
+    assert rt.pages_of(0) == [0, 1, 2] and rt.pages_of(1) == []
+    rt.buffer_tensor("table").data = held
+    rt.pages_fork(0, [1], 20)
+    assert rt.pages_of(1) == [0, 1, 2]

@@ -891,9 +891,11 @@ class Runtime:
 
     def _page_table(self) -> tuple[int, int, int]:
         """Address of the page table, page size and pages per sequence."""
-        pt, page, pps, _ = self._paging
+        pt, page, pps, slots = self._paging
         if pt.lent and pt.address() != pt.ptr:
             pt.look_again()
+        if pt.n < pps * slots:
+            raise ValueError(f"the page table has {pt.n} entries, need {pps * slots}")
         return pt.ptr, page, pps
 
     def _kv_pair(self, kc: str, vc: str, min_n: int) -> tuple[_Buffer, _Buffer]:
