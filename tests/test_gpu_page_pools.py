@@ -89,3 +89,11 @@ def test_a_table_in_a_smaller_storage_is_refused(rt, torch):
     rt.buffer_tensor("table").data = held
     rt.pages_fork(0, [1], 20)
     assert rt.pages_of(1) == [0, 1, 2]
+
+
+@pytest.mark.parametrize("blocks,positions,pages", [(10, 8, 4), (9, 8, 2), (4, 16, 4), (2, 8, 4)])
+def test_a_4_bit_pool_that_is_not_whole_pages_is_refused(rt, blocks, positions, pages):
+    """Its bytes may divide by the pages all the same: 10 blocks of 144 bytes make 4 times 360."""
+    rt.alloc_kv4("p", blocks, positions, 32)
+    with pytest.raises(ValueError):
+        rt.set_page_pools(["p"], pages)

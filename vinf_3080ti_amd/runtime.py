@@ -763,7 +763,8 @@ class Runtime:
     def set_page_pools(self, pools: Sequence[str], pages: int) -> None:
         """The runtime deals the pages from now on: `pools` are the caches (buffers of `pages` pages each, of any precision) that
         share set_paging's page table, page i of one belonging to page i of every other. Every slot is empty then. set_paging with
-        another table or shape ends it, and a pool that is allocated anew keeps its size and precision. No counterpart in the reference, whose callers write the table."""
+        another table or shape ends it, and a pool that is allocated anew keeps its size and precision. No counterpart in the
+        reference, whose callers write the table."""
         with self._pages_lock:
             if self._paging is None:
                 raise RuntimeError("set_paging first")
@@ -772,15 +773,16 @@ class Runtime:
                 raise ValueError("pools are distinct buffer names")
             if not 1 <= pages < 1 << 31:
                 raise ValueError("pages must be positive")
+            _, page, per_slot, slots = self._paging
             sizes, made = [], {}
             for name in names:
                 b = self._any_buffer(name)
                 made[name] = b.made_as()
                 n = b.kv4[3] if b.kv4 else b.n * b.elem
-                if n % pages:
+                # (A page of a 4-bit pool is whole blocks of its positions.)
+                if n % pages or (b.kv4 and (b.kv4[0] % pages or b.kv4[1] != page)):
                     raise ValueError(f"device buffer {name} is not {pages} pages of one size")
                 sizes.append(n // pages)
-            _, page, per_slot, slots = self._paging
             self._pages = (PageBook(int(pages), page, per_slot, slots), made, sizes)
 
     def _page_work(self, what: str, plan, *args) -> None:
