@@ -314,14 +314,16 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerArgs a, VerTab
                 __syncthreads();
                 continue;
             }
-            // The first chunk whose cumulative sum exceeds the target, else the last with any weight.
+            // The first chunk whose cumulative sum exceeds the target, else the last with any weight. One without weight is never
+            // taken: a thread's `before` is the scan less its own share, which may round past the target where the thread before
+            // ended at it.
             const double target = v * total;
             double before = upto - mine, mine_base = 0.0;
             int found = INT_MAX, some_at = -1;
             for (int c = c0; c < c1; ++c) {
                 const double w = of_chunk(c);
                 if (w > 0.0) some_at = c;
-                if (before + w > target) {
+                if (w > 0.0 && before + w > target) {
                     found = c, mine_base = before;
                     break;
                 }
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerArgs a, VerTab
             for (int e = 0; e < kEach; ++e) {
                 if (w[e] > 0.0) some_at = e0 + e;
                 before += w[e];
-                if (before > target && found == INT_MAX) found = e0 + e;
+                if (w[e] > 0.0 && before > target && found == INT_MAX) found = e0 + e;
             }
             const int2 el = group_span(found, some_at, span);
             if (tid == 0) token = !none && el.x != INT_MAX ? el.x : el.y >= 0 ? el.y : chunk * kChunk;
