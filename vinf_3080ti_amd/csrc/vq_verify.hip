@@ -47,9 +47,10 @@ struct VerArgs {
 
 // A logit as it counts: NaN never wins, like -inf.
 __device__ __forceinline__ float logit(float x) { return x == x ? x : -INFINITY; }
-// 2^x for x <= 0: x = n + f with |f| <= 1/2, the Taylor polynomial of degree 12 in f ln 2 (the rest is below 2^-53), times 2^n. Below
-// -1100 the result is 0 anyway. The math library's exp, which also serves x > 0 and NaN, takes twice the instructions, and they are
-// as many as hide behind the logits' loads: see verify_stats_kernel.
+// 2^x for x <= 0: x = n + f with |f| <= 1/2, the Taylor polynomial of degree 12 in f ln 2, times 2^n. What it leaves out is at most
+// (ln 2 / 2)^13 / 13! = 1.7e-16, 2.4e-16 of 2^f at f = -1/2, as much as the roundings of the evaluation. Below -1100 the result is 0
+// anyway. The math library's exp, which also serves x > 0 and NaN, takes twice the instructions, and they are as many as hide behind
+// the logits' loads: see verify_stats_kernel.
 __device__ __forceinline__ double exp2_neg(double x) {
     constexpr double L = 0.6931471805599453;
     x = fmax(x, -1100.0);
