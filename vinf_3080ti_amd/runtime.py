@@ -17,6 +17,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import numbers
 import threading
 import types
 from dataclasses import dataclass
@@ -1202,7 +1203,7 @@ class Runtime:
         ks = [int(k) for k in drafted]
         if not ks or vocab < 1 or any(not 0 <= k <= _lib.VQ_MAX_DRAFT for k in ks):
             raise ValueError(f"drafted must give 0 to {_lib.VQ_MAX_DRAFT} tokens for each sequence, of a positive vocab")
-        ts = [float(temperature)] * len(ks) if isinstance(temperature, (int, float)) else [float(t) for t in temperature]
+        ts = [float(temperature)] * len(ks) if isinstance(temperature, numbers.Real) else [float(t) for t in temperature]
         if len(ts) != len(ks) or any(not 0.0 <= t < math.inf for t in ts):
             raise ValueError("temperature must be one finite number >= 0, or one for each sequence")
         total = sum(ks)
