@@ -89,10 +89,8 @@ class _Buffer:
 
     def look_again(self) -> None:
         self.ptr, self.n = self.address(), self.data.numel()
-
-    def made_as(self) -> tuple:
-        """What the places of its values follow from: a 4-bit cache's shape, else elements and their size."""
-        return self.kv4 or (self.n, self.elem)
+        # What the places of its values follow from: a 4-bit cache's shape (while all of it is there), else elements and their size.
+        self.made = self.kv4 if self.kv4 and self.n >= self.kv4[3] else (self.n, self.elem)
 
 
 def _check_upload_args(name: str, nbytes_given: int, type_id: int, cols: int, rows: int) -> tuple[int, int]:
@@ -181,7 +179,7 @@ class Runtime:
         self._segments: list[tuple[int, int, int, int]] = []
         self._seg_tables: list[tuple[ctypes.Array, int]] = []  # as int32 tables of one launch each
         self._seg_span = self._seg_longest = 0
-        # The book, what each pool was when the book was made (_Buffer.made_as), and the bytes of a page of each.
+        # The book, what each pool was when the book was made (_Buffer.made), and the bytes of a page of each.
         self._pages: tuple[PageBook, dict[str, tuple], list[int]] | None = None
         self._pages_lock = threading.RLock()  # (a call's arguments may be an iterator that asks pages_of)
         # Resident-weight memory: an optional arena and the executor's per-layer weight groups. Nothing streams
@@ -778,7 +776,7 @@ class Runtime:
             sizes, made = [], {}
             for name in names:
                 b = self._any_buffer(name)
-                made[name] = b.made_as()
+                made[name] = b.made
                 n = b.kv4[3] if b.kv4 else b.n * b.elem
                 # (A page of a 4-bit pool is whole blocks of its positions.)
                 if n % pages or (b.kv4 and (b.kv4[0] % pages or b.kv4[1] != page)):
@@ -796,7 +794,7 @@ class Runtime:
             b = self.buffers.get(name)
             if b is None or b.lent:
                 b = self._any_buffer(name)
-            if b.made_as() != made or (b.kv4 and b.n < b.kv4[3]):
+            if b.made != made:
                 raise ValueError(f"device buffer {name} is another one than set_page_pools was given (set_page_pools again)")
             ptrs.append(b.ptr)
         table, _, _ = self._page_table()
