@@ -1055,7 +1055,8 @@ __global__ __launch_bounds__(256, 2) void attention4_kernel(const float *__restr
     const int bases = C.base[lane];
     // The first workgroups, one to a CU, are joined by those past 256. Where that leaves some CUs with one, it is a prompt's longest
     // groups that are alone: the first and the last of the launch take the end of the list, which holds the shorter ones. 512 rows
-    // over 2048 keys: 70.4 instead of 72.1 us, 480 over 480: 21.4 and 23.4.
+    // over 2048 keys: 70.4 instead of 72.1 us, 480 over 480: 21.4 and 23.4. With several prompts the end of the list holds shorter and
+    // longer ones: 256 and 256 rows over 2048 keys take 69 us either way, 300 and 300 over 800 34.0 and 34.3 with it.
     int unit = blockIdx.x;
     if (VECS != 16 && T.n == 1 && gridDim.x > 256 && gridDim.x < 512) {
         const int twice = gridDim.x - 256;
@@ -1378,7 +1379,8 @@ bool fits(const SegTable &T, int heads) {
 }
 // Chunks for the 512 workgroups that run at once (two per CU): of the lengths that make one to four full rounds, and of whole
 // contexts, the one with the least rounds x (keys of a chunk + what a chunk costs besides, in keys: its start and end, 160 keys' time,
-// and with more than one chunk the partial results of a group, 100 for each tile).
+// and with more than one chunk the partial results of a group, 100 for each tile). Both were found at hd 256; half and twice as much
+// change decode, verification and 16 rows of a prompt at hd 64, 96, 128 and 256 by 3 % at most, mostly by less than 1.
 struct Shape {
     int heads, kv_heads, vecs;
     int groups(const Seg &s) const { return (s.rows * (heads / kv_heads) + vecs - 1) / vecs; }

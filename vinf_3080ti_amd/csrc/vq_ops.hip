@@ -320,7 +320,6 @@ __global__ __launch_bounds__(64 * kAttnWaves) void attention_kernel(const float 
 // accumulation throughout. Visibility rules of attention_kernel.
 constexpr int kFaKeys = 32;  // keys per LDS tile
 
-
 // The keys [k_lo, k_hi) of kv head kvh of a sequence, 32 per LDS tile (all four waves stage each tile; fp16 caches
 // widened to fp32), against the 16 query vectors a wave holds in qf (query vector col = lane & 15 sees keys
 // [qs, qe)). Updates the online softmax (m, l) and the unnormalised output o of the lane's query vector.

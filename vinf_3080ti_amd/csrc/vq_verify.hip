@@ -133,8 +133,9 @@ __device__ __forceinline__ int2 group_span(int lo, int hi, int2 *lds) {
 
 // Workgroup (chunk, row of a sequence, sequence): (maximum, sum of weights against it), for a greedy row (maximum, its lowest index).
 // Bound by the logits' bytes and by the weights' 22 instructions of 64 bits a logit, nearly equally: 64 rows of 248320 are 64 MB, 12.5
-// us at the rate of a copy, and 9 us of instructions; this takes 19 (22 with an exp of 27 instructions). Workgroups of several chunks that load one while they compute
-// with the one before take longer (4 chunks: 24 us): many workgroups at different points overlap the two better.
+// us at the rate of a copy, and 9 us of instructions; this takes 19 (22 with an exp of 27 instructions). Workgroups of several chunks
+// that load one while they compute with the one before take longer (4 chunks: 24 us): many workgroups at different points overlap the
+// two better.
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerArgs a, VerTable T) {
     __shared__ float smax[4];
     __shared__ double ssum[4];
