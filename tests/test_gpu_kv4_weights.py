@@ -63,3 +63,37 @@ def test_one_dominant_key(rt, oracle_mod, heads, kvh, hd, ntok, sink, gap):
         rt.attention("q", "kc", "vc", "o", heads, kvh, hd, n, n - ntok + 1, ntok)
         off = np.abs(get(rt, "o", q.shape) - want)
         assert (off <= rel[..., None] * want + floor).all(), (off / want).max()
+
+
+@pytest.mark.parametrize("heads,kvh,hd", [(24, 4, 256), (32, 8, 128), (8, 2, 64), (6, 2, 96)])
+@pytest.mark.parametrize("ntok", [1, 40])
+@pytest.mark.parametrize("power", [20, 22, 24, 26, 28, 40, 80])
+def test_scores_whose_roundings_are_large(rt, oracle_mod, heads, kvh, hd, ntok, power):
+    """Scores near 2^power, whose differences are far beyond their fp32 roundings and beyond what exp holds: the keys of the largest one
+    share all of the softmax. Off by a rounding for each of them, in numerator and denominator, and for 16 joins and the pairs."""
+    n = 700
+    rng = np.random.default_rng(power + ntok)
+    k = np.zeros((n, kvh, hd), np.float32)
+    k[:, :, 0] = rng.permuted(np.repeat(np.arange(1.0, n + 1)[:, None], kvh, 1), axis=0)
+    v = rng.standard_normal((n, kvh, hd)).astype(np.float32)
+    caches(rt, kvh, n, hd)
+    put(rt, "k", k)
+    put(rt, "v", v)
+    rt.kv_append("k", "v", "kc", "vc", kvh, n, hd, 0, n)
+    wk, wv = (x.transpose(1, 0, 2) for x in oracle_mod.kv4_values(k, v))
+    q = np.zeros((ntok, heads, hd), np.float32)
+    q[..., 0] = 2.0 ** power * np.sqrt(hd) / n * rng.uniform(0.7, 1, (ntok, heads))
+    put(rt, "q", q)
+    kv = np.arange(heads) * kvh // heads
+    for invariant in (False, True):
+        rt.set_batch_invariant(invariant)
+        put(rt, "o", np.zeros(q.size))
+        rt.attention("q", "kc", "vc", "o", heads, kvh, hd, n, n - ntok + 1, ntok)
+        got = get(rt, "o", q.shape)
+        for t in range(ntok):
+            sees = wk[kv, : n - ntok + 1 + t, 0]
+            best = sees.max(1, keepdims=True)
+            top = [np.flatnonzero(row == b[0]) for row, b in zip(sees, best)]
+            want = np.stack([wv[h, i].mean(0) for h, i in zip(kv, top)])
+            most = np.stack([np.abs(wv[h, i]).max(0) for h, i in zip(kv, top)])
+            assert (np.abs(got[t] - want) <= most * (len(max(top, key=len)) + 16) * 2.0 ** -23).all(), (t, np.abs(got[t] - want).max())

@@ -382,10 +382,23 @@ __device__ __forceinline__ float softmax_step(const float (&v)[N], float unit, f
     bm = max_across(bm) * unit;
     const float mn = bm > m + kMost ? bm - kLift : m, ms = mn == -INFINITY ? 0.0f : mn;  // ms: exp2(-inf - ms) is 0 also before any key
     const float alpha = __builtin_amdgcn_exp2f(m - ms);
-    float ps = 0.0f;
+    float x[N], ps = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = fmaf(v[j], unit, -ms);
+    // Past 2^21 the roundings of bm and m would show: an exponent could come to 16, an infinite f16, or the largest key's weight to
+    // nothing. There products are rounded as bm was, which leaves the largest one an exponent of 0 or more, and exponents end at 15.
+    const bool far = fabsf(mn) > 0x1p21f;
+    if (__any(far)) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float y = v[j] * unit - ms;
+            x[j] = far ? (y > kMost ? kMost : y) : x[j];  // (NaN stays)
+        }
+    }
 #pragma unroll
     for (int j = 0; j < N; j += 2) {
-        const ff2 w{__builtin_amdgcn_exp2f(fmaf(v[j], unit, -ms)), __builtin_amdgcn_exp2f(fmaf(v[j + 1], unit, -ms))};
+        const ff2 w{__builtin_amdgcn_exp2f(x[j]), __builtin_amdgcn_exp2f(x[j + 1])};
         ps += w[0];
         ps += w[1];
         const fh2 hi = __builtin_convertvector(w, fh2);
